@@ -9,7 +9,8 @@
  *     (a hipStream_t passed as void*; NULL = the null stream);
  *   - tensors are dense row-major with the innermost dimension contiguous;
  *   - every tensor, weight vector and workspace starts on a 16-byte boundary
- *     (the kernels move 16 bytes per access); a pointer off it is VIG_EINVAL;
+ *     (the kernels move 16 bytes per access); a pointer off it is VIG_EINVAL
+ *     (the gated scan and the update of many tensors take any element);
  *   - return value: 0 on success, a negative VIG_E* code otherwise
  *     (vig_gla_strerror() gives the text); a failed call enqueues nothing;
  *   - dtype codes: VIG_F32 = 0, VIG_BF16 = 1.
@@ -799,6 +800,75 @@ int vig_linear_bwd_weight_many_later(const void* const* dy, const long long* dy_
                                const long long* x_row_stride, float* const* dweight, float* const* dbias, void* workspace,
                                size_t workspace_bytes, long long rows, const int* N, const int* K, int count, vig_sum_jobs* later, void* stream);
 int vig_sum_jobs_run(vig_sum_jobs* jobs, void* stream);
+
+/*
+ * Gated linear recurrence of a vector state, the op above with one number a channel for the Dk x Dv state:
+ *
+ *   h_t  = exp(g_fwd_t) h_{t-1} + x_t      (t = 0..L-1, from initial_state or 0)
+ *   h'_t = exp(g_bwd_t) h'_{t+1} + x_t     (t = L-1..0, from 0)
+ *   o_t  = out_scale * (h_t + h'_t)        (g_bwd == NULL: h_t alone, the causal op)
+ *
+ * x, g_fwd, g_bwd [B, L, D] (types io_dtype, gate_dtype), o [B, L, D] dense, of io_dtype.  g_* are natural-log decays (<= 0); -infinity
+ * lets nothing through (a sequence packed behind another starts with it in g_fwd, and ends with it in g_bwd), and a token of
+ * x = 0, g = 0 changes nothing (padding).  A value that is not finite makes every later output of its channel so, whatever the gates.
+ * States are fp32 [B, D], of the causal op only: initial_state (NULL: zeros) and final_state (NULL: not wanted), the state
+ * behind the last token.
+ * x_strides, g_strides: elements between batch elements and between tokens, e.g. of the columns of a projection's rows
+ * (NULL: dense); both gate tensors lie alike.  Tensors begin on any element (the exception to the 16-byte rule, as those of the update
+ * below are; the workspace keeps it).  Any B, L >= 1 and D >= 1 with D and the token strides up to 524288 and L up to 2^30; four channels
+ * move at once where D, the strides and the addresses are whole quads of elements.  Sums and states are held in fp32 and their order is fixed.
+ * Outputs may not overlap inputs.  `workspace`: vig_gated_scan_fwd_workspace(...) bytes (0: may be NULL).
+ */
+size_t vig_gated_scan_fwd_workspace(int B, int L, int D, int both);
+int vig_gated_scan_fwd(const void* x, const void* g_fwd, const void* g_bwd, const float* initial_state, void* o, float* final_state,
+                       void* workspace, size_t workspace_bytes, int B, int L, int D, const long long* x_strides,
+                       const long long* g_strides, float out_scale, int io_dtype, int gate_dtype, void* stream);
+/*
+ * Its gradients: d_o [B, L, D] dense of io_dtype -> dx (io_dtype), dg_fwd, dg_bwd (gate_dtype; dg_bwd NULL exactly where g_bwd is), dense,
+ * and for the causal op d_final_state (NULL: zeros) -> d_initial_state (NULL: not wanted), fp32 [B, D].  The states are
+ * computed again from x and the gates in fp32.
+ */
+size_t vig_gated_scan_bwd_workspace(int B, int L, int D, int both);
+int vig_gated_scan_bwd(const void* x, const void* g_fwd, const void* g_bwd, const float* initial_state, const void* d_o,
+                       const float* d_final_state, void* dx, void* dg_fwd, void* dg_bwd, float* d_initial_state, void* workspace,
+                       size_t workspace_bytes, int B, int L, int D, const long long* x_strides, const long long* g_strides,
+                       float out_scale, int io_dtype, int gate_dtype, void* stream);
+/*
+ * One token of each of B sequences: state <- exp(g) state + x, o = state.  x, g [B, D] with rows x_stride, g_stride elements
+ * apart (0 = packed), state fp32 [B, D], o [B, D] of io_dtype.  B * D < 2^31 - 256.
+ */
+int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int B, int D, long long x_stride, long long g_stride,
+                        int io_dtype, int gate_dtype, void* stream);
+
+/*
+ * One AdamW step over `count` tensors, in place:
+ *
+ *   g' = *grad_scale g;  m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2
+ *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *
+ * param[j], grad[j]: n[j] elements of param_dtype[j], grad_dtype[j], beginning on any element (the exception to the 16-byte rule).
+ * t = *step_on_device or, where that is NULL, step >= 1; lr likewise *lr_on_device or lr.  grad_scale NULL: 1; a NaN there leaves every tensor as it is.
+ * state_bits 32: exp_avg = m and exp_avg_sq = v in fp32 (avg_scale, sq_scale are not read).
+ * state_bits 8: m and r = sqrt(v) as e4m3 values times a scale for each 256 elements of a tensor (avg_scale[j], sq_scale[j]:
+ * ceil(n[j] / 256) floats, the block's largest magnitude / 448).  A block that takes in a value that is not finite is NaN from then on.
+ * States in 8 bits and bf16 parameters are rounded stochastically.  The element's word: w = mix(number ^ key), number = 256 * (blocks of 256 of
+ * the tensors in front) + element (its bits past 32 times 0x9E3779B9 are added to the key), key = mix(mix(mix(seed) + (seed >> 32)) + t) in
+ * 32-bit words, mix(x): x ^= x >> 16, x *= 0x6A09E667, x ^= x >> 15, x *= 0xBB67AE85, x ^= x >> 16.  m is rounded up in magnitude where the lower half of w
+ * reaches past what the step lacks, r by the upper half (never from above 0 to 0), a bf16 parameter by the upper half of 0x9E3779B9 w.
+ * Tensors that are written may not overlap one another or a gradient (VIG_EINVAL).  Up to 2^40 elements in all.
+ */
+int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq, float* const* avg_scale,
+                   float* const* sq_scale, const long long* n, const int* param_dtype, const int* grad_dtype, int count, int state_bits,
+                   double lr, double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,
+                   const long long* step_on_device, const float* grad_scale, unsigned long long seed, void* stream);
+/*
+ * norm[0] = sqrt of the sum of squares of all elements of `count` tensors (added up in fp64, in a fixed order), and, where `scale` is not NULL,
+ * scale[0] = min(1, max_norm / (norm + 1e-6)), NaN where the norm is not finite: what vig_adamw_many takes as grad_scale.
+ * Tensors begin on any element.
+ */
+size_t vig_grad_norm_workspace(const long long* n, int count);
+int vig_grad_norm(const void* const* grad, const long long* n, const int* dtype, int count, float max_norm, float* norm, float* scale,
+                  void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

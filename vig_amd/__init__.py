@@ -6,16 +6,21 @@ interfaces over it.
 """
 from . import ops  # noqa: F401
 from .ops import (  # noqa: F401
+    adamw_step,
     batch_bid_fused_chunk_gla,
     bid_fused_recurrent_gla,
+    bid_gated_scan,
     dirgate,
     dwconv3x3,
     fused_chunk_gla,
     fused_recurrent_gla,
+    gated_scan,
+    gated_scan_step,
     gla_bidir_backward,
     gla_bidir_forward,
     gla_causal_state_forward,
     gla_bidir_locality_gate,
+    grad_norm,
     locality_blend,
     locality_gate,
     rmsnorm,
@@ -24,6 +29,7 @@ from .ops import (  # noqa: F401
 )
 
 __all__ = [
+    "adamw_step", "bid_gated_scan", "gated_scan", "gated_scan_step", "grad_norm",
     "batch_bid_fused_chunk_gla", "bid_fused_recurrent_gla", "dirgate", "dwconv3x3", "fused_chunk_gla",
     "fused_recurrent_gla", "gla_bidir_backward", "gla_bidir_forward", "gla_causal_state_forward", "gla_bidir_locality_gate", "locality_blend", "locality_gate", "rmsnorm", "split_heads", "swiglu",
 ]

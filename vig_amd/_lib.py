@@ -17,6 +17,7 @@ VIG_OK, VIG_EINVAL, VIG_ENOTSUP, VIG_ENOSPC, VIG_ELAUNCH = 0, -22, -95, -28, -5 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_float = ctypes.c_float
+_c_double = ctypes.c_double
 _c_size_t = ctypes.c_size_t
 _c_longlong = ctypes.c_longlong
 
@@ -116,6 +117,14 @@ SIGNATURES = {
     "vig_stem_norm_bwd_workspace": (_c_size_t, [_c_longlong, _c_int]),
     "vig_stem_norm_bwd": (_c_int, [_c_void_p] * 8 + [_c_size_t, _c_longlong, _c_int, _c_float, _c_int, _c_int, _c_int, _c_void_p]),
     "vig_sum_jobs_run": (_c_int, [_c_void_p, _c_void_p]),
+    "vig_gated_scan_fwd_workspace": (_c_size_t, [_c_int] * 4),
+    "vig_gated_scan_fwd": (_c_int, [_c_void_p] * 7 + [_c_size_t] + [_c_int] * 3 + [_c_void_p] * 2 + [_c_float, _c_int, _c_int, _c_void_p]),
+    "vig_gated_scan_bwd_workspace": (_c_size_t, [_c_int] * 4),
+    "vig_gated_scan_bwd": (_c_int, [_c_void_p] * 11 + [_c_size_t] + [_c_int] * 3 + [_c_void_p] * 2 + [_c_float, _c_int, _c_int, _c_void_p]),
+    "vig_gated_scan_step": (_c_int, [_c_void_p] * 4 + [_c_int] * 2 + [_c_longlong] * 2 + [_c_int] * 2 + [_c_void_p]),
+    "vig_adamw_many": (_c_int, [_c_void_p] * 9 + [_c_int] * 2 + [_c_double] * 5 + [_c_longlong] + [_c_void_p] * 3 + [ctypes.c_ulonglong, _c_void_p]),
+    "vig_grad_norm_workspace": (_c_size_t, [_c_void_p, _c_int]),
+    "vig_grad_norm": (_c_int, [_c_void_p] * 3 + [_c_int, _c_float] + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),
 }
 
 _lib = None

@@ -4,6 +4,7 @@
 #include "launch.h"
 #include <algorithm>
 #include <mutex>
+#include <vector>
 
 namespace vig {
 int launch_dirgate(const void* in, void* out, int B, int L, int H, int Dk, float inv_norm, float clamp_min,
@@ -105,6 +106,58 @@ static bool room_for(const vig_sum_jobs* later, int n) { return !later || (later
 template <typename... P>
 static bool aligned16(P... p) {
   return ((reinterpret_cast<uintptr_t>(static_cast<const void*>(p)) % 16 == 0) && ...);
+}
+static int element_size(int dtype) { return dtype == VIG_BF16 ? 2 : 4; }
+static bool on_element(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+static bool scan_sizes_ok(int B, int L, int D) { return B > 0 && L > 0 && D > 0 && L <= (1 << 30) && D <= vig::kScanRow; }
+// The arguments that the gated scan and its backward share: checked and put into `s`.
+static int scan_arguments(vig::GatedScan& s, void* workspace, int B, int L, int D, const long long* x_strides, const long long* g_strides, float out_scale,
+                          int io_dtype, int gate_dtype) {
+  if (!s.x || !s.g_fwd || B <= 0 || L <= 0 || D <= 0 || (s.g_bwd && (s.initial || s.final))) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !dtype_ok(gate_dtype) || !scan_sizes_ok(B, L, D)) return VIG_ENOTSUP;
+  for (const void* p : {s.x, s.d_o, (const void*)s.o, (const void*)s.dx})
+    if (!on_element(p, element_size(io_dtype))) return VIG_EINVAL;
+  for (const void* p : {s.g_fwd, s.g_bwd, (const void*)s.dg_fwd, (const void*)s.dg_bwd})
+    if (!on_element(p, element_size(gate_dtype))) return VIG_EINVAL;
+  for (const float* p : {s.initial, s.d_final, (const float*)s.final, (const float*)s.d_initial})
+    if (!on_element(p, 4)) return VIG_EINVAL;
+  if (!aligned16(workspace)) return VIG_EINVAL;
+  for (int i = 0; i < 2; ++i) {
+    const long long* from = i ? g_strides : x_strides;
+    long long* to = i ? s.g_strides : s.x_strides;
+    to[0] = from ? from[0] : (long long)L * D, to[1] = from ? from[1] : D;
+    if (to[0] < 0 || to[1] < D) return VIG_EINVAL;
+    if (to[1] > vig::kScanRow) return VIG_ENOTSUP;
+  }
+  s.B = B, s.L = L, s.D = D, s.out_scale = out_scale, s.io_dtype = io_dtype, s.gate_dtype = gate_dtype, s.workspace = workspace;
+  return VIG_OK;
+}
+
+// Whether the tensors that an update writes overlap none of its others (gradients may overlap one another).
+static bool apart(const vig::AdamW& a) {
+  struct Range {
+    uintptr_t from, to;
+    bool written;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve((size_t)a.count * (a.state_bits == 8 ? 6 : 4));
+  for (int j = 0; j < a.count; ++j) {
+    const uintptr_t n = (uintptr_t)a.n[j];
+    if (!n) continue;
+    auto add = [&](const void* p, uintptr_t bytes, bool written) { ranges.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written}); };
+    const uintptr_t state = a.state_bits == 8 ? n : 4 * n;
+    add(a.param[j], n * element_size(a.param_dtype[j]), true), add(a.grad[j], n * element_size(a.grad_dtype[j]), false);
+    add(a.exp_avg[j], state, true), add(a.exp_avg_sq[j], state, true);
+    if (a.state_bits == 8) add(a.avg_scale[j], (n + 255) / 256 * 4, true), add(a.sq_scale[j], (n + 255) / 256 * 4, true);
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.from < y.from; });
+  uintptr_t written = 0, any = 0;  // how far the ranges so far reach
+  for (const Range& r : ranges) {
+    if (r.from < written || (r.written && r.from < any)) return false;
+    any = std::max(any, r.to);
+    if (r.written) written = std::max(written, r.to);
+  }
+  return true;
 }
 static bool dk_ok(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
 static bool dv_ok(int d) { return d == 32 || d == 64 || d == 128; }
@@ -1068,6 +1121,105 @@ int vig_sum_jobs_run(vig_sum_jobs* jobs, void* stream) {
   const int rc = vig::launch_sum_jobs(*jobs, (hipStream_t)stream);
   if (rc == VIG_OK) jobs->count = 0;
   return rc;
+}
+
+size_t vig_gated_scan_fwd_workspace(int B, int L, int D, int both) {
+  return scan_sizes_ok(B, L, D) ? vig::gated_scan_workspace(B, L, D, both != 0, false) : 0;
+}
+
+size_t vig_gated_scan_bwd_workspace(int B, int L, int D, int both) {
+  return scan_sizes_ok(B, L, D) ? vig::gated_scan_workspace(B, L, D, both != 0, true) : 0;
+}
+
+int vig_gated_scan_fwd(const void* x, const void* g_fwd, const void* g_bwd, const float* initial_state, void* o, float* final_state, void* workspace,
+                       size_t workspace_bytes, int B, int L, int D, const long long* x_strides, const long long* g_strides, float out_scale, int io_dtype,
+                       int gate_dtype, void* stream) {
+  vig::GatedScan s{};
+  s.x = x, s.g_fwd = g_fwd, s.g_bwd = g_bwd, s.initial = initial_state, s.o = o, s.final = final_state;
+  if (!o || o == x || o == g_fwd || o == g_bwd || (final_state && final_state == initial_state)) return VIG_EINVAL;
+  const int rc = scan_arguments(s, workspace, B, L, D, x_strides, g_strides, out_scale, io_dtype, gate_dtype);
+  if (rc != VIG_OK) return rc;
+  const size_t need = vig::gated_scan_workspace(B, L, D, g_bwd != nullptr, false);
+  if (need && (!workspace || workspace_bytes < need)) return VIG_ENOSPC;
+  return vig::launch_gated_scan(s, (hipStream_t)stream);
+}
+
+int vig_gated_scan_bwd(const void* x, const void* g_fwd, const void* g_bwd, const float* initial_state, const void* d_o, const float* d_final_state,
+                       void* dx, void* dg_fwd, void* dg_bwd, float* d_initial_state, void* workspace, size_t workspace_bytes, int B, int L, int D,
+                       const long long* x_strides, const long long* g_strides, float out_scale, int io_dtype, int gate_dtype, void* stream) {
+  vig::GatedScan s{};
+  s.x = x, s.g_fwd = g_fwd, s.g_bwd = g_bwd, s.initial = initial_state, s.d_o = d_o, s.d_final = d_final_state;
+  s.dx = dx, s.dg_fwd = dg_fwd, s.dg_bwd = dg_bwd, s.d_initial = d_initial_state;
+  if (!d_o || !dx || !dg_fwd || !dg_bwd != !g_bwd || (g_bwd && (d_final_state || d_initial_state))) return VIG_EINVAL;
+  for (const void* out : {(const void*)dx, (const void*)dg_fwd, (const void*)dg_bwd})
+    if (out && (out == x || out == g_fwd || out == g_bwd || out == d_o)) return VIG_EINVAL;
+  if (dx == dg_fwd || dx == dg_bwd || dg_fwd == dg_bwd) return VIG_EINVAL;
+  if (d_initial_state && (d_initial_state == d_final_state || d_initial_state == initial_state)) return VIG_EINVAL;
+  const int rc = scan_arguments(s, workspace, B, L, D, x_strides, g_strides, out_scale, io_dtype, gate_dtype);
+  if (rc != VIG_OK) return rc;
+  const size_t need = vig::gated_scan_workspace(B, L, D, g_bwd != nullptr, true);
+  if (need && (!workspace || workspace_bytes < need)) return VIG_ENOSPC;
+  return vig::launch_gated_scan(s, (hipStream_t)stream);
+}
+
+int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int B, int D, long long x_stride, long long g_stride, int io_dtype,
+                        int gate_dtype, void* stream) {
+  if (!x || !g || !state || !o || B <= 0 || D <= 0) return VIG_EINVAL;
+  if (x_stride == 0) x_stride = D;
+  if (g_stride == 0) g_stride = D;
+  if (x_stride < D || g_stride < D || o == x || o == g || o == state || state == x || state == g) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !dtype_ok(gate_dtype)) return VIG_ENOTSUP;
+  if (!on_element(x, element_size(io_dtype)) || !on_element(o, element_size(io_dtype)) || !on_element(g, element_size(gate_dtype)) || !on_element(state, 4))
+    return VIG_EINVAL;
+  return vig::launch_gated_scan_step({x, g, state, o, B, D, x_stride, g_stride, io_dtype, gate_dtype}, (hipStream_t)stream);
+}
+
+int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq, float* const* avg_scale,
+                   float* const* sq_scale, const long long* n, const int* param_dtype, const int* grad_dtype, int count, int state_bits, double lr,
+                   double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,
+                   const long long* step_on_device, const float* grad_scale, unsigned long long seed, void* stream) {
+  if (!param || !grad || !exp_avg || !exp_avg_sq || !n || !param_dtype || !grad_dtype || count <= 0) return VIG_EINVAL;
+  if (state_bits != 8 && state_bits != 32) return VIG_ENOTSUP;
+  const bool bits8 = state_bits == 8;
+  if (bits8 && (!avg_scale || !sq_scale)) return VIG_EINVAL;
+  // (written so that a NaN is refused too)
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0) || (!step_on_device && step < 1)) return VIG_EINVAL;
+  if (!on_element(lr_on_device, 4) || !on_element(step_on_device, 8) || !on_element(grad_scale, 4)) return VIG_EINVAL;
+  long long blocks = 0;
+  for (int j = 0; j < count; ++j) {
+    if (!dtype_ok(param_dtype[j]) || !dtype_ok(grad_dtype[j])) return VIG_ENOTSUP;
+    if (n[j] < 0) return VIG_EINVAL;
+    if (n[j] > vig::kUpdateElements || (blocks += (n[j] + 255) / 256) > vig::kUpdateElements / 256) return VIG_ENOTSUP;
+    if (n[j] == 0) continue;
+    if (!param[j] || !grad[j] || !exp_avg[j] || !exp_avg_sq[j] || (bits8 && (!avg_scale[j] || !sq_scale[j]))) return VIG_EINVAL;
+    if (!on_element(param[j], element_size(param_dtype[j])) || !on_element(grad[j], element_size(grad_dtype[j]))) return VIG_EINVAL;
+    if (!bits8 && (!on_element(exp_avg[j], 4) || !on_element(exp_avg_sq[j], 4))) return VIG_EINVAL;
+    if (bits8 && (!on_element(avg_scale[j], 4) || !on_element(sq_scale[j], 4))) return VIG_EINVAL;
+  }
+  const vig::AdamW a{param, grad, exp_avg, exp_avg_sq, avg_scale, sq_scale, n, param_dtype, grad_dtype, count, state_bits, lr, beta1, beta2, eps, weight_decay, step,
+                     lr_on_device, step_on_device, grad_scale, seed};
+  try {
+    if (!apart(a)) return VIG_EINVAL;
+  } catch (...) {  // (no memory for the list of ranges)
+    return VIG_ENOSPC;
+  }
+  return vig::launch_adamw(a, (hipStream_t)stream);
+}
+
+size_t vig_grad_norm_workspace(const long long* n, int count) { return n && count > 0 ? vig::grad_norm_workspace(n, count) : 0; }
+
+int vig_grad_norm(const void* const* grad, const long long* n, const int* dtype, int count, float max_norm, float* norm, float* scale, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  if (!grad || !n || !dtype || !norm || count <= 0 || norm == scale || (scale && !(max_norm >= 0.f))) return VIG_EINVAL;
+  if (!on_element(norm, 4) || !on_element(scale, 4) || !on_element(workspace, 8)) return VIG_EINVAL;
+  long long elements = 0;
+  for (int j = 0; j < count; ++j) {
+    if (!dtype_ok(dtype[j])) return VIG_ENOTSUP;
+    if (n[j] < 0 || (n[j] > 0 && (!grad[j] || !on_element(grad[j], element_size(dtype[j]))))) return VIG_EINVAL;
+    if (n[j] > vig::kUpdateElements || (elements += n[j]) > vig::kUpdateElements) return VIG_ENOTSUP;
+  }
+  if (!workspace || workspace_bytes < vig::grad_norm_workspace(n, count)) return VIG_ENOSPC;
+  return vig::launch_grad_norm(grad, n, dtype, count, max_norm, norm, scale, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,580 @@
+// The gated linear recurrence of a vector state, forward and backward, and its step for one token.
+//
+//   h_t = e^{g_t} h_{t-1} + x_t,      o_t = h_t                        (causal; h_{-1} = initial state or 0)
+//   o_t = s (h_t + h'_t),  h'_t = e^{g'_t} h'_{t+1} + x_t              (both directions)
+//
+// What a run of tokens does to the state that enters it is an affine map per channel, h -> A h + S, and maps compose in any grouping:
+//   (A, S) then (A', S')  =  (A A', A' S + S').
+// A thread folds the eight tokens that it holds in registers, a wave its four threads of a channel by shuffles, a workgroup its waves through LDS;
+// then every thread knows the state that enters its tokens and walks them once more, which costs one fused multiply-add a value.  Memory is what
+// bounds it: rows and gates are read once.  Sequences that one workgroup does not hold are cut in chunks: a first launch folds the chunks
+// (reads everything once, writes 8 bytes a chunk and channel), the second folds the chunks in front of its own and walks.
+//
+// Backward: dh_t = do_t + e^{g_{t+1}} dh_{t+1}; with D_t = e^{g_t} dh_t, what token t hands back, the walk against the direction is D -> e^{g_t} (do_t + D), an
+// affine map again, and dx_t = dh_t, dg_t = dh_t u_t with u_t = e^{g_t} h_{t-1} from the walk along it, recomputed in 32 bits from x and g (the stored
+// output is rounded, and for both directions holds their sum).
+#include "common.h"
+#include "launch.h"
+#include <algorithm>
+
+namespace vig {
+namespace {
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr unsigned kBeyond = 0x40000000u;  // byte offset that no descriptor here covers (kScanRow)
+constexpr int kTokens = 8;                 // of a thread
+constexpr int kMaxWaves = 16;
+
+// N consecutive channels of one token as stored
+template <typename T, int N> struct Piece;
+template <> struct Piece<uint16_t, 4> {
+  u32x2_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); }
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? bf16hi_to_f32(v[i >> 1]) : bf16lo_to_f32(v[i >> 1]); }
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[4]) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])}, r, off, 0, 0);
+  }
+};
+template <> struct Piece<float, 4> {
+  u32x4_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float(v[i]); }
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[4]) {
+    __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])}, r, off, 0, 0);
+  }
+};
+template <> struct Piece<uint16_t, 1> {
+  uint16_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0); }
+  __device__ __forceinline__ float get(int) const { return bf16_to_f32(v); }
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[1]) {
+    __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x[0]), r, off, 0, 0);
+  }
+};
+template <> struct Piece<float, 1> {
+  uint32_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+  __device__ __forceinline__ float get(int) const { return __uint_as_float(v); }
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[1]) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, off, 0, 0);
+  }
+};
+
+// h -> a h + s for each of a thread's channels
+template <int N> struct Map {
+  float a[N], s[N];
+  __device__ __forceinline__ void identity() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = 1.f, s[i] = 0.f;
+  }
+  // this one behind `first`
+  __device__ __forceinline__ void behind(const Map& first) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = fmaf(a[i], first.s[i], s[i]), a[i] *= first.a[i];
+  }
+  __device__ __forceinline__ void apply(float (&h)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = fmaf(a[i], h[i], s[i]);
+  }
+};
+
+template <bool UP, int N>
+__device__ __forceinline__ Map<N> shifted(const Map<N>& m, int lanes) {
+  Map<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    r.a[i] = UP ? __shfl_up(m.a[i], lanes) : __shfl_down(m.a[i], lanes);
+    r.s[i] = UP ? __shfl_up(m.s[i], lanes) : __shfl_down(m.s[i], lanes);
+  }
+  return r;
+}
+
+// Where a thread stands: LPR lanes side by side take a token's channels, 64 / LPR runs of tokens lie behind one another in a wave.
+template <int N, int LPR> struct Place {
+  int wave, waves, lane, run, lc;  // lc: lane of the token's channels
+  __device__ __forceinline__ Place()
+      : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), run((threadIdx.x & 63) / LPR), lc(threadIdx.x % LPR) {}
+};
+
+// LDS of one direction: each wave's map of a channel
+template <int N, int LPR> struct Board {
+  alignas(8 * N) float v[kMaxWaves][LPR][2 * N];
+};
+
+// Folds the threads' maps along a wave.  UP: tokens in their order; else against it.  Leaves in `m` the map of what lies in front of this
+// thread in its wave, and the whole wave's on the board.
+template <bool UP, int N, int LPR>
+__device__ __forceinline__ void fold_wave(Map<N>& m, const Place<N, LPR>& at, Board<N, LPR>& board) {
+#pragma unroll
+  for (int d = LPR; d < 64; d *= 2) {
+    const Map<N> p = shifted<UP, N>(m, d);
+    if (UP ? at.lane >= d : at.lane + d < 64) m.behind(p);
+  }
+  if (UP ? at.lane >= 64 - LPR : at.lane < LPR) {
+    float* to = board.v[at.wave][at.lc];
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[2 * i] = m.a[i], to[2 * i + 1] = m.s[i];
+  }
+  if constexpr (LPR < 64) {
+    m = shifted<UP, N>(m, LPR);
+    if (UP ? at.lane < LPR : at.lane >= 64 - LPR) m.identity();
+  } else {
+    m.identity();
+  }
+}
+// (behind the barrier) h: state that enters the workgroup -> the one that enters this thread's tokens
+template <bool UP, int N, int LPR>
+__device__ __forceinline__ void enter(float (&h)[N], const Map<N>& m, const Place<N, LPR>& at, const Board<N, LPR>& board) {
+  for (int w = UP ? 0 : at.waves - 1; w != at.wave; w += UP ? 1 : -1) {
+    const float* from = board.v[w][at.lc];
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = fmaf(from[2 * i], h[i], from[2 * i + 1]);
+  }
+  m.apply(h);
+}
+// (behind the barrier) the map of the whole workgroup
+template <bool UP, int N, int LPR>
+__device__ __forceinline__ Map<N> whole(const Place<N, LPR>& at, const Board<N, LPR>& board) {
+  Map<N> t;
+  t.identity();
+  for (int k = 0; k < at.waves; ++k) {
+    const float* from = board.v[UP ? k : at.waves - 1 - k][at.lc];
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.s[i] = fmaf(from[2 * i], t.s[i], from[2 * i + 1]), t.a[i] *= from[2 * i];
+  }
+  return t;
+}
+
+struct ScanArgs {
+  const void *x, *g[2], *d_o;  // d_o: dense, like the outputs
+  void *o, *dx, *dg[2];
+  const float *h0, *dhT;
+  float *hT, *dh0;
+  float* maps;  // [B, directions, chunks, D, 2]; directions: gates 0 along, gates 0 against (backward), gates 1 against, gates 1 along (backward)
+  long long xb, xl, gb, gl;  // strides of batch element and token, in elements
+  int L, D, groups, chunks, chunk;
+  float scale;
+};
+
+// The workgroup's piece of the tensors
+struct Tile {
+  int b, ch, cg, t0, rows;
+  __device__ __forceinline__ Tile(const ScanArgs& p) {
+    unsigned id = blockIdx.x;
+    const unsigned q = id / (unsigned)p.groups;
+    cg = (int)(id - q * p.groups);
+    b = (int)(q / (unsigned)p.chunks);
+    ch = (int)(q - (unsigned)b * p.chunks);
+    t0 = ch * p.chunk;
+    rows = min(p.chunk, p.L - t0);
+  }
+  template <typename T>
+  __device__ __forceinline__ rsrc_t rows_of(const void* base, long long sb, long long sl) const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(base)) + b * sb + t0 * sl, 0, (int)(rows * sl * (long long)sizeof(T)), 0x00020000);
+  }
+};
+
+// gates as the factors they stand for; tokens behind the sequence read as gates of 0 and rows of 0, the map that changes nothing
+template <typename T, int N>
+__device__ __forceinline__ void factors(const Piece<T, N> (&raw)[kTokens], float (&a)[kTokens][N]) {
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[t][i] = exp_fast(raw[t].get(i));
+}
+template <typename T, int N>
+__device__ __forceinline__ void load_run(Piece<T, N> (&raw)[kTokens], rsrc_t r, unsigned first, unsigned pitch) {
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) raw[t].load(r, first + t * pitch);
+}
+
+// A thread's map along its tokens (h -> a h + x) or against them; BACK: h -> a (h + scale x), what gradients do
+template <bool UP, bool BACK, typename T, int N>
+__device__ __forceinline__ Map<N> fold_run(const float (&a)[kTokens][N], const Piece<T, N> (&x)[kTokens], float scale = 1.f) {
+  Map<N> m;
+  m.identity();
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) {
+    const int t = UP ? k : kTokens - 1 - k;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      m.s[i] = BACK ? a[t][i] * fmaf(scale, x[t].get(i), m.s[i]) : fmaf(a[t][i], m.s[i], x[t].get(i));
+      m.a[i] *= a[t][i];
+    }
+  }
+  return m;
+}
+
+// The state that enters this workgroup's chunk from the chunks in front of it: each of the workgroup's runs folds a
+// stretch of them, and the runs fold as tokens do.
+template <bool UP, int N, int LPR>
+__device__ __forceinline__ Map<N> fold_chunks(const ScanArgs& p, const Tile& tile, const Place<N, LPR>& at, int dir, int dirs, int c, bool has) {
+  const int n = UP ? tile.ch : p.chunks - 1 - tile.ch;  // chunks in front
+  const int runs = at.waves * (64 / LPR), each = (n + runs - 1) / runs;
+  const int slot = at.wave * (64 / LPR) + at.run;
+  // (runs in the order of the tokens; against it the last run comes first)
+  const int first = UP ? slot * each : tile.ch + 1 + slot * each, end = min(first + each, UP ? n : p.chunks);
+  const float* from = p.maps + (((size_t)tile.b * dirs + dir) * p.chunks) * p.D * 2;
+  Map<N> m;
+  m.identity();
+  for (int k = 0; k < each; ++k) {
+    const int j = UP ? first + k : end - 1 - k;
+    if (j < first || j >= end || !has) continue;
+    const float* v = from + ((size_t)j * p.D + c) * 2;
+    if constexpr (N == 4) {
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(v), hi = *reinterpret_cast<const f32x4_t*>(v + 4);
+      const float a[4] = {lo[0], lo[2], hi[0], hi[2]}, s[4] = {lo[1], lo[3], hi[1], hi[3]};
+#pragma unroll
+      for (int i = 0; i < N; ++i) m.s[i] = fmaf(a[i], m.s[i], s[i]), m.a[i] *= a[i];
+    } else {
+      m.s[0] = fmaf(v[0], m.s[0], v[1]), m.a[0] *= v[0];
+    }
+  }
+  return m;
+}
+template <int N>
+__device__ __forceinline__ void store_map(const ScanArgs& p, const Tile& tile, int dir, int dirs, int c, const Map<N>& m) {
+  float* v = p.maps + ((((size_t)tile.b * dirs + dir) * p.chunks + tile.ch) * p.D + c) * 2;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[2 * i] = m.a[i], v[2 * i + 1] = m.s[i];
+}
+template <int N>
+__device__ __forceinline__ void load_state(float (&h)[N], const float* from, const ScanArgs& p, int b, int c, bool has) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) h[i] = from && has ? from[(size_t)b * p.D + c + i] : 0.f;
+}
+template <int N>
+__device__ __forceinline__ void store_state(float* to, const float (&h)[N], const ScanArgs& p, int b, int c) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) to[(size_t)b * p.D + c + i] = h[i];
+}
+
+// ---- forward.  FOLD: only the chunks' maps
+
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int LPR>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) {
+  __shared__ Board<N, LPR> board[BOTH ? 2 : 1], front[FOLD ? 1 : BOTH ? 2 : 1];
+  const Place<N, LPR> at;
+  const Tile tile(p);
+  const int c = (tile.cg * LPR + at.lc) * N;
+  const bool has = c < p.D;
+  const int first = (at.wave * (64 / LPR) + at.run) * kTokens;
+  auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
+  Piece<TX, N> x[kTokens];
+  Piece<TG, N> raw[kTokens];
+  float a[kTokens][N], a2[BOTH ? kTokens : 1][N];
+  load_run(raw, tile.rows_of<TG>(p.g[0], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
+  load_run(x, tile.rows_of<TX>(p.x, p.xb, p.xl), offset(p.xl, sizeof(TX)), (unsigned)(p.xl * sizeof(TX)));
+  [[maybe_unused]] Piece<TG, N> raw2[BOTH ? kTokens : 1];
+  if constexpr (BOTH) load_run(raw2, tile.rows_of<TG>(p.g[1], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
+  constexpr int dirs = BOTH ? 2 : 1;
+  [[maybe_unused]] Map<N> before, after;
+  if constexpr (!FOLD) {
+    if (p.chunks > 1) {
+      before = fold_chunks<true, N, LPR>(p, tile, at, 0, dirs, c, has);
+      fold_wave<true, N, LPR>(before, at, front[0]);
+      if constexpr (BOTH) {
+        after = fold_chunks<false, N, LPR>(p, tile, at, 1, dirs, c, has);
+        fold_wave<false, N, LPR>(after, at, front[BOTH ? 1 : 0]);
+      }
+    }
+  }
+  factors(raw, a);
+  Map<N> m = fold_run<true, false>(a, x), m2;
+  fold_wave<true, N, LPR>(m, at, board[0]);
+  if constexpr (BOTH) {
+    factors(raw2, a2);
+    m2 = fold_run<false, false>(a2, x);
+    fold_wave<false, N, LPR>(m2, at, board[BOTH ? 1 : 0]);
+  }
+  __syncthreads();
+  if constexpr (FOLD) {
+    if (at.wave == 0 && at.run == 0 && has) {
+      store_map(p, tile, 0, dirs, c, whole<true, N, LPR>(at, board[0]));
+      if constexpr (BOTH) store_map(p, tile, 1, dirs, c, whole<false, N, LPR>(at, board[BOTH ? 1 : 0]));
+    }
+    return;
+  }
+  float h[N], y[kTokens][N];
+  load_state(h, p.h0, p, tile.b, c, has);
+  if (p.chunks > 1) whole<true, N, LPR>(at, front[0]).apply(h);
+  enter<true, N, LPR>(h, m, at, board[0]);
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[t][i] = h[i] = fmaf(a[t][i], h[i], x[t].get(i));
+  // (tokens behind the sequence change nothing: the last run ends with the state behind its last token)
+  if (p.hT && tile.ch == p.chunks - 1 && at.wave == at.waves - 1 && at.run == 64 / LPR - 1 && has) store_state(p.hT, h, p, tile.b, c);
+  if constexpr (BOTH) {
+    float r[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = 0.f;
+    if (p.chunks > 1) whole<false, N, LPR>(at, front[BOTH ? 1 : 0]).apply(r);
+    enter<false, N, LPR>(r, m2, at, board[BOTH ? 1 : 0]);
+#pragma unroll
+    for (int t = kTokens - 1; t >= 0; --t)
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = fmaf(a2[t][i], r[i], x[t].get(i)), y[t][i] += r[i];
+  }
+  const rsrc_t out = tile.rows_of<TX>(p.o, (long long)p.L * p.D, p.D);
+  const unsigned to = offset(p.D, sizeof(TX));
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[t][i] *= p.scale;
+    Piece<TX, N>::store(out, to + t * (unsigned)(p.D * sizeof(TX)), y[t]);
+  }
+}
+
+// ---- backward
+
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int LPR>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs p) {
+  constexpr int dirs = BOTH ? 4 : 2;
+  __shared__ Board<N, LPR> board[dirs], front[FOLD ? 1 : dirs];
+  const Place<N, LPR> at;
+  const Tile tile(p);
+  const int c = (tile.cg * LPR + at.lc) * N;
+  const bool has = c < p.D;
+  const int first = (at.wave * (64 / LPR) + at.run) * kTokens;
+  auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
+  const long long dense = (long long)p.L * p.D;
+  Piece<TX, N> x[kTokens], dy[kTokens];
+  load_run(x, tile.rows_of<TX>(p.x, p.xb, p.xl), offset(p.xl, sizeof(TX)), (unsigned)(p.xl * sizeof(TX)));
+  load_run(dy, tile.rows_of<TX>(p.d_o, dense, p.D), offset(p.D, sizeof(TX)), (unsigned)(p.D * sizeof(TX)));
+  Piece<TG, N> raw[BOTH ? 2 : 1][kTokens];
+#pragma unroll
+  for (int w = 0; w < (BOTH ? 2 : 1); ++w)
+    load_run(raw[w], tile.rows_of<TG>(p.g[w], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
+  float a[BOTH ? 2 : 1][kTokens][N];
+  Map<N> along[BOTH ? 2 : 1], against[BOTH ? 2 : 1];
+  if constexpr (!FOLD) {
+    if (p.chunks > 1) {
+      // (only the boards are wanted)
+#pragma unroll
+      for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
+        Map<N> f = w ? fold_chunks<false, N, LPR>(p, tile, at, 2, dirs, c, has) : fold_chunks<true, N, LPR>(p, tile, at, 0, dirs, c, has);
+        if (w) fold_wave<false, N, LPR>(f, at, front[BOTH ? 2 : 0]);
+        else fold_wave<true, N, LPR>(f, at, front[0]);
+        f = w ? fold_chunks<true, N, LPR>(p, tile, at, 3, dirs, c, has) : fold_chunks<false, N, LPR>(p, tile, at, 1, dirs, c, has);
+        if (w) fold_wave<true, N, LPR>(f, at, front[BOTH ? 3 : 0]);
+        else fold_wave<false, N, LPR>(f, at, front[1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
+    factors(raw[w], a[w]);
+    if (w == 0) {
+      along[w] = fold_run<true, false>(a[w], x);
+      fold_wave<true, N, LPR>(along[w], at, board[0]);
+      against[w] = fold_run<false, true>(a[w], dy, p.scale);
+      fold_wave<false, N, LPR>(against[w], at, board[1]);
+    } else {
+      along[w] = fold_run<false, false>(a[w], x);
+      fold_wave<false, N, LPR>(along[w], at, board[BOTH ? 2 : 0]);
+      against[w] = fold_run<true, true>(a[w], dy, p.scale);
+      fold_wave<true, N, LPR>(against[w], at, board[BOTH ? 3 : 0]);
+    }
+  }
+  __syncthreads();
+  if constexpr (FOLD) {
+    if (at.wave == 0 && at.run == 0 && has) {
+      store_map(p, tile, 0, dirs, c, whole<true, N, LPR>(at, board[0]));
+      store_map(p, tile, 1, dirs, c, whole<false, N, LPR>(at, board[1]));
+      if constexpr (BOTH) {
+        store_map(p, tile, 2, dirs, c, whole<false, N, LPR>(at, board[BOTH ? 2 : 0]));
+        store_map(p, tile, 3, dirs, c, whole<true, N, LPR>(at, board[BOTH ? 3 : 0]));
+      }
+    }
+    return;
+  }
+  float dx[kTokens][N];
+#pragma unroll
+  for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
+    float h[N], d[N], u[kTokens][N];
+    load_state(h, w ? nullptr : p.h0, p, tile.b, c, has);
+    load_state(d, w ? nullptr : p.dhT, p, tile.b, c, has);
+    if (w == 0) {
+      if (p.chunks > 1) whole<true, N, LPR>(at, front[0]).apply(h), whole<false, N, LPR>(at, front[FOLD ? 0 : 1]).apply(d);
+      enter<true, N, LPR>(h, along[w], at, board[0]);
+      enter<false, N, LPR>(d, against[w], at, board[1]);
+    } else {
+      if (p.chunks > 1) whole<false, N, LPR>(at, front[FOLD || !BOTH ? 0 : 2]).apply(h), whole<true, N, LPR>(at, front[FOLD || !BOTH ? 0 : 3]).apply(d);
+      enter<false, N, LPR>(h, along[w], at, board[BOTH ? 2 : 0]);
+      enter<true, N, LPR>(d, against[w], at, board[BOTH ? 3 : 0]);
+    }
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int t = w == 0 ? k : kTokens - 1 - k;
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[t][i] = a[w][t][i] * h[i], h[i] = u[t][i] + x[t].get(i);
+    }
+    const rsrc_t out = tile.rows_of<TG>(p.dg[w], dense, p.D);
+    const unsigned to = offset(p.D, sizeof(TG));
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int t = w == 0 ? kTokens - 1 - k : k;
+      float dg[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float dh = fmaf(p.scale, dy[t].get(i), d[i]);
+        dx[t][i] = w == 0 ? dh : dx[t][i] + dh;
+        dg[i] = dh * u[t][i];
+        d[i] = a[w][t][i] * dh;
+      }
+      Piece<TG, N>::store(out, to + t * (unsigned)(p.D * sizeof(TG)), dg);
+    }
+    if (w == 0 && p.dh0 && tile.ch == 0 && at.wave == 0 && at.run == 0 && has) store_state(p.dh0, d, p, tile.b, c);
+  }
+  const rsrc_t out = tile.rows_of<TX>(p.dx, dense, p.D);
+  const unsigned to = offset(p.D, sizeof(TX));
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) Piece<TX, N>::store(out, to + t * (unsigned)(p.D * sizeof(TX)), dx[t]);
+}
+
+// ---- one token
+
+template <typename T>
+__device__ __forceinline__ void load_some(const T* p, float (&x)[1]) { x[0] = Elem<T>::load(p); }
+__device__ __forceinline__ void load_some(const float* p, float (&x)[4]) {
+  const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = v[i];
+}
+__device__ __forceinline__ void load_some(const uint16_t* p, float (&x)[4]) {
+  const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p);
+  x[0] = bf16lo_to_f32(v[0]), x[1] = bf16hi_to_f32(v[0]), x[2] = bf16lo_to_f32(v[1]), x[3] = bf16hi_to_f32(v[1]);
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, const float (&x)[1]) { Elem<T>::store(p, x[0]); }
+__device__ __forceinline__ void store_some(float* p, const float (&x)[4]) { *reinterpret_cast<f32x4_t*>(p) = f32x4_t{x[0], x[1], x[2], x[3]}; }
+__device__ __forceinline__ void store_some(uint16_t* p, const float (&x)[4]) {
+  *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+}
+
+template <typename TX, typename TG, int N>
+__global__ __launch_bounds__(256) void gated_scan_step_kernel(const TX* x, const TG* g, float* h, TX* o, unsigned n, unsigned per_row, long long xl, long long gl, int D) {
+  const unsigned id = blockIdx.x * 256u + threadIdx.x;
+  if (id >= n) return;
+  const unsigned b = id / per_row, c = (id - b * per_row) * N;
+  const TX* xr = x + b * xl + c;
+  const TG* gr = g + b * gl + c;
+  const size_t at = (size_t)b * D + c;
+  float a[N], v[N], s[N];
+  load_some(gr, a), load_some(xr, v), load_some(h + at, s);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = fmaf(exp_fast(a[i]), s[i], v[i]);
+  store_some(h + at, v), store_some(o + at, v);
+}
+
+// ---- host side
+
+struct Cut {
+  int lanes, channels, waves, chunks, chunk, groups;
+};
+// Whether four channels move at once: whole quads in every row, on boundaries of their size (a null pointer stands on any)
+inline bool quads(int D, long long a, long long b, long long c, long long d) { return D % 4 == 0 && (a | b | c | d) % 4 == 0; }
+template <typename... P>
+bool on_quads(int dtype, P... p) {
+  const uintptr_t size = dtype == VIG_BF16 ? 8 : 16;
+  return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...);
+}
+
+inline Cut cut(int B, int L, int D, bool vector) {
+  Cut k;
+  k.channels = vector ? 4 : 1;
+  k.lanes = vector ? 16 : 64;
+  k.groups = (D + 63) / 64;
+  const int run = 64 / k.lanes * kTokens;  // tokens of a wave
+  const int waves = (L + run - 1) / run;
+  k.chunks = (waves + kMaxWaves - 1) / kMaxWaves;
+  k.waves = (waves + k.chunks - 1) / k.chunks;
+  k.chunk = k.waves * run;
+  k.chunks = (L + k.chunk - 1) / k.chunk;
+  return k;
+}
+
+template <typename TX, typename TG, bool BOTH, int N, int LPR>
+void start(const ScanArgs& p, bool bwd, bool fold, dim3 grid, dim3 block, hipStream_t stream) {
+  if (bwd) {
+    if (fold) hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, true, N, LPR>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, false, N, LPR>), grid, block, 0, stream, p);
+  } else {
+    if (fold) hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, true, N, LPR>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, false, N, LPR>), grid, block, 0, stream, p);
+  }
+}
+template <typename TX, typename TG>
+void start(const ScanArgs& p, bool bwd, bool fold, bool vector, dim3 grid, dim3 block, hipStream_t stream) {
+  if (p.g[1]) {
+    if (vector) start<TX, TG, true, 4, 16>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, true, 1, 64>(p, bwd, fold, grid, block, stream);
+  } else {
+    if (vector) start<TX, TG, false, 4, 16>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, false, 1, 64>(p, bwd, fold, grid, block, stream);
+  }
+}
+int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t stream) {
+  const bool vector = quads(p.D, p.xb, p.xl, p.gb, p.gl) && on_quads(io_dtype, p.x, p.d_o, p.o, p.dx) && on_quads(gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
+  const Cut k = cut(B, p.L, p.D, vector);
+  p.groups = k.groups, p.chunks = k.chunks, p.chunk = k.chunk;
+  const long long groups = (long long)B * k.groups * k.chunks;
+  if (groups > 0x7fffffffLL) return VIG_ENOTSUP;
+  const dim3 grid((unsigned)groups), block(64 * k.waves);
+  for (int fold = k.chunks > 1; fold >= 0; --fold) {
+    if (io_dtype == VIG_BF16) {
+      if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, vector, grid, block, stream);
+      else start<uint16_t, float>(p, bwd, fold, vector, grid, block, stream);
+    } else {
+      if (gate_dtype == VIG_BF16) start<float, uint16_t>(p, bwd, fold, vector, grid, block, stream);
+      else start<float, float>(p, bwd, fold, vector, grid, block, stream);
+    }
+    if (hipGetLastError() != hipSuccess) return VIG_ELAUNCH;
+  }
+  return VIG_OK;
+}
+
+}  // namespace
+
+// Bytes for the chunks' maps, whichever way the rows lie (rows that move one channel at a time have the more chunks).
+size_t gated_scan_workspace(int B, int L, int D, bool both, bool bwd) {
+  const int chunks = std::max(cut(B, L, D, false).chunks, cut(B, L, D, true).chunks);
+  return chunks > 1 ? (size_t)B * (both ? 2 : 1) * (bwd ? 2 : 1) * chunks * D * 2 * sizeof(float) : 0;
+}
+
+int launch_gated_scan(const GatedScan& s, hipStream_t stream) {
+  ScanArgs p{};
+  p.x = s.x, p.g[0] = s.g_fwd, p.g[1] = s.g_bwd, p.o = s.o, p.h0 = s.initial, p.hT = s.final, p.maps = static_cast<float*>(s.workspace);
+  p.xb = s.x_strides[0], p.xl = s.x_strides[1], p.gb = s.g_strides[0], p.gl = s.g_strides[1];
+  p.L = s.L, p.D = s.D, p.scale = s.out_scale;
+  p.d_o = s.d_o, p.dx = s.dx, p.dg[0] = s.dg_fwd, p.dg[1] = s.dg_bwd, p.dhT = s.d_final, p.dh0 = s.d_initial;
+  return run(p, s.d_o != nullptr, s.B, s.io_dtype, s.gate_dtype, stream);
+}
+
+template <typename TX, typename TG>
+static void start_step(const GatedScanStep& s, bool vector, hipStream_t stream) {
+  const unsigned per_row = vector ? s.D / 4 : s.D, n = (unsigned)s.B * per_row;
+  const dim3 grid((n + 255) / 256), block(256);
+  if (vector)
+    hipLaunchKernelGGL((gated_scan_step_kernel<TX, TG, 4>), grid, block, 0, stream, (const TX*)s.x, (const TG*)s.g, s.state, (TX*)s.o, n, per_row, s.x_stride,
+                       s.g_stride, s.D);
+  else
+    hipLaunchKernelGGL((gated_scan_step_kernel<TX, TG, 1>), grid, block, 0, stream, (const TX*)s.x, (const TG*)s.g, s.state, (TX*)s.o, n, per_row, s.x_stride,
+                       s.g_stride, s.D);
+}
+
+int launch_gated_scan_step(const GatedScanStep& s, hipStream_t stream) {
+  if ((long long)s.B * s.D > 0x7fffff00LL) return VIG_ENOTSUP;
+  const bool vector = quads(s.D, s.x_stride, s.g_stride, 0, 0) && on_quads(s.io_dtype, s.x, s.o) && on_quads(s.gate_dtype, s.g) && on_quads(VIG_F32, s.state);
+  if (s.io_dtype == VIG_BF16) {
+    if (s.gate_dtype == VIG_BF16) start_step<uint16_t, uint16_t>(s, vector, stream);
+    else start_step<uint16_t, float>(s, vector, stream);
+  } else {
+    if (s.gate_dtype == VIG_BF16) start_step<float, uint16_t>(s, vector, stream);
+    else start_step<float, float>(s, vector, stream);
+  }
+  return hipGetLastError() == hipSuccess ? VIG_OK : VIG_ELAUNCH;
+}
+
+}  // namespace vig

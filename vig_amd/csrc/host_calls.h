@@ -100,6 +100,12 @@ PyObject* block_mlp(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* stem_conv(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* stem_norm(PyObject*, PyObject* const* a, Py_ssize_t n);
 
+// the methods of scan_calls.cpp
+PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n);
+
 // the methods of model_forward.cpp
 PyObject* make_plan(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* plan_describes(PyObject*, PyObject* const* a, Py_ssize_t n);

@@ -117,6 +117,58 @@ struct LinearWgrad {
 size_t linear_wgrad_workspace(long long T, const LinearWgrad* layers, int count);
 int launch_linear_wgrad(const LinearWgrad* layers, int count, long long T, void* workspace, vig_sum_jobs* later, hipStream_t stream);
 
+// The gated linear recurrence of a vector state (gated_scan.hip); with d_o its backward.
+struct GatedScan {
+  const void *x, *g_fwd, *g_bwd;  // g_bwd null: causal
+  const void* d_o;                // dense; null: forward
+  void* o;
+  void *dx, *dg_fwd, *dg_bwd;
+  const float *initial, *d_final;  // may be null, [B, D] like the next two; causal only
+  float *final, *d_initial;
+  void* workspace;
+  long long x_strides[2], g_strides[2];  // batch element, token
+  int B, L, D;
+  float out_scale;
+  int io_dtype, gate_dtype;
+};
+// Widest row and largest distance between rows, in elements: a workgroup's rows stay within 2^30 bytes of its first.
+constexpr long long kScanRow = 1 << 19;
+size_t gated_scan_workspace(int B, int L, int D, bool both, bool bwd);
+int launch_gated_scan(const GatedScan& s, hipStream_t stream);
+struct GatedScanStep {
+  const void *x, *g;
+  float* state;
+  void* o;
+  int B, D;
+  long long x_stride, g_stride;
+  int io_dtype, gate_dtype;
+};
+int launch_gated_scan_step(const GatedScanStep& s, hipStream_t stream);
+
+// Norm of many gradients and AdamW over many tensors (update.hip).
+struct AdamW {
+  void* const* param;
+  const void* const* grad;
+  void* const* exp_avg;     // fp32; with states in 8 bits e4m3, and the squares' roots in exp_avg_sq
+  void* const* exp_avg_sq;
+  float* const* avg_scale;  // states in 8 bits: a scale for each block of 256
+  float* const* sq_scale;
+  const long long* n;
+  const int *param_dtype, *grad_dtype;
+  int count, state_bits;
+  double lr, beta1, beta2, eps, weight_decay;
+  long long step;
+  const float* lr_on_device;         // null: lr
+  const long long* step_on_device;   // null: step
+  const float* grad_scale;           // null: 1
+  unsigned long long seed;
+};
+constexpr long long kUpdateElements = 1LL << 40;  // of a list: its blocks of 256 are numbered in 32 bits
+int launch_adamw(const AdamW& a, hipStream_t stream);
+size_t grad_norm_workspace(const long long* n, int count);
+int launch_grad_norm(const void* const* g, const long long* n, const int* dtype, int count, float max_norm, float* norm, float* scale, void* workspace,
+                     hipStream_t stream);
+
 // Most tensors one launch_cast_many takes.
 constexpr int kMaxCastJobs = 16;
 

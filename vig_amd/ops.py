@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -1053,3 +1053,274 @@ def _swiglu_raw(gate_up: torch.Tensor) -> torch.Tensor:
         rc = lib.vig_swiglu_fwd(gate_up.data_ptr(), out.data_ptr(), rows, I, _dt(gate_up), _stream_ptr(gate_up))
     _lib.check(rc, "vig_swiglu_fwd")
     return out
+
+
+# ---------------------------------------------------------------------------
+# gated linear recurrence of a vector state
+# ---------------------------------------------------------------------------
+
+def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.Tensor] = None,
+               output_final_state: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Causal gated recurrence h_t = e^{g_t} h_{t-1} + x_t, o_t = h_t, on [B,L,D] (or [B,H,L,D]) tensors: (o, final_state or None).
+
+    The causal GLA ops' sibling whose state is one number a channel.  g: natural-log decays (<= 0), of any of the built dtypes whatever
+    x has; a token of x = 0, g = 0 changes nothing (padding), g = -inf starts a new sequence behind the last one (packed
+    sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
+    and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
+    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd)."""
+    return _gated_scan(x, g, initial_state, False, bool(output_final_state))
+
+
+def bid_gated_scan(x: torch.Tensor, g: torch.Tensor) -> Tuple[torch.Tensor, None]:
+    """The recurrence in both directions, averaged as bid_fused_recurrent_gla does: x [B,L,D] (or [B,H,L,D]), g [2B,...] = cat(fwd gates,
+    bwd gates), both in natural order; o = (o_f + o_b)/2, and no state.  Packed sequences: g = -inf at the first token of each in the first half, at the
+    last token in the second.  Differentiable in x and g."""
+    return _gated_scan(x, g, None, True, False)
+
+
+def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
+    """gated_scan for one token of every sequence: state (fp32 [B,D], contiguous) <- e^g state + x in place, returned in x's dtype.
+    x, g: [B,D], or columns of wider rows.  Inference only."""
+    calls = _ext.calls()
+    if calls is not None:
+        o = calls.gated_scan_step(x, g, state)
+        if o is not None:
+            return o
+    lib = _lib.load()
+    _check_cuda(x, g, state)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, g, state)):
+        raise ValueError("gated_scan_step updates its state in place and records no gradient; use gated_scan")
+    if x.dim() != 2 or g.shape != x.shape or state.shape != x.shape:
+        raise ValueError("x, g and state must be [B,D]")
+    if state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError("state must be a contiguous float32 tensor (it is updated in place)")
+    io_dt, g_dt = _dt(x), _dt(g)
+    B, D = x.shape
+    o = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        return o
+    x, g = _scan_rows(x), _scan_rows(g)
+    pitch = lambda t: D if B == 1 else t.stride(0)  # noqa: E731
+    with torch.cuda.device(x.device):
+        rc = lib.vig_gated_scan_step(x.data_ptr(), g.data_ptr(), state.data_ptr(), o.data_ptr(), B, D, pitch(x), pitch(g), io_dt, g_dt, _stream_ptr(x))
+    _lib.check(rc, "vig_gated_scan_step")
+    torch.autograd.graph.increment_version(state)
+    return o
+
+
+def _gated_scan(x, g, initial_state, both, want_final):
+    if x.dim() == 4:  # heads: sequences of their own
+        if g.dim() != 4 or g.shape[1:] != x.shape[1:]:
+            raise ValueError("shape mismatch between x and g")
+        B, H, L, D = x.shape
+        h0 = initial_state.reshape(B * H, D) if initial_state is not None and tuple(initial_state.shape) == (B, H, D) else initial_state
+        if initial_state is not None and h0 is initial_state:
+            raise ValueError(f"initial_state must be [B,H,D] = {(B, H, D)}; got {tuple(initial_state.shape)}")
+        o, h = _gated_scan(x.reshape(B * H, L, D), g.reshape(g.shape[0] * H, L, D), h0, both, want_final)
+        return o.view(B, H, L, D), h.view(B, H, D) if h is not None else None
+    if initial_state is not None:
+        initial_state = initial_state.float()
+    calls = _ext.calls()
+    if calls is not None:  # one native call for what the kernels take; None: not of that kind
+        r = calls.gated_scan(x, g, initial_state, both, want_final)
+        if r is not None:
+            return r if want_final else (r, None)
+    _check_cuda(x, g, initial_state)
+    if x.dim() != 3 or g.dim() != 3 or g.shape[1:] != x.shape[1:]:
+        raise ValueError("x and g must be [B,L,D] (or [B,H,L,D]) of the same sizes")
+    B, L, D = x.shape
+    if g.shape[0] != (2 * B if both else B):
+        raise ValueError(f"bidirectional gates must be [2B,...]; got batch {g.shape[0]} for B={B}" if both else "shape mismatch between x and g")
+    if initial_state is not None and tuple(initial_state.shape) != (B, D):
+        raise ValueError(f"initial_state must be [B,D] = {(B, D)}; got {tuple(initial_state.shape)}")
+    _dt(x), _dt(g)
+    if x.numel() == 0:  # nothing happens to the state
+        state = initial_state if initial_state is not None else torch.zeros(B, D, dtype=torch.float32, device=x.device)
+        return x.clone(), state.clone() if want_final else None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, g, initial_state)):
+        o, h = _GatedScanFunction.apply(x, g, initial_state, both, want_final)
+    else:
+        o, h = _gated_scan_raw(x, g, initial_state, both, want_final)
+    return o, h
+
+
+def _scan_rows(t):
+    """t as it lies where its channels stand side by side in rows that do not overlap, else packed."""
+    side = t.shape[-1] == 1 or t.stride(-1) == 1
+    return t if side and (t.shape[-2] == 1 or t.shape[-1] <= t.stride(-2) <= 1 << 19) else t.contiguous()
+
+
+def _scan_strides(t):
+    return (ctypes.c_longlong * 2)(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else t.shape[2])
+
+
+def _second_gates(g, both):
+    return g.data_ptr() + g.shape[0] // 2 * g.stride(0) * g.element_size() if both else None
+
+
+def _gated_scan_raw(x, g, h0, both, want_final):
+    lib = _lib.load()
+    x, g = _scan_rows(x), _scan_rows(g)
+    h0 = h0.contiguous() if h0 is not None else None
+    B, L, D = x.shape
+    o = torch.empty(B, L, D, dtype=x.dtype, device=x.device)
+    h = torch.empty(B, D, dtype=torch.float32, device=x.device) if want_final else None
+    need = lib.vig_gated_scan_fwd_workspace(B, L, D, int(both))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    with torch.cuda.device(x.device):
+        rc = lib.vig_gated_scan_fwd(ptr(x), ptr(g), _second_gates(g, both), ptr(h0), ptr(o), ptr(h), ptr(ws), need, B, L, D, _scan_strides(x), _scan_strides(g),
+                                    0.5 if both else 1.0, _dt(x), _dt(g), _stream_ptr(x))
+    _lib.check(rc, "vig_gated_scan_fwd")
+    return o, h
+
+
+class _GatedScanFunction(torch.autograd.Function):
+    """Autograd node of the gated scan: forward and backward each the library's kernels."""
+
+    @staticmethod
+    def forward(ctx, x, g, h0, both, want_final):
+        ctx.save_for_backward(x, g, h0)
+        ctx.both = both
+        ctx.set_materialize_grads(False)
+        return _gated_scan_raw(x, g, h0, both, want_final)
+
+    @staticmethod
+    def backward(ctx, d_o, d_final):
+        lib = _lib.load()
+        x, g, h0 = ctx.saved_tensors
+        x, g, both = _scan_rows(x), _scan_rows(g), ctx.both
+        h0 = h0.contiguous() if h0 is not None else None
+        B, L, D = x.shape
+        dense = lambda dtype, n: torch.empty(n, L, D, dtype=dtype, device=x.device)  # noqa: E731
+        d_o = d_o.contiguous() if d_o is not None else torch.zeros_like(dense(x.dtype, B))
+        d_final = d_final.contiguous() if d_final is not None else None
+        dx, dg = dense(x.dtype, B), dense(g.dtype, 2 * B if both else B)
+        dh0 = torch.empty_like(h0) if h0 is not None and ctx.needs_input_grad[2] else None
+        need = lib.vig_gated_scan_bwd_workspace(B, L, D, int(both))
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        with torch.cuda.device(x.device):
+            rc = lib.vig_gated_scan_bwd(ptr(x), ptr(g), _second_gates(g, both), ptr(h0), ptr(d_o), ptr(d_final), ptr(dx), ptr(dg), _second_gates(dg, both),
+                                        ptr(dh0), ptr(ws), need, B, L, D, _scan_strides(x), _scan_strides(g), 0.5 if both else 1.0, _dt(x), _dt(g),
+                                        _stream_ptr(x))
+        _lib.check(rc, "vig_gated_scan_bwd")
+        return dx, dg, dh0, None, None
+
+
+# ---------------------------------------------------------------------------
+# the update of a training step
+# ---------------------------------------------------------------------------
+
+def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(norm, scale) of a list of tensors on one device as fp32 numbers there: the root of the sum of all squares (added up in fp64, in a fixed order) and, where
+    max_norm is given, min(1, max_norm / (norm + 1e-6)), the factor that clips to it; NaN where the norm is not finite, with which
+    adamw_step leaves everything as it is.  Nothing waits for the GPU."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no tensors")
+    if max_norm is not None and not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative; got {max_norm}")
+    calls = _ext.calls()
+    if calls is not None:
+        r = calls.grad_norm(grads, max_norm)
+        if r is not None:
+            return r
+    lib = _lib.load()
+    _check_cuda(*grads)
+    grads = [t.detach() if _gapless(t) else t.detach().contiguous() for t in grads]
+    dev = grads[0].device
+    n, dtypes = _longs([t.numel() for t in grads]), _ints([_dt(t) for t in grads])
+    need = lib.vig_grad_norm_workspace(n, len(grads))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    scale = torch.empty_like(norm) if max_norm is not None else None
+    with torch.cuda.device(dev):
+        rc = lib.vig_grad_norm(_pointers(grads), n, dtypes, len(grads), float(max_norm or 0.0), norm.data_ptr(), scale.data_ptr() if scale is not None else None,
+                               ws.data_ptr(), need, _stream_ptr(norm))
+    _lib.check(rc, "vig_grad_norm")
+    return norm, scale
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
+               avg_scales: Optional[Sequence[torch.Tensor]] = None, sq_scales: Optional[Sequence[torch.Tensor]] = None, *, step, lr=1e-3,
+               betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, grad_scale: Optional[torch.Tensor] = None,
+               seed: int = 0) -> None:
+    """One AdamW step over lists of tensors, in place, in a few launches whatever their number:
+
+        m <- b1 m + (1-b1) g,  v <- b2 v + (1-b2) g^2,  p <- p (1 - lr decay) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps),  g = grad_scale grad
+
+    params and grads in fp32 or bf16, in any mixture; a tensor's moments lie as it does.  Without scales exp_avgs, exp_avg_sqs are m and v in fp32.  With scales
+    the states are held in 8 bits: exp_avgs m and exp_avg_sqs sqrt(v) as torch.float8_e4m3fn, times avg_scales[j], sq_scales[j], a
+    float32 number for each 256 elements of tensor j (ceil(n/256) of them); all zeros is where they begin.  A block that takes in a value that is not finite is
+    NaN from then on.  States in 8 bits and bf16 parameters are rounded stochastically, by a word made of seed, step and the element's
+    number in the list: the same calls give the same bits.
+    step counts from 1; it and lr may be int64 and float32 numbers on the device (a captured step).  grad_scale: a float32 number there, as grad_norm gives it; NaN
+    leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient."""
+    params, grads, exp_avgs, exp_avg_sqs = (list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
+    if not params:
+        return
+    calls = _ext.calls()
+    if calls is not None and calls.adamw(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed):
+        return
+    lib = _lib.load()
+    bits8 = avg_scales is not None
+    if bits8 != (sq_scales is not None):
+        raise ValueError("states in 8 bits take scales for both moments")
+    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([list(avg_scales), list(sq_scales)] if bits8 else [])
+    if any(len(t) != len(params) for t in lists):
+        raise ValueError("lists of different lengths")
+    _check_cuda(*(t for some in lists for t in some))
+    dev = params[0].device
+    for name, t, dtype in (("step", step, torch.int64), ("lr", lr, torch.float32), ("grad_scale", grad_scale, torch.float32)):
+        if isinstance(t, torch.Tensor) and (t.dtype != dtype or t.numel() != 1 or t.device != dev):
+            raise ValueError(f"{name} must be one {dtype} number on the tensors' device")
+    on_device = lambda t: t.data_ptr() if isinstance(t, torch.Tensor) else None  # noqa: E731
+    if on_device(step) is None and step < 1:
+        raise ValueError(f"step counts from 1; got {step}")
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+        raise ValueError(f"betas must lie in [0, 1) and eps must not be negative; got {betas}, {eps}")
+    kept = []
+    for j, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if g.shape != p.shape or m.shape != p.shape or v.shape != p.shape:
+            raise ValueError(f"tensor {j}: parameter, gradient and moments must have the same shape")
+        if not _gapless(p) or not _alike(m, p) or not _alike(v, p):
+            raise ValueError(f"tensor {j}: a parameter must lie without gaps, and its moments as it does")
+        if m.dtype != v.dtype or m.dtype != (torch.float8_e4m3fn if bits8 else torch.float32):
+            raise TypeError(f"tensor {j}: moments must be {'float8_e4m3fn beside scales' if bits8 else 'float32'}")
+        if bits8 and any(s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != -(-p.numel() // 256) for s in (lists[4][j], lists[5][j])):
+            raise ValueError(f"tensor {j}: scales must be contiguous float32, one for each 256 elements")
+        g = g.detach()
+        kept.append(g if _alike(g, p) else torch.empty_like(p, dtype=g.dtype).copy_(g))
+    n, p_dt, g_dt = _longs([t.numel() for t in params]), _ints([_dt(t) for t in params]), _ints([_dt(t) for t in kept])
+    with torch.cuda.device(dev):
+        rc = lib.vig_adamw_many(_pointers(params), _pointers(kept), _pointers(exp_avgs), _pointers(exp_avg_sqs), _pointers(lists[4]) if bits8 else None,
+                                _pointers(lists[5]) if bits8 else None, n, p_dt, g_dt, len(params), 8 if bits8 else 32, 0.0 if on_device(lr) else float(lr),
+                                betas[0], betas[1], eps, weight_decay, 1 if on_device(step) else step, on_device(lr), on_device(step), on_device(grad_scale),
+                                seed & (2 ** 64 - 1), _stream_ptr(params[0]))
+    if rc == _lib.VIG_EINVAL:
+        raise ValueError("tensors that are written overlap one another or a gradient (a parameter twice in the list?)")
+    _lib.check(rc, "vig_adamw_many")
+    torch.autograd.graph.increment_version([t for some in [lists[0]] + lists[2:] for t in some if not t.is_inference()])
+
+
+def _gapless(t):
+    """Whether t's elements fill a stretch of memory, in whatever order of the axes."""
+    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
+
+
+def _alike(a, b):
+    """Whether two tensors' elements lie in the same order, without gaps."""
+    return a.shape == b.shape and (a.is_contiguous() if b.is_contiguous() else _gapless(a) and a.stride() == b.stride())
+
+
+def _pointers(ts):
+    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+
+
+def _longs(v):
+    return (ctypes.c_longlong * len(v))(*v)
+
+
+def _ints(v):
+    return (ctypes.c_int * len(v))(*v)
