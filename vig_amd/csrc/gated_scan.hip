@@ -5,8 +5,8 @@
 //
 // What a run of tokens does to the state that enters it is an affine map per channel, h -> A h + S, and maps compose in any grouping:
 //   (A, S) then (A', S')  =  (A A', A' S + S').
-// A thread folds the eight tokens that it holds in registers, a wave its four threads of a channel by shuffles, a workgroup its waves through LDS;
-// then every thread knows the state that enters its tokens and walks them once more, which costs one fused multiply-add a value.  Memory is what
+// A thread folds the eight tokens that it holds in registers, a wave its four threads of a channel by swaps of lane rows, a workgroup its waves through
+// LDS; then every thread knows the state that enters its tokens and walks them once more, which costs one fused multiply-add a value.  Memory is what
 // bounds it: rows and gates are read once.  Sequences that one workgroup does not hold are cut in chunks: a first launch folds the chunks
 // (reads everything once, writes 8 bytes a chunk and channel), the second folds the chunks in front of its own and walks.
 //
@@ -23,24 +23,24 @@ namespace {
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 constexpr unsigned kBeyond = 0x40000000u;  // byte offset that no descriptor here covers (kScanRow)
 constexpr int kTokens = 8;                 // of a thread
+constexpr int kLanes = 16;                 // that take a token's channels
+constexpr int kRuns = 64 / kLanes;         // of tokens in a wave
 constexpr int kMaxWaves = 16;
 
 // N consecutive channels of one token as stored
 template <typename T, int N> struct Piece;
-template <> struct Piece<uint16_t, 4> {
+template <> struct Piece<uint16_t, 2> {
+  uint32_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+  __device__ __forceinline__ float get(int i) const { return i ? bf16hi_to_f32(v) : bf16lo_to_f32(v); }
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[2]) { __builtin_amdgcn_raw_buffer_store_b32(pack_bf16x2(x[0], x[1]), r, off, 0, 0); }
+};
+template <> struct Piece<float, 2> {
   u32x2_t v;
   __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); }
-  __device__ __forceinline__ float get(int i) const { return i & 1 ? bf16hi_to_f32(v[i >> 1]) : bf16lo_to_f32(v[i >> 1]); }
-  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[4]) {
-    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])}, r, off, 0, 0);
-  }
-};
-template <> struct Piece<float, 4> {
-  u32x4_t v;
-  __device__ __forceinline__ void load(rsrc_t r, unsigned off) { v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(v[i]); }
-  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[4]) {
-    __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])}, r, off, 0, 0);
+  static __device__ __forceinline__ void store(rsrc_t r, unsigned off, const float (&x)[2]) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(x[0]), __float_as_uint(x[1])}, r, off, 0, 0);
   }
 };
 template <> struct Piece<uint16_t, 1> {
@@ -78,53 +78,57 @@ template <int N> struct Map {
   }
 };
 
-template <bool UP, int N>
-__device__ __forceinline__ Map<N> shifted(const Map<N>& m, int lanes) {
-  Map<N> r;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    r.a[i] = UP ? __shfl_up(m.a[i], lanes) : __shfl_down(m.a[i], lanes);
-    r.s[i] = UP ? __shfl_up(m.s[i], lanes) : __shfl_down(m.s[i], lanes);
-  }
-  return r;
-}
-
-// Where a thread stands: LPR lanes side by side take a token's channels, 64 / LPR runs of tokens lie behind one another in a wave.
-template <int N, int LPR> struct Place {
+// Where a thread stands: sixteen lanes side by side take a token's channels, the wave's four rows of lanes four runs of tokens behind one another.
+struct Place {
   int wave, waves, lane, run, lc;  // lc: lane of the token's channels
   __device__ __forceinline__ Place()
-      : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), run((threadIdx.x & 63) / LPR), lc(threadIdx.x % LPR) {}
+      : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), run((threadIdx.x & 63) / kLanes), lc(threadIdx.x % kLanes) {}
 };
 
 // LDS of one direction: each wave's map of a channel
-template <int N, int LPR> struct Board {
-  alignas(8 * N) float v[kMaxWaves][LPR][2 * N];
+template <int N> struct Board {
+  alignas(8 * N) float v[kMaxWaves][kLanes][2 * N];
 };
+
+// A map's values in the lower and the upper of each two rows of lanes (HALVES: of the wave's halves), in both of them
+template <bool HALVES, int N>
+__device__ __forceinline__ void both_of(const Map<N>& m, Map<N>& low, Map<N>& high) {
+  auto swap = [](float x, float& l, float& h) {
+    const unsigned v = __float_as_uint(x);
+    const auto r = HALVES ? __builtin_amdgcn_permlane32_swap(v, v, false, false) : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    l = __uint_as_float(r[0]), h = __uint_as_float(r[1]);
+  };
+#pragma unroll
+  for (int i = 0; i < N; ++i) swap(m.a[i], low.a[i], high.a[i]), swap(m.s[i], low.s[i], high.s[i]);
+}
 
 // Folds the threads' maps along a wave.  UP: tokens in their order; else against it.  Leaves in `m` the map of what lies in front of this
 // thread in its wave, and the whole wave's on the board.
-template <bool UP, int N, int LPR>
-__device__ __forceinline__ void fold_wave(Map<N>& m, const Place<N, LPR>& at, Board<N, LPR>& board) {
+template <bool UP, int N>
+__device__ __forceinline__ void fold_wave(Map<N>& m, const Place& at, Board<N>& board) {
+  Map<N> low, high, first, second;
+  both_of<false>(m, low, high);
+  const bool behind = UP ? at.run & 1 : !(at.run & 1), last = UP ? at.run >= 2 : at.run < 2;
 #pragma unroll
-  for (int d = LPR; d < 64; d *= 2) {
-    const Map<N> p = shifted<UP, N>(m, d);
-    if (UP ? at.lane >= d : at.lane + d < 64) m.behind(p);
+  for (int i = 0; i < N; ++i) m.a[i] = behind ? (UP ? low : high).a[i] : 1.f, m.s[i] = behind ? (UP ? low : high).s[i] : 0.f;
+  if (UP) high.behind(low);
+  else low.behind(high);
+  both_of<true>(UP ? high : low, first, second);  // (the halves' maps)
+  if (!UP) {
+    const Map<N> t = first;
+    first = second, second = t;
   }
-  if (UP ? at.lane >= 64 - LPR : at.lane < LPR) {
+  if (last) m.behind(first);
+  second.behind(first);
+  if (at.lane < kLanes) {
     float* to = board.v[at.wave][at.lc];
 #pragma unroll
-    for (int i = 0; i < N; ++i) to[2 * i] = m.a[i], to[2 * i + 1] = m.s[i];
-  }
-  if constexpr (LPR < 64) {
-    m = shifted<UP, N>(m, LPR);
-    if (UP ? at.lane < LPR : at.lane >= 64 - LPR) m.identity();
-  } else {
-    m.identity();
+    for (int i = 0; i < N; ++i) to[2 * i] = second.a[i], to[2 * i + 1] = second.s[i];
   }
 }
 // (behind the barrier) h: state that enters the workgroup -> the one that enters this thread's tokens
-template <bool UP, int N, int LPR>
-__device__ __forceinline__ void enter(float (&h)[N], const Map<N>& m, const Place<N, LPR>& at, const Board<N, LPR>& board) {
+template <bool UP, int N>
+__device__ __forceinline__ void enter(float (&h)[N], const Map<N>& m, const Place& at, const Board<N>& board) {
   for (int w = UP ? 0 : at.waves - 1; w != at.wave; w += UP ? 1 : -1) {
     const float* from = board.v[w][at.lc];
 #pragma unroll
@@ -133,8 +137,8 @@ __device__ __forceinline__ void enter(float (&h)[N], const Map<N>& m, const Plac
   m.apply(h);
 }
 // (behind the barrier) the map of the whole workgroup
-template <bool UP, int N, int LPR>
-__device__ __forceinline__ Map<N> whole(const Place<N, LPR>& at, const Board<N, LPR>& board) {
+template <bool UP, int N>
+__device__ __forceinline__ Map<N> whole(const Place& at, const Board<N>& board) {
   Map<N> t;
   t.identity();
   for (int k = 0; k < at.waves; ++k) {
@@ -156,11 +160,14 @@ struct ScanArgs {
   float scale;
 };
 
-// The workgroup's piece of the tensors
+// The workgroup's piece of the tensors.  Workgroups go round the eight XCDs: each of them takes a stretch of neighbouring pieces, so that the halves of a
+// 128-byte line are met in one L2.
 struct Tile {
   int b, ch, cg, t0, rows;
   __device__ __forceinline__ Tile(const ScanArgs& p) {
+    const unsigned each = gridDim.x / 8;
     unsigned id = blockIdx.x;
+    if (id < 8 * each) id = id % 8 * each + id / 8;
     const unsigned q = id / (unsigned)p.groups;
     cg = (int)(id - q * p.groups);
     b = (int)(q / (unsigned)p.chunks);
@@ -188,30 +195,41 @@ __device__ __forceinline__ void load_run(Piece<T, N> (&raw)[kTokens], rsrc_t r, 
   for (int t = 0; t < kTokens; ++t) raw[t].load(r, first + t * pitch);
 }
 
-// A thread's map along its tokens (h -> a h + x) or against them; BACK: h -> a (h + scale x), what gradients do
-template <bool UP, bool BACK, typename T, int N>
-__device__ __forceinline__ Map<N> fold_run(const float (&a)[kTokens][N], const Piece<T, N> (&x)[kTokens], float scale = 1.f) {
+// A thread's map along its tokens, h -> a h + x
+template <bool UP, typename T, int N>
+__device__ __forceinline__ Map<N> fold_run(const float (&a)[kTokens][N], const Piece<T, N> (&x)[kTokens]) {
   Map<N> m;
   m.identity();
 #pragma unroll
   for (int k = 0; k < kTokens; ++k) {
     const int t = UP ? k : kTokens - 1 - k;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      m.s[i] = BACK ? a[t][i] * fmaf(scale, x[t].get(i), m.s[i]) : fmaf(a[t][i], m.s[i], x[t].get(i));
-      m.a[i] *= a[t][i];
-    }
+    for (int i = 0; i < N; ++i) m.s[i] = fmaf(a[t][i], m.s[i], x[t].get(i)), m.a[i] *= a[t][i];
+  }
+  return m;
+}
+// ... and the gradient's against them, h -> a (h + scale y), whose factor is the same
+template <bool UP, typename T, int N>
+__device__ __forceinline__ Map<N> fold_back(const float (&a)[kTokens][N], const Piece<T, N> (&y)[kTokens], float scale, const Map<N>& along) {
+  Map<N> m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m.a[i] = along.a[i], m.s[i] = 0.f;
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) {
+    const int t = UP ? k : kTokens - 1 - k;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m.s[i] = a[t][i] * fmaf(scale, y[t].get(i), m.s[i]);
   }
   return m;
 }
 
 // The state that enters this workgroup's chunk from the chunks in front of it: each of the workgroup's runs folds a
 // stretch of them, and the runs fold as tokens do.
-template <bool UP, int N, int LPR>
-__device__ __forceinline__ Map<N> fold_chunks(const ScanArgs& p, const Tile& tile, const Place<N, LPR>& at, int dir, int dirs, int c, bool has) {
+template <bool UP, int N>
+__device__ __forceinline__ Map<N> fold_chunks(const ScanArgs& p, const Tile& tile, const Place& at, int dir, int dirs, int c, bool has) {
   const int n = UP ? tile.ch : p.chunks - 1 - tile.ch;  // chunks in front
-  const int runs = at.waves * (64 / LPR), each = (n + runs - 1) / runs;
-  const int slot = at.wave * (64 / LPR) + at.run;
+  const int runs = at.waves * kRuns, each = (n + runs - 1) / runs;
+  const int slot = at.wave * kRuns + at.run;
   // (runs in the order of the tokens; against it the last run comes first)
   const int first = UP ? slot * each : tile.ch + 1 + slot * each, end = min(first + each, UP ? n : p.chunks);
   const float* from = p.maps + (((size_t)tile.b * dirs + dir) * p.chunks) * p.D * 2;
@@ -221,11 +239,10 @@ __device__ __forceinline__ Map<N> fold_chunks(const ScanArgs& p, const Tile& til
     const int j = UP ? first + k : end - 1 - k;
     if (j < first || j >= end || !has) continue;
     const float* v = from + ((size_t)j * p.D + c) * 2;
-    if constexpr (N == 4) {
-      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(v), hi = *reinterpret_cast<const f32x4_t*>(v + 4);
-      const float a[4] = {lo[0], lo[2], hi[0], hi[2]}, s[4] = {lo[1], lo[3], hi[1], hi[3]};
+    if constexpr (N == 2) {
+      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) m.s[i] = fmaf(a[i], m.s[i], s[i]), m.a[i] *= a[i];
+      for (int i = 0; i < N; ++i) m.s[i] = fmaf(w[2 * i], m.s[i], w[2 * i + 1]), m.a[i] *= w[2 * i];
     } else {
       m.s[0] = fmaf(v[0], m.s[0], v[1]), m.a[0] *= v[0];
     }
@@ -251,14 +268,14 @@ __device__ __forceinline__ void store_state(float* to, const float (&h)[N], cons
 
 // ---- forward.  FOLD: only the chunks' maps
 
-template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int LPR>
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) {
-  __shared__ Board<N, LPR> board[BOTH ? 2 : 1], front[FOLD ? 1 : BOTH ? 2 : 1];
-  const Place<N, LPR> at;
+  __shared__ Board<N> board[BOTH ? 2 : 1], front[FOLD ? 1 : BOTH ? 2 : 1];
+  const Place at;
   const Tile tile(p);
-  const int c = (tile.cg * LPR + at.lc) * N;
+  const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
-  const int first = (at.wave * (64 / LPR) + at.run) * kTokens;
+  const int first = (at.wave * kRuns + at.run) * kTokens;
   auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
   Piece<TX, N> x[kTokens];
   Piece<TG, N> raw[kTokens];
@@ -271,46 +288,46 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
   [[maybe_unused]] Map<N> before, after;
   if constexpr (!FOLD) {
     if (p.chunks > 1) {
-      before = fold_chunks<true, N, LPR>(p, tile, at, 0, dirs, c, has);
-      fold_wave<true, N, LPR>(before, at, front[0]);
+      before = fold_chunks<true, N>(p, tile, at, 0, dirs, c, has);
+      fold_wave<true, N>(before, at, front[0]);
       if constexpr (BOTH) {
-        after = fold_chunks<false, N, LPR>(p, tile, at, 1, dirs, c, has);
-        fold_wave<false, N, LPR>(after, at, front[BOTH ? 1 : 0]);
+        after = fold_chunks<false, N>(p, tile, at, 1, dirs, c, has);
+        fold_wave<false, N>(after, at, front[BOTH ? 1 : 0]);
       }
     }
   }
   factors(raw, a);
-  Map<N> m = fold_run<true, false>(a, x), m2;
-  fold_wave<true, N, LPR>(m, at, board[0]);
+  Map<N> m = fold_run<true>(a, x), m2;
+  fold_wave<true, N>(m, at, board[0]);
   if constexpr (BOTH) {
     factors(raw2, a2);
-    m2 = fold_run<false, false>(a2, x);
-    fold_wave<false, N, LPR>(m2, at, board[BOTH ? 1 : 0]);
+    m2 = fold_run<false>(a2, x);
+    fold_wave<false, N>(m2, at, board[BOTH ? 1 : 0]);
   }
   __syncthreads();
   if constexpr (FOLD) {
     if (at.wave == 0 && at.run == 0 && has) {
-      store_map(p, tile, 0, dirs, c, whole<true, N, LPR>(at, board[0]));
-      if constexpr (BOTH) store_map(p, tile, 1, dirs, c, whole<false, N, LPR>(at, board[BOTH ? 1 : 0]));
+      store_map(p, tile, 0, dirs, c, whole<true, N>(at, board[0]));
+      if constexpr (BOTH) store_map(p, tile, 1, dirs, c, whole<false, N>(at, board[BOTH ? 1 : 0]));
     }
     return;
   }
   float h[N], y[kTokens][N];
   load_state(h, p.h0, p, tile.b, c, has);
-  if (p.chunks > 1) whole<true, N, LPR>(at, front[0]).apply(h);
-  enter<true, N, LPR>(h, m, at, board[0]);
+  if (p.chunks > 1) whole<true, N>(at, front[0]).apply(h);
+  enter<true, N>(h, m, at, board[0]);
 #pragma unroll
   for (int t = 0; t < kTokens; ++t)
 #pragma unroll
     for (int i = 0; i < N; ++i) y[t][i] = h[i] = fmaf(a[t][i], h[i], x[t].get(i));
   // (tokens behind the sequence change nothing: the last run ends with the state behind its last token)
-  if (p.hT && tile.ch == p.chunks - 1 && at.wave == at.waves - 1 && at.run == 64 / LPR - 1 && has) store_state(p.hT, h, p, tile.b, c);
+  if (p.hT && tile.ch == p.chunks - 1 && at.wave == at.waves - 1 && at.run == kRuns - 1 && has) store_state(p.hT, h, p, tile.b, c);
   if constexpr (BOTH) {
     float r[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) r[i] = 0.f;
-    if (p.chunks > 1) whole<false, N, LPR>(at, front[BOTH ? 1 : 0]).apply(r);
-    enter<false, N, LPR>(r, m2, at, board[BOTH ? 1 : 0]);
+    if (p.chunks > 1) whole<false, N>(at, front[BOTH ? 1 : 0]).apply(r);
+    enter<false, N>(r, m2, at, board[BOTH ? 1 : 0]);
 #pragma unroll
     for (int t = kTokens - 1; t >= 0; --t)
 #pragma unroll
@@ -328,15 +345,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
 
 // ---- backward
 
-template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int LPR>
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs p) {
   constexpr int dirs = BOTH ? 4 : 2;
-  __shared__ Board<N, LPR> board[dirs], front[FOLD ? 1 : dirs];
-  const Place<N, LPR> at;
+  __shared__ Board<N> board[dirs], front[FOLD ? 1 : dirs];
+  const Place at;
   const Tile tile(p);
-  const int c = (tile.cg * LPR + at.lc) * N;
+  const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
-  const int first = (at.wave * (64 / LPR) + at.run) * kTokens;
+  const int first = (at.wave * kRuns + at.run) * kTokens;
   auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
   const long long dense = (long long)p.L * p.D;
   Piece<TX, N> x[kTokens], dy[kTokens];
@@ -353,12 +370,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
       // (only the boards are wanted)
 #pragma unroll
       for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
-        Map<N> f = w ? fold_chunks<false, N, LPR>(p, tile, at, 2, dirs, c, has) : fold_chunks<true, N, LPR>(p, tile, at, 0, dirs, c, has);
-        if (w) fold_wave<false, N, LPR>(f, at, front[BOTH ? 2 : 0]);
-        else fold_wave<true, N, LPR>(f, at, front[0]);
-        f = w ? fold_chunks<true, N, LPR>(p, tile, at, 3, dirs, c, has) : fold_chunks<false, N, LPR>(p, tile, at, 1, dirs, c, has);
-        if (w) fold_wave<true, N, LPR>(f, at, front[BOTH ? 3 : 0]);
-        else fold_wave<false, N, LPR>(f, at, front[1]);
+        Map<N> f = w ? fold_chunks<false, N>(p, tile, at, 2, dirs, c, has) : fold_chunks<true, N>(p, tile, at, 0, dirs, c, has);
+        if (w) fold_wave<false, N>(f, at, front[BOTH ? 2 : 0]);
+        else fold_wave<true, N>(f, at, front[0]);
+        f = w ? fold_chunks<true, N>(p, tile, at, 3, dirs, c, has) : fold_chunks<false, N>(p, tile, at, 1, dirs, c, has);
+        if (w) fold_wave<true, N>(f, at, front[BOTH ? 3 : 0]);
+        else fold_wave<false, N>(f, at, front[1]);
       }
     }
   }
@@ -366,25 +383,25 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
   for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
     factors(raw[w], a[w]);
     if (w == 0) {
-      along[w] = fold_run<true, false>(a[w], x);
-      fold_wave<true, N, LPR>(along[w], at, board[0]);
-      against[w] = fold_run<false, true>(a[w], dy, p.scale);
-      fold_wave<false, N, LPR>(against[w], at, board[1]);
+      along[w] = fold_run<true>(a[w], x);
+      against[w] = fold_back<false>(a[w], dy, p.scale, along[w]);
+      fold_wave<true>(along[w], at, board[0]);
+      fold_wave<false>(against[w], at, board[1]);
     } else {
-      along[w] = fold_run<false, false>(a[w], x);
-      fold_wave<false, N, LPR>(along[w], at, board[BOTH ? 2 : 0]);
-      against[w] = fold_run<true, true>(a[w], dy, p.scale);
-      fold_wave<true, N, LPR>(against[w], at, board[BOTH ? 3 : 0]);
+      along[w] = fold_run<false>(a[w], x);
+      against[w] = fold_back<true>(a[w], dy, p.scale, along[w]);
+      fold_wave<false>(along[w], at, board[BOTH ? 2 : 0]);
+      fold_wave<true>(against[w], at, board[BOTH ? 3 : 0]);
     }
   }
   __syncthreads();
   if constexpr (FOLD) {
     if (at.wave == 0 && at.run == 0 && has) {
-      store_map(p, tile, 0, dirs, c, whole<true, N, LPR>(at, board[0]));
-      store_map(p, tile, 1, dirs, c, whole<false, N, LPR>(at, board[1]));
+      store_map(p, tile, 0, dirs, c, whole<true, N>(at, board[0]));
+      store_map(p, tile, 1, dirs, c, whole<false, N>(at, board[1]));
       if constexpr (BOTH) {
-        store_map(p, tile, 2, dirs, c, whole<false, N, LPR>(at, board[BOTH ? 2 : 0]));
-        store_map(p, tile, 3, dirs, c, whole<true, N, LPR>(at, board[BOTH ? 3 : 0]));
+        store_map(p, tile, 2, dirs, c, whole<false, N>(at, board[BOTH ? 2 : 0]));
+        store_map(p, tile, 3, dirs, c, whole<true, N>(at, board[BOTH ? 3 : 0]));
       }
     }
     return;
@@ -396,13 +413,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
     load_state(h, w ? nullptr : p.h0, p, tile.b, c, has);
     load_state(d, w ? nullptr : p.dhT, p, tile.b, c, has);
     if (w == 0) {
-      if (p.chunks > 1) whole<true, N, LPR>(at, front[0]).apply(h), whole<false, N, LPR>(at, front[FOLD ? 0 : 1]).apply(d);
-      enter<true, N, LPR>(h, along[w], at, board[0]);
-      enter<false, N, LPR>(d, against[w], at, board[1]);
+      if (p.chunks > 1) whole<true, N>(at, front[0]).apply(h), whole<false, N>(at, front[FOLD ? 0 : 1]).apply(d);
+      enter<true, N>(h, along[w], at, board[0]);
+      enter<false, N>(d, against[w], at, board[1]);
     } else {
-      if (p.chunks > 1) whole<false, N, LPR>(at, front[FOLD || !BOTH ? 0 : 2]).apply(h), whole<true, N, LPR>(at, front[FOLD || !BOTH ? 0 : 3]).apply(d);
-      enter<false, N, LPR>(h, along[w], at, board[BOTH ? 2 : 0]);
-      enter<true, N, LPR>(d, against[w], at, board[BOTH ? 3 : 0]);
+      if (p.chunks > 1) whole<false, N>(at, front[FOLD || !BOTH ? 0 : 2]).apply(h), whole<true, N>(at, front[FOLD || !BOTH ? 0 : 3]).apply(d);
+      enter<false, N>(h, along[w], at, board[BOTH ? 2 : 0]);
+      enter<true, N>(d, against[w], at, board[BOTH ? 3 : 0]);
     }
 #pragma unroll
     for (int k = 0; k < kTokens; ++k) {
@@ -471,22 +488,20 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const TX* x, const
 // ---- host side
 
 struct Cut {
-  int lanes, channels, waves, chunks, chunk, groups;
+  int waves, chunks, chunk, groups;
 };
-// Whether four channels move at once: whole quads in every row, on boundaries of their size (a null pointer stands on any)
-inline bool quads(int D, long long a, long long b, long long c, long long d) { return D % 4 == 0 && (a | b | c | d) % 4 == 0; }
+// Whether N channels move at once: whole ones of them in every row, on boundaries of their size (a null pointer stands on any)
+inline bool whole(int n, int D, long long a, long long b, long long c, long long d) { return D % n == 0 && (a | b | c | d) % n == 0; }
 template <typename... P>
-bool on_quads(int dtype, P... p) {
-  const uintptr_t size = dtype == VIG_BF16 ? 8 : 16;
+bool on(int n, int dtype, P... p) {
+  const uintptr_t size = n * (dtype == VIG_BF16 ? 2 : 4);
   return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...);
 }
 
-inline Cut cut(int B, int L, int D, bool vector) {
+inline Cut cut(int B, int L, int D, bool pairs) {
   Cut k;
-  k.channels = vector ? 4 : 1;
-  k.lanes = vector ? 16 : 64;
-  k.groups = (D + 63) / 64;
-  const int run = 64 / k.lanes * kTokens;  // tokens of a wave
+  const int tile = kLanes * (pairs ? 2 : 1), run = kRuns * kTokens;  // channels of a workgroup, tokens of a wave
+  k.groups = (D + tile - 1) / tile;
   const int waves = (L + run - 1) / run;
   k.chunks = (waves + kMaxWaves - 1) / kMaxWaves;
   k.waves = (waves + k.chunks - 1) / k.chunks;
@@ -495,40 +510,40 @@ inline Cut cut(int B, int L, int D, bool vector) {
   return k;
 }
 
-template <typename TX, typename TG, bool BOTH, int N, int LPR>
+template <typename TX, typename TG, bool BOTH, int N>
 void start(const ScanArgs& p, bool bwd, bool fold, dim3 grid, dim3 block, hipStream_t stream) {
   if (bwd) {
-    if (fold) hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, true, N, LPR>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, false, N, LPR>), grid, block, 0, stream, p);
+    if (fold) hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, true, N>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, false, N>), grid, block, 0, stream, p);
   } else {
-    if (fold) hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, true, N, LPR>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, false, N, LPR>), grid, block, 0, stream, p);
+    if (fold) hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, true, N>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, false, N>), grid, block, 0, stream, p);
   }
 }
 template <typename TX, typename TG>
-void start(const ScanArgs& p, bool bwd, bool fold, bool vector, dim3 grid, dim3 block, hipStream_t stream) {
+void start(const ScanArgs& p, bool bwd, bool fold, bool pairs, dim3 grid, dim3 block, hipStream_t stream) {
   if (p.g[1]) {
-    if (vector) start<TX, TG, true, 4, 16>(p, bwd, fold, grid, block, stream);
-    else start<TX, TG, true, 1, 64>(p, bwd, fold, grid, block, stream);
+    if (pairs) start<TX, TG, true, 2>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, true, 1>(p, bwd, fold, grid, block, stream);
   } else {
-    if (vector) start<TX, TG, false, 4, 16>(p, bwd, fold, grid, block, stream);
-    else start<TX, TG, false, 1, 64>(p, bwd, fold, grid, block, stream);
+    if (pairs) start<TX, TG, false, 2>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, false, 1>(p, bwd, fold, grid, block, stream);
   }
 }
 int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t stream) {
-  const bool vector = quads(p.D, p.xb, p.xl, p.gb, p.gl) && on_quads(io_dtype, p.x, p.d_o, p.o, p.dx) && on_quads(gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
-  const Cut k = cut(B, p.L, p.D, vector);
+  const bool pairs = whole(2, p.D, p.xb, p.xl, p.gb, p.gl) && on(2, io_dtype, p.x, p.d_o, p.o, p.dx) && on(2, gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
+  const Cut k = cut(B, p.L, p.D, pairs);
   p.groups = k.groups, p.chunks = k.chunks, p.chunk = k.chunk;
   const long long groups = (long long)B * k.groups * k.chunks;
   if (groups > 0x7fffffffLL) return VIG_ENOTSUP;
   const dim3 grid((unsigned)groups), block(64 * k.waves);
   for (int fold = k.chunks > 1; fold >= 0; --fold) {
     if (io_dtype == VIG_BF16) {
-      if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, vector, grid, block, stream);
-      else start<uint16_t, float>(p, bwd, fold, vector, grid, block, stream);
+      if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, pairs, grid, block, stream);
+      else start<uint16_t, float>(p, bwd, fold, pairs, grid, block, stream);
     } else {
-      if (gate_dtype == VIG_BF16) start<float, uint16_t>(p, bwd, fold, vector, grid, block, stream);
-      else start<float, float>(p, bwd, fold, vector, grid, block, stream);
+      if (gate_dtype == VIG_BF16) start<float, uint16_t>(p, bwd, fold, pairs, grid, block, stream);
+      else start<float, float>(p, bwd, fold, pairs, grid, block, stream);
     }
     if (hipGetLastError() != hipSuccess) return VIG_ELAUNCH;
   }
@@ -566,7 +581,7 @@ static void start_step(const GatedScanStep& s, bool vector, hipStream_t stream) 
 
 int launch_gated_scan_step(const GatedScanStep& s, hipStream_t stream) {
   if ((long long)s.B * s.D > 0x7fffff00LL) return VIG_ENOTSUP;
-  const bool vector = quads(s.D, s.x_stride, s.g_stride, 0, 0) && on_quads(s.io_dtype, s.x, s.o) && on_quads(s.gate_dtype, s.g) && on_quads(VIG_F32, s.state);
+  const bool vector = whole(4, s.D, s.x_stride, s.g_stride, 0, 0) && on(4, s.io_dtype, s.x, s.o) && on(4, s.gate_dtype, s.g) && on(4, VIG_F32, s.state);
   if (s.io_dtype == VIG_BF16) {
     if (s.gate_dtype == VIG_BF16) start_step<uint16_t, uint16_t>(s, vector, stream);
     else start_step<uint16_t, float>(s, vector, stream);

@@ -145,7 +145,8 @@ __device__ __forceinline__ float store_codes(void* p, size_t i, int left, const 
   uint32_t code[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float y = fabsf(x[k]) * inv;
+    // (a division's bits: the remainder of the quotient by the reciprocal, times it)
+    const float near = fabsf(x[k]) * inv, y = fmaf(fmaf(-near, scale, fabsf(x[k])), inv, near);
     const uint32_t normal = ((__float_as_uint(y) + (bits[k] << 4)) >> 20) - (120u << 3);
     const uint32_t below = (uint32_t)floorf(fmaf(y, 512.f, (float)bits[k] * 0x1p-16f));
     uint32_t q = y >= 0x1p-6f ? normal : below;
@@ -228,9 +229,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(UpdateJobs by_value, UpdateS
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
+      // (products and sums rounded one by one: a last bit can turn a code over, and so the moments' bits are those of their formula)
+#pragma clang fp contract(off)
       const float x = G[k][e] * clip;
-      M[k][e] = fmaf(s.b1, M[k][e], s.c1 * x);
-      V[k][e] = fmaf(s.b2, V[k][e], s.c2 * x * x);
+      M[k][e] = s.b1 * M[k][e] + s.c1 * x;
+      V[k][e] = s.b2 * V[k][e] + s.c2 * x * x;
       root[e] = sqrtf(V[k][e]);
       P[k][e] = fmaf(P[k][e], s.keep, -(s.step * M[k][e] / fmaf(root[e], s.rs2, s.eps)));
     }
