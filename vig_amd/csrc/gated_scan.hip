@@ -164,10 +164,11 @@ struct ScanArgs {
 // 128-byte line are met in one L2.
 struct Tile {
   int b, ch, cg, t0, rows;
-  __device__ __forceinline__ Tile(const ScanArgs& p) {
+  __device__ __forceinline__ Tile(const ScanArgs& p, bool fold) {
     const unsigned each = gridDim.x / 8;
     unsigned id = blockIdx.x;
     if (id < 8 * each) id = id % 8 * each + id / 8;
+    if (!fold && p.chunks > 1) id = gridDim.x - 1 - id;
     const unsigned q = id / (unsigned)p.groups;
     cg = (int)(id - q * p.groups);
     b = (int)(q / (unsigned)p.chunks);
@@ -272,7 +273,7 @@ template <typename TX, typename TG, bool BOTH, bool FOLD, int N>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) {
   __shared__ Board<N> board[BOTH ? 2 : 1], front[FOLD ? 1 : BOTH ? 2 : 1];
   const Place at;
-  const Tile tile(p);
+  const Tile tile(p, FOLD);
   const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
   const int first = (at.wave * kRuns + at.run) * kTokens;
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
   constexpr int dirs = BOTH ? 4 : 2;
   __shared__ Board<N> board[dirs], front[FOLD ? 1 : dirs];
   const Place at;
-  const Tile tile(p);
+  const Tile tile(p, FOLD);
   const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
   const int first = (at.wave * kRuns + at.run) * kTokens;
