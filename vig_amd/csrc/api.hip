@@ -3,6 +3,7 @@
 #include "../../include/vig_gla.h"
 #include "launch.h"
 #include <algorithm>
+#include <iterator>
 #include <mutex>
 #include <vector>
 
@@ -133,26 +134,32 @@ static int scan_arguments(vig::GatedScan& s, void* workspace, int B, int L, int 
   return VIG_OK;
 }
 
-// Whether the tensors that an update writes overlap none of its others (gradients may overlap one another).
+// Whether the tensors that an update writes overlap none of its others (gradients may overlap one another).  Lists of a trainer's tensors are sorted by address
+// as a rule, and the lists are merged: 720 ranges in 4 us where one sort of all takes 25.
 static bool apart(const vig::AdamW& a) {
   struct Range {
     uintptr_t from, to;
     bool written;
   };
-  std::vector<Range> ranges;
-  ranges.reserve((size_t)a.count * (a.state_bits == 8 ? 6 : 4));
-  for (int j = 0; j < a.count; ++j) {
-    const uintptr_t n = (uintptr_t)a.n[j];
-    if (!n) continue;
-    auto add = [&](const void* p, uintptr_t bytes, bool written) { ranges.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written}); };
-    const uintptr_t state = a.state_bits == 8 ? n : 4 * n;
-    add(a.param[j], n * element_size(a.param_dtype[j]), true), add(a.grad[j], n * element_size(a.grad_dtype[j]), false);
-    add(a.exp_avg[j], state, true), add(a.exp_avg_sq[j], state, true);
-    if (a.state_bits == 8) add(a.avg_scale[j], (n + 255) / 256 * 4, true), add(a.sq_scale[j], (n + 255) / 256 * 4, true);
+  const auto before = [](const Range& x, const Range& y) { return x.from < y.from; };
+  std::vector<Range> all, some, both;
+  const size_t lists = a.state_bits == 8 ? 6 : 4;
+  all.reserve(a.count * lists), both.reserve(a.count * lists), some.reserve(a.count);
+  for (size_t k = 0; k < lists; ++k) {
+    some.clear();
+    for (int j = 0; j < a.count; ++j) {
+      const uintptr_t n = (uintptr_t)a.n[j], state = a.state_bits == 8 ? n : 4 * n, scales = (n + 255) / 256 * 4;
+      const void* const p = k == 0 ? a.param[j] : k == 1 ? a.grad[j] : k == 2 ? a.exp_avg[j] : k == 3 ? a.exp_avg_sq[j] : k == 4 ? a.avg_scale[j] : a.sq_scale[j];
+      const uintptr_t bytes = k == 0 ? n * element_size(a.param_dtype[j]) : k == 1 ? n * element_size(a.grad_dtype[j]) : k < 4 ? state : scales;
+      if (n) some.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, k != 1});
+    }
+    if (!std::is_sorted(some.begin(), some.end(), before)) std::sort(some.begin(), some.end(), before);
+    both.clear();
+    std::merge(all.begin(), all.end(), some.begin(), some.end(), std::back_inserter(both), before);
+    all.swap(both);
   }
-  std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.from < y.from; });
   uintptr_t written = 0, any = 0;  // how far the ranges so far reach
-  for (const Range& r : ranges) {
+  for (const Range& r : all) {
     if (r.from < written || (r.written && r.from < any)) return false;
     any = std::max(any, r.to);
     if (r.written) written = std::max(written, r.to);

@@ -156,25 +156,23 @@ PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 namespace {
 
-// the tensors of a list or tuple; false where something else is among them
-bool tensors(PyObject* o, std::vector<Tensor>& out) {
-  PyObject* fast = PySequence_Fast(o, "a list of tensors");
-  if (!fast) {
-    PyErr_Clear();
-    return false;
-  }
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
-  PyObject** items = PySequence_Fast_ITEMS(fast);
+// The tensors of a list, which holds them for the call; false where something else is among them.
+typedef std::vector<const Tensor*> List;
+bool tensors(PyObject* o, List& out) {
+  if (!PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(o);
   out.reserve(n);
-  bool ok = true;
-  for (Py_ssize_t i = 0; i < n && ok; ++i)
-    if ((ok = is_tensor(items[i]))) out.push_back(THPVariable_Unpack(items[i]));
-  Py_DECREF(fast);
-  return ok;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* t = PyList_GET_ITEM(o, i);
+    if (!is_tensor(t)) return false;
+    out.push_back(&THPVariable_Unpack(t));
+  }
+  return true;
 }
 // whether two tensors' elements lie in the same order, without gaps
 bool alike(const Tensor& a, const Tensor& b) {
-  return a.sizes() == b.sizes() && (a.is_contiguous() ? b.is_contiguous() : a.is_non_overlapping_and_dense() && a.strides() == b.strides());
+  return &a == &b ? a.is_non_overlapping_and_dense()
+                  : a.sizes() == b.sizes() && (a.is_contiguous() ? b.is_contiguous() : a.is_non_overlapping_and_dense() && a.strides() == b.strides());
 }
 
 }  // namespace
@@ -184,14 +182,14 @@ bool alike(const Tensor& a, const Tensor& b) {
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 14, "adamw takes 14 arguments");
-  std::vector<Tensor> p, g, m, v, ms, vs;
+  List p, g, m, v, ms, vs;
   const bool bits8 = a[4] != Py_None;
   if (!tensors(a[0], p) || !tensors(a[1], g) || !tensors(a[2], m) || !tensors(a[3], v)) Py_RETURN_NONE;
   if (bits8 && (!tensors(a[4], ms) || !tensors(a[5], vs))) Py_RETURN_NONE;
   const size_t count = p.size();
   if (!count || count > (1u << 30) || g.size() != count || m.size() != count || v.size() != count || (bits8 && (ms.size() != count || vs.size() != count))) Py_RETURN_NONE;
-  if (!simple(p[0]) || observed()) Py_RETURN_NONE;
-  const auto dev = p[0].device();
+  if (!simple(*p[0]) || observed()) Py_RETURN_NONE;
+  const auto dev = p[0]->device();
   auto on_device = [&](PyObject* o, at::ScalarType type, Tensor& t) {  // a number there, or none
     if (!is_tensor(o)) return true;
     t = THPVariable_Unpack(o);
@@ -215,26 +213,26 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::vector<int> pd(count), gd(count);
   const auto state = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
   for (size_t j = 0; j < count; ++j) {
-    for (const Tensor* t : {&p[j], &g[j], &m[j], &v[j]})
-      if (!simple(*t) || t->device() != dev || !alike(*t, p[j])) Py_RETURN_NONE;
-    if (m[j].scalar_type() != state || v[j].scalar_type() != state) Py_RETURN_NONE;
-    sizes[j] = p[j].numel(), pd[j] = dtype_code(p[j]), gd[j] = dtype_code(g[j]);
+    for (const Tensor* t : {p[j], g[j], m[j], v[j]})
+      if (!simple(*t) || t->device() != dev || !alike(*t, *p[j])) Py_RETURN_NONE;
+    if (m[j]->scalar_type() != state || v[j]->scalar_type() != state) Py_RETURN_NONE;
+    sizes[j] = p[j]->numel(), pd[j] = dtype_code(*p[j]), gd[j] = dtype_code(*g[j]);
     if (pd[j] < 0 || gd[j] < 0) Py_RETURN_NONE;
-    pp[j] = p[j].data_ptr(), gp[j] = g[j].const_data_ptr(), mp[j] = m[j].data_ptr(), vp[j] = v[j].data_ptr();
+    pp[j] = p[j]->data_ptr(), gp[j] = g[j]->const_data_ptr(), mp[j] = m[j]->data_ptr(), vp[j] = v[j]->data_ptr();
     if (!bits8) continue;
-    for (const Tensor* t : {&ms[j], &vs[j]})
+    for (const Tensor* t : {ms[j], vs[j]})
       if (!simple(*t) || t->device() != dev || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != (sizes[j] + 255) / 256) Py_RETURN_NONE;
-    msp[j] = ms[j].data_ptr<float>(), vsp[j] = vs[j].data_ptr<float>();
+    msp[j] = ms[j]->data_ptr<float>(), vsp[j] = vs[j]->data_ptr<float>();
   }
   const c10::DeviceGuard guard(dev);
   const int rc = vig_adamw_many(pp.data(), gp.data(), mp.data(), vp.data(), msp.data(), vsp.data(), sizes.data(), pd.data(), gd.data(), (int)count, bits8 ? 8 : 32, x[0],
                                 x[1], x[2], x[3], x[4], step, lr_t.defined() ? lr_t.const_data_ptr<float>() : nullptr,
                                 step_t.defined() ? reinterpret_cast<const long long*>(step_t.const_data_ptr<int64_t>()) : nullptr,
-                                scale_t.defined() ? scale_t.const_data_ptr<float>() : nullptr, seed, stream_of(p[0]));
+                                scale_t.defined() ? scale_t.const_data_ptr<float>() : nullptr, seed, stream_of(*p[0]));
   if (rc == VIG_EINVAL) Py_RETURN_NONE;
   check_rc(rc, "vig_adamw_many");
-  for (const auto* list : {&p, &m, &v, &ms, &vs})
-    for (const Tensor& t : *list) written(t);
+  for (const List* list : {&p, &m, &v, &ms, &vs})
+    for (const Tensor* t : *list) written(*t);
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -243,28 +241,30 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 2, "grad_norm takes 2 arguments");
-  std::vector<Tensor> g;
-  if (!tensors(a[0], g) || g.empty() || g.size() > (1u << 30) || !simple(g[0]) || observed()) Py_RETURN_NONE;
+  List list;
+  if (!tensors(a[0], list) || list.empty() || list.size() > (1u << 30) || !simple(*list[0]) || observed()) Py_RETURN_NONE;
+  const Tensor& like = *list[0];
   const bool clip = a[1] != Py_None;
   const double most = clip ? PyFloat_AsDouble(a[1]) : 0.0;
   if (PyErr_Occurred()) return nullptr;
-  const size_t count = g.size();
+  const size_t count = list.size();
   std::vector<const void*> gp(count);
   std::vector<long long> sizes(count);
   std::vector<int> gd(count);
   for (size_t j = 0; j < count; ++j) {
-    if (!simple(g[j]) || g[j].device() != g[0].device() || !g[j].is_non_overlapping_and_dense()) Py_RETURN_NONE;
-    gp[j] = g[j].const_data_ptr(), sizes[j] = g[j].numel(), gd[j] = dtype_code(g[j]);
+    const Tensor& g = *list[j];
+    if (!simple(g) || g.device() != like.device() || !g.is_non_overlapping_and_dense()) Py_RETURN_NONE;
+    gp[j] = g.const_data_ptr(), sizes[j] = g.numel(), gd[j] = dtype_code(g);
     if (gd[j] < 0) Py_RETURN_NONE;
   }
-  const c10::DeviceGuard guard(g[0].device());
-  const auto options = g[0].options().dtype(at::kFloat);
+  const c10::DeviceGuard guard(like.device());
+  const auto options = like.options().dtype(at::kFloat);
   const size_t need = vig_grad_norm_workspace(sizes.data(), (int)count);
-  const Tensor ws = bytes_like(need, g[0]);
+  const Tensor ws = bytes_like(need, like);
   Tensor norm = at::empty({}, options), scale;
   if (clip) scale = at::empty({}, options);
   const int rc = vig_grad_norm(gp.data(), sizes.data(), gd.data(), (int)count, (float)most, norm.data_ptr<float>(), clip ? scale.data_ptr<float>() : nullptr, ws.data_ptr(),
-                               need, stream_of(g[0]));
+                               need, stream_of(like));
   if (rc == VIG_EINVAL) Py_RETURN_NONE;
   check_rc(rc, "vig_grad_norm");
   PyObject* pair = PyTuple_New(2);

@@ -1258,6 +1258,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     step counts from 1; it and lr may be int64 and float32 numbers on the device (a captured step).  grad_scale: a float32 number there, as grad_norm gives it; NaN
     leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient."""
     params, grads, exp_avgs, exp_avg_sqs = (list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
+    avg_scales, sq_scales = (None if t is None else list(t) for t in (avg_scales, sq_scales))
     if not params:
         return
     calls = _ext.calls()
@@ -1267,7 +1268,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     bits8 = avg_scales is not None
     if bits8 != (sq_scales is not None):
         raise ValueError("states in 8 bits take scales for both moments")
-    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([list(avg_scales), list(sq_scales)] if bits8 else [])
+    lists = [params, grads, exp_avgs, exp_avg_sqs] + ([avg_scales, sq_scales] if bits8 else [])
     if any(len(t) != len(params) for t in lists):
         raise ValueError("lists of different lengths")
     _check_cuda(*(t for some in lists for t in some))
