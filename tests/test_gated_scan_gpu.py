@@ -120,6 +120,48 @@ def test_against_the_recurrence(B, L, D, types, both):
 
 
 @pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("B,L,D", [(300, 1, 64), (260, 8, 64), (300, 15, 64), (257, 16, 64), (300, 17, 64), (130, 40, 120), (256, 196, 64), (64, 197, 256), (258, 255, 64), (256, 256, 64)])
+def test_many_short_sequences(B, L, D, both):
+    """bf16 rows that move 16 bytes a lane, from 256 workgroups on."""
+    announce(f"gated scan, many: B{B} L{L} D{D} both={both}")
+    x, g, h0, do, dh = draw(B, L, D, BF16, BF16, both, B + L, strong=L % 2 == 0, state=not both)
+    wide = torch.randn(B, L + 2, D + 16, device="cuda").bfloat16()
+    rows = wide[:, 1:L + 1, 8:D + 8]  # (the same rows in the columns of wider ones, on 16-byte boundaries)
+    rows.copy_(x)
+    for rows in (x, rows):
+        given = [t.detach().requires_grad_() for t in ((rows, g) if both else (rows, g, h0))]
+        o, h = vig_amd.bid_gated_scan(*given) if both else vig_amd.gated_scan(*given, True)
+        got = torch.autograd.grad((o,) if both else (o, h), given, (do,) if both else (do, dh))
+        want = reference(x, g, h0, both, do, dh)
+        close(o, want["o"], "o")
+        for name, t in zip(("dx", "dg", "dh0"), got):
+            close(t, want[name], name)
+        if not both:
+            close(h, want["final"], "final")
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("B,L,D", [(1, 1024, 36), (2, 1000, 7), (1, 1023, 66)])
+def test_one_workgroup_up_to_1024_tokens(B, L, D, types, both):
+    test_against_the_recurrence(B, L, D, types, both)
+
+
+def test_many_chunks_of_many_channels():
+    """Gradients of long causal sequences in so many workgroups that a thread takes 16 tokens."""
+    B, L, D = 1, 1100, 16384
+    announce(f"gated scan B{B} L{L} D{D}")
+    x, g, h0, do, dh = draw(B, L, D, BF16, BF16, False, 5, state=True)
+    given = [t.requires_grad_() for t in (x, g, h0)]
+    o, h = vig_amd.gated_scan(*given, True)
+    got = torch.autograd.grad((o, h), given, (do, dh))
+    some = slice(8000, 8100)
+    want = reference(x[..., some], g[..., some], h0[:, some], False, do[..., some], dh[:, some])
+    close(o[..., some], want["o"], "o"), close(h[:, some], want["final"], "final"), close(got[2][:, some], want["dh0"], "dh0")
+    close(got[0][..., some], want["dx"], "dx"), close(got[1][..., some], want["dg"], "dg")
+
+
+@pytest.mark.parametrize("both", [False, True])
 @pytest.mark.parametrize("B,L,D", [(1, 4100, 68), (2, 9001, 5), (1, 70000, 4)])
 def test_many_chunks(B, L, D, both):
     announce(f"gated scan, long: B{B} L{L} D{D} both={both}")

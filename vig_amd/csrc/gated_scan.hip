@@ -22,7 +22,7 @@ namespace {
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 constexpr unsigned kBeyond = 0x40000000u;  // byte offset that no descriptor here covers (kScanRow)
-constexpr int kTokens = 8;                 // of a thread
+constexpr int kTokens = 8;                 // of a thread, where a comment does not say otherwise
 constexpr int kLanes = 16;                 // that take a token's channels
 constexpr int kRuns = 64 / kLanes;         // of tokens in a wave
 constexpr int kMaxWaves = 16;
@@ -85,9 +85,17 @@ struct Place {
       : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), run((threadIdx.x & 63) / kLanes), lc(threadIdx.x % kLanes) {}
 };
 
-// LDS of one direction: each wave's map of a channel
+// LDS of one direction: each wave's map of a channel; `waves` of them, as many as the workgroup has
 template <int N> struct Board {
-  alignas(8 * N) float v[kMaxWaves][kLanes][2 * N];
+  float (*v)[kLanes][2 * N];
+  static constexpr size_t kBytes = sizeof(float) * kLanes * 2 * N;  // of a wave
+};
+
+template <int N, int DIRS> struct Boards {
+  char* at;
+  int waves;
+  __device__ __forceinline__ Boards(char* at, int waves) : at(at), waves(waves) {}
+  __device__ __forceinline__ Board<N> operator[](int dir) const { return {reinterpret_cast<float (*)[kLanes][2 * N]>(at + dir * waves * Board<N>::kBytes)}; }
 };
 
 // A map's values in the lower and the upper of each two rows of lanes (HALVES: of the wave's halves), in both of them
@@ -105,7 +113,7 @@ __device__ __forceinline__ void both_of(const Map<N>& m, Map<N>& low, Map<N>& hi
 // Folds the threads' maps along a wave.  UP: tokens in their order; else against it.  Leaves in `m` the map of what lies in front of this
 // thread in its wave, and the whole wave's on the board.
 template <bool UP, int N>
-__device__ __forceinline__ void fold_wave(Map<N>& m, const Place& at, Board<N>& board) {
+__device__ __forceinline__ void fold_wave(Map<N>& m, const Place& at, const Board<N>& board) {
   Map<N> low, high, first, second;
   both_of<false>(m, low, high);
   const bool behind = UP ? at.run & 1 : !(at.run & 1), last = UP ? at.run >= 2 : at.run < 2;
@@ -183,41 +191,41 @@ struct Tile {
 };
 
 // gates as the factors they stand for; tokens behind the sequence read as gates of 0 and rows of 0, the map that changes nothing
-template <typename T, int N>
-__device__ __forceinline__ void factors(const Piece<T, N> (&raw)[kTokens], float (&a)[kTokens][N]) {
+template <typename T, int N, int TOKENS>
+__device__ __forceinline__ void factors(const Piece<T, N> (&raw)[TOKENS], float (&a)[TOKENS][N]) {
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t)
+  for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
     for (int i = 0; i < N; ++i) a[t][i] = exp_fast(raw[t].get(i));
 }
-template <typename T, int N>
-__device__ __forceinline__ void load_run(Piece<T, N> (&raw)[kTokens], rsrc_t r, unsigned first, unsigned pitch) {
+template <typename T, int N, int TOKENS>
+__device__ __forceinline__ void load_run(Piece<T, N> (&raw)[TOKENS], rsrc_t r, unsigned first, unsigned pitch) {
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t) raw[t].load(r, first + t * pitch);
+  for (int t = 0; t < TOKENS; ++t) raw[t].load(r, first + t * pitch);
 }
 
 // A thread's map along its tokens, h -> a h + x
-template <bool UP, typename T, int N>
-__device__ __forceinline__ Map<N> fold_run(const float (&a)[kTokens][N], const Piece<T, N> (&x)[kTokens]) {
+template <bool UP, typename T, int N, int TOKENS>
+__device__ __forceinline__ Map<N> fold_run(const float (&a)[TOKENS][N], const Piece<T, N> (&x)[TOKENS]) {
   Map<N> m;
   m.identity();
 #pragma unroll
-  for (int k = 0; k < kTokens; ++k) {
-    const int t = UP ? k : kTokens - 1 - k;
+  for (int k = 0; k < TOKENS; ++k) {
+    const int t = UP ? k : TOKENS - 1 - k;
 #pragma unroll
     for (int i = 0; i < N; ++i) m.s[i] = fmaf(a[t][i], m.s[i], x[t].get(i)), m.a[i] *= a[t][i];
   }
   return m;
 }
 // ... and the gradient's against them, h -> a (h + scale y), whose factor is the same
-template <bool UP, typename T, int N>
-__device__ __forceinline__ Map<N> fold_back(const float (&a)[kTokens][N], const Piece<T, N> (&y)[kTokens], float scale, const Map<N>& along) {
+template <bool UP, typename T, int N, int TOKENS>
+__device__ __forceinline__ Map<N> fold_back(const float (&a)[TOKENS][N], const Piece<T, N> (&y)[TOKENS], float scale, const Map<N>& along) {
   Map<N> m;
 #pragma unroll
   for (int i = 0; i < N; ++i) m.a[i] = along.a[i], m.s[i] = 0.f;
 #pragma unroll
-  for (int k = 0; k < kTokens; ++k) {
-    const int t = UP ? k : kTokens - 1 - k;
+  for (int k = 0; k < TOKENS; ++k) {
+    const int t = UP ? k : TOKENS - 1 - k;
 #pragma unroll
     for (int i = 0; i < N; ++i) m.s[i] = a[t][i] * fmaf(scale, y[t].get(i), m.s[i]);
   }
@@ -269,23 +277,24 @@ __device__ __forceinline__ void store_state(float* to, const float (&h)[N], cons
 
 // ---- forward.  FOLD: only the chunks' maps
 
-template <typename TX, typename TG, bool BOTH, bool FOLD, int N>
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int TOKENS>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) {
-  __shared__ Board<N> board[BOTH ? 2 : 1], front[FOLD ? 1 : BOTH ? 2 : 1];
+  constexpr int dirs = BOTH ? 2 : 1;
+  extern __shared__ __align__(16) char lds[];
   const Place at;
+  const Boards<N, dirs> board(lds, at.waves), front(lds + dirs * at.waves * Board<N>::kBytes, at.waves);
   const Tile tile(p, FOLD);
   const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
-  const int first = (at.wave * kRuns + at.run) * kTokens;
+  const int first = (at.wave * kRuns + at.run) * TOKENS;
   auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
-  Piece<TX, N> x[kTokens];
-  Piece<TG, N> raw[kTokens];
-  float a[kTokens][N], a2[BOTH ? kTokens : 1][N];
+  Piece<TX, N> x[TOKENS];
+  Piece<TG, N> raw[TOKENS];
+  float a[TOKENS][N], a2[BOTH ? TOKENS : 1][N];
   load_run(raw, tile.rows_of<TG>(p.g[0], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
   load_run(x, tile.rows_of<TX>(p.x, p.xb, p.xl), offset(p.xl, sizeof(TX)), (unsigned)(p.xl * sizeof(TX)));
-  [[maybe_unused]] Piece<TG, N> raw2[BOTH ? kTokens : 1];
+  [[maybe_unused]] Piece<TG, N> raw2[BOTH ? TOKENS : 1];
   if constexpr (BOTH) load_run(raw2, tile.rows_of<TG>(p.g[1], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
-  constexpr int dirs = BOTH ? 2 : 1;
   [[maybe_unused]] Map<N> before, after;
   if constexpr (!FOLD) {
     if (p.chunks > 1) {
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
       fold_wave<true, N>(before, at, front[0]);
       if constexpr (BOTH) {
         after = fold_chunks<false, N>(p, tile, at, 1, dirs, c, has);
-        fold_wave<false, N>(after, at, front[BOTH ? 1 : 0]);
+        fold_wave<false, N>(after, at, front[1]);
       }
     }
   }
@@ -303,22 +312,22 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
   if constexpr (BOTH) {
     factors(raw2, a2);
     m2 = fold_run<false>(a2, x);
-    fold_wave<false, N>(m2, at, board[BOTH ? 1 : 0]);
+    fold_wave<false, N>(m2, at, board[1]);
   }
   __syncthreads();
   if constexpr (FOLD) {
     if (at.wave == 0 && at.run == 0 && has) {
       store_map(p, tile, 0, dirs, c, whole<true, N>(at, board[0]));
-      if constexpr (BOTH) store_map(p, tile, 1, dirs, c, whole<false, N>(at, board[BOTH ? 1 : 0]));
+      if constexpr (BOTH) store_map(p, tile, 1, dirs, c, whole<false, N>(at, board[1]));
     }
     return;
   }
-  float h[N], y[kTokens][N];
+  float h[N], y[TOKENS][N];
   load_state(h, p.h0, p, tile.b, c, has);
   if (p.chunks > 1) whole<true, N>(at, front[0]).apply(h);
   enter<true, N>(h, m, at, board[0]);
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t)
+  for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
     for (int i = 0; i < N; ++i) y[t][i] = h[i] = fmaf(a[t][i], h[i], x[t].get(i));
   // (tokens behind the sequence change nothing: the last run ends with the state behind its last token)
@@ -327,17 +336,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
     float r[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) r[i] = 0.f;
-    if (p.chunks > 1) whole<false, N>(at, front[BOTH ? 1 : 0]).apply(r);
-    enter<false, N>(r, m2, at, board[BOTH ? 1 : 0]);
+    if (p.chunks > 1) whole<false, N>(at, front[1]).apply(r);
+    enter<false, N>(r, m2, at, board[1]);
 #pragma unroll
-    for (int t = kTokens - 1; t >= 0; --t)
+    for (int t = TOKENS - 1; t >= 0; --t)
 #pragma unroll
       for (int i = 0; i < N; ++i) r[i] = fmaf(a2[t][i], r[i], x[t].get(i)), y[t][i] += r[i];
   }
   const rsrc_t out = tile.rows_of<TX>(p.o, (long long)p.L * p.D, p.D);
   const unsigned to = offset(p.D, sizeof(TX));
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t) {
+  for (int t = 0; t < TOKENS; ++t) {
 #pragma unroll
     for (int i = 0; i < N; ++i) y[t][i] *= p.scale;
     Piece<TX, N>::store(out, to + t * (unsigned)(p.D * sizeof(TX)), y[t]);
@@ -346,25 +355,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_kernel(ScanArgs p) 
 
 // ---- backward
 
-template <typename TX, typename TG, bool BOTH, bool FOLD, int N>
+template <typename TX, typename TG, bool BOTH, bool FOLD, int N, int TOKENS>
 __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs p) {
   constexpr int dirs = BOTH ? 4 : 2;
-  __shared__ Board<N> board[dirs], front[FOLD ? 1 : dirs];
+  extern __shared__ __align__(16) char lds[];
   const Place at;
+  const Boards<N, dirs> board(lds, at.waves), front(lds + dirs * at.waves * Board<N>::kBytes, at.waves);
   const Tile tile(p, FOLD);
   const int c = (tile.cg * kLanes + at.lc) * N;
   const bool has = c < p.D;
-  const int first = (at.wave * kRuns + at.run) * kTokens;
+  const int first = (at.wave * kRuns + at.run) * TOKENS;
   auto offset = [&](long long sl, int size) { return has ? (unsigned)((first * sl + c) * size) : kBeyond; };
   const long long dense = (long long)p.L * p.D;
-  Piece<TX, N> x[kTokens], dy[kTokens];
+  Piece<TX, N> x[TOKENS], dy[TOKENS];
   load_run(x, tile.rows_of<TX>(p.x, p.xb, p.xl), offset(p.xl, sizeof(TX)), (unsigned)(p.xl * sizeof(TX)));
   load_run(dy, tile.rows_of<TX>(p.d_o, dense, p.D), offset(p.D, sizeof(TX)), (unsigned)(p.D * sizeof(TX)));
-  Piece<TG, N> raw[BOTH ? 2 : 1][kTokens];
+  Piece<TG, N> raw[BOTH ? 2 : 1][TOKENS];
 #pragma unroll
   for (int w = 0; w < (BOTH ? 2 : 1); ++w)
     load_run(raw[w], tile.rows_of<TG>(p.g[w], p.gb, p.gl), offset(p.gl, sizeof(TG)), (unsigned)(p.gl * sizeof(TG)));
-  float a[BOTH ? 2 : 1][kTokens][N];
+  float a[BOTH ? 2 : 1][TOKENS][N];
   Map<N> along[BOTH ? 2 : 1], against[BOTH ? 2 : 1];
   if constexpr (!FOLD) {
     if (p.chunks > 1) {
@@ -372,10 +382,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
 #pragma unroll
       for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
         Map<N> f = w ? fold_chunks<false, N>(p, tile, at, 2, dirs, c, has) : fold_chunks<true, N>(p, tile, at, 0, dirs, c, has);
-        if (w) fold_wave<false, N>(f, at, front[BOTH ? 2 : 0]);
+        if (w) fold_wave<false, N>(f, at, front[2]);
         else fold_wave<true, N>(f, at, front[0]);
         f = w ? fold_chunks<true, N>(p, tile, at, 3, dirs, c, has) : fold_chunks<false, N>(p, tile, at, 1, dirs, c, has);
-        if (w) fold_wave<true, N>(f, at, front[BOTH ? 3 : 0]);
+        if (w) fold_wave<true, N>(f, at, front[3]);
         else fold_wave<false, N>(f, at, front[1]);
       }
     }
@@ -391,8 +401,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
     } else {
       along[w] = fold_run<false>(a[w], x);
       against[w] = fold_back<true>(a[w], dy, p.scale, along[w]);
-      fold_wave<false>(along[w], at, board[BOTH ? 2 : 0]);
-      fold_wave<true>(against[w], at, board[BOTH ? 3 : 0]);
+      fold_wave<false>(along[w], at, board[2]);
+      fold_wave<true>(against[w], at, board[3]);
     }
   }
   __syncthreads();
@@ -401,38 +411,38 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
       store_map(p, tile, 0, dirs, c, whole<true, N>(at, board[0]));
       store_map(p, tile, 1, dirs, c, whole<false, N>(at, board[1]));
       if constexpr (BOTH) {
-        store_map(p, tile, 2, dirs, c, whole<false, N>(at, board[BOTH ? 2 : 0]));
-        store_map(p, tile, 3, dirs, c, whole<true, N>(at, board[BOTH ? 3 : 0]));
+        store_map(p, tile, 2, dirs, c, whole<false, N>(at, board[2]));
+        store_map(p, tile, 3, dirs, c, whole<true, N>(at, board[3]));
       }
     }
     return;
   }
-  float dx[kTokens][N];
+  float dx[TOKENS][N];
 #pragma unroll
   for (int w = 0; w < (BOTH ? 2 : 1); ++w) {
-    float h[N], d[N], u[kTokens][N];
+    float h[N], d[N], u[TOKENS][N];
     load_state(h, w ? nullptr : p.h0, p, tile.b, c, has);
     load_state(d, w ? nullptr : p.dhT, p, tile.b, c, has);
     if (w == 0) {
-      if (p.chunks > 1) whole<true, N>(at, front[0]).apply(h), whole<false, N>(at, front[FOLD ? 0 : 1]).apply(d);
+      if (p.chunks > 1) whole<true, N>(at, front[0]).apply(h), whole<false, N>(at, front[1]).apply(d);
       enter<true, N>(h, along[w], at, board[0]);
       enter<false, N>(d, against[w], at, board[1]);
     } else {
-      if (p.chunks > 1) whole<false, N>(at, front[FOLD || !BOTH ? 0 : 2]).apply(h), whole<true, N>(at, front[FOLD || !BOTH ? 0 : 3]).apply(d);
-      enter<false, N>(h, along[w], at, board[BOTH ? 2 : 0]);
-      enter<true, N>(d, against[w], at, board[BOTH ? 3 : 0]);
+      if (p.chunks > 1) whole<false, N>(at, front[2]).apply(h), whole<true, N>(at, front[3]).apply(d);
+      enter<false, N>(h, along[w], at, board[2]);
+      enter<true, N>(d, against[w], at, board[3]);
     }
 #pragma unroll
-    for (int k = 0; k < kTokens; ++k) {
-      const int t = w == 0 ? k : kTokens - 1 - k;
+    for (int k = 0; k < TOKENS; ++k) {
+      const int t = w == 0 ? k : TOKENS - 1 - k;
 #pragma unroll
       for (int i = 0; i < N; ++i) u[t][i] = a[w][t][i] * h[i], h[i] = u[t][i] + x[t].get(i);
     }
     const rsrc_t out = tile.rows_of<TG>(p.dg[w], dense, p.D);
     const unsigned to = offset(p.D, sizeof(TG));
 #pragma unroll
-    for (int k = 0; k < kTokens; ++k) {
-      const int t = w == 0 ? kTokens - 1 - k : k;
+    for (int k = 0; k < TOKENS; ++k) {
+      const int t = w == 0 ? TOKENS - 1 - k : k;
       float dg[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -448,7 +458,212 @@ __global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_bwd_kernel(ScanArgs
   const rsrc_t out = tile.rows_of<TX>(p.dx, dense, p.D);
   const unsigned to = offset(p.D, sizeof(TX));
 #pragma unroll
-  for (int t = 0; t < kTokens; ++t) Piece<TX, N>::store(out, to + t * (unsigned)(p.D * sizeof(TX)), dx[t]);
+  for (int t = 0; t < TOKENS; ++t) Piece<TX, N>::store(out, to + t * (unsigned)(p.D * sizeof(TX)), dx[t]);
+}
+
+// ---- bf16 sequences of at most 256 tokens whose rows keep 16-byte boundaries: everything moves 16 bytes a lane and by whole lines
+//
+// Loads of four bytes a lane keep the address units busy four times as long as ones of sixteen, and lines whose halves two workgroups write go to memory by halves: a
+// copy of three tensors into one in the pattern of the kernels above takes 20.5 us at 128 x 196 x 384, one of 16 bytes a lane and 128-byte rows 14.3.  Here a wave has
+// 16 tokens of 64 channels; its rows go straight to its own part of LDS, from where each lane takes its channels, and back the same way, past the caches; the waves' maps
+// lie where the gates were.  128 x 196 x 384: causal 15.9 -> 13.5 us, its gradients 26.8 -> 25.9, those of both directions 41.6 -> 35.6, of 1024 x 20 x 384 26.6 -> 23.7.  (The
+// forward of both directions needs more registers than two workgroups a compute unit leave: 21.7 -> 23.3; a persistent form with the next rows on their way 20.7.)
+
+typedef Piece<uint16_t, 2> Pair;
+constexpr int kHalf = 32;                        // lanes that take a token's channels: two runs of eight tokens a wave
+constexpr int kStep = 2 * kTokens;               // tokens of a wave
+constexpr int kRow = 4 * kHalf;                  // bytes of a token's row
+constexpr int kRows = kStep * kRow;              // of a wave's rows of one tensor, two loads of a kilobyte
+constexpr int kHalfBoard = kHalf * 4 * (int)sizeof(float);  // of a wave's maps in one direction
+constexpr int kRowsTokens = kMaxWaves * kStep;
+static_assert(kRows == 2048 && 2 * kHalfBoard <= kRows, "two boards take a tensor's place");
+
+struct HalfPlace {
+  int wave, waves, lane, run, lc;
+  __device__ __forceinline__ HalfPlace()
+      : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), lane(threadIdx.x & 63), run((threadIdx.x & 63) / kHalf), lc(threadIdx.x % kHalf) {}
+};
+
+// Token t of the second run lies beside token t of the first, so that a read of both meets every bank once.
+__device__ __forceinline__ int token_of_row(int row) { return (row >> 1) + kTokens * (row & 1); }
+// a wave's rows into LDS; tokens and pieces of a row that the tensor does not have are read from its last ones
+__device__ __forceinline__ void fetch_rows(const uint16_t* base, long long pitch, int first, int rows, int width, int lane, uint32_t lds) {
+  const int piece = min(lane % 8, width / 8 - 1);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int t = min(first + token_of_row(k * 8 + lane / 8), rows - 1);
+    load_to_lds16(base, (unsigned)t * (unsigned)(2 * pitch) + piece * 16u, lds + k * 1024);
+  }
+}
+__device__ __forceinline__ void take_rows(const char* lds, const HalfPlace& at, Pair (&x)[kTokens]) {
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) x[t].v = *reinterpret_cast<const uint32_t*>(lds + (2 * t + at.run) * kRow + 4 * at.lc);
+}
+// tokens behind the sequence: nothing
+__device__ __forceinline__ void cut_rows(int left, Pair (&x)[kTokens]) {
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) x[t].v = t < left ? x[t].v : 0u;
+}
+// the thread's values of its token t into the wave's rows ...
+__device__ __forceinline__ void put_row(char* lds, const HalfPlace& at, int t, const float (&y)[2]) {
+  *reinterpret_cast<uint32_t*>(lds + (2 * t + at.run) * kRow + 4 * at.lc) = pack_bf16x2(y[0], y[1]);
+}
+// ... and the rows to memory
+__device__ __forceinline__ void send_rows(const char* lds, void* base, const ScanArgs& p, int b, int first, int c0, int width, int lane) {
+  const rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(static_cast<uint16_t*>(base) + (long long)b * p.L * p.D, 0, p.L * p.D * 2, 0x00020000);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int t = first + token_of_row(k * 8 + lane / 8);
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(lds + k * 1024 + lane * 16);
+    const unsigned to = lane % 8 * 8 < width ? (unsigned)(t * p.D + c0) * 2u + lane % 8 * 16u : kBeyond;
+    __builtin_amdgcn_raw_buffer_store_b128(v, out, to, 0, 2);  // (non-temporal)
+  }
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// As fold_wave: what lies in front of this thread in its wave stays in `m`, the wave's map goes to its board.
+template <bool UP>
+__device__ __forceinline__ void fold_halves(Map<2>& m, const HalfPlace& at, char* board) {
+  Map<2> low, high;
+  both_of<true>(m, low, high);
+  const bool behind = UP ? at.run == 1 : at.run == 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) m.a[i] = behind ? (UP ? low : high).a[i] : 1.f, m.s[i] = behind ? (UP ? low : high).s[i] : 0.f;
+  if (UP) high.behind(low);
+  else low.behind(high);
+  const Map<2>& t = UP ? high : low;
+  if (at.run == 0) reinterpret_cast<f32x4_t*>(board)[at.lc] = f32x4_t{t.a[0], t.s[0], t.a[1], t.s[1]};
+}
+// (behind the barrier) the state that enters this thread's tokens, four waves' maps at a time; boards lie `pitch` bytes apart
+template <bool UP>
+__device__ __forceinline__ void enter_halves(float (&h)[2], const Map<2>& m, const HalfPlace& at, const char* boards, int pitch) {
+  const int n = UP ? at.wave : at.waves - 1 - at.wave;
+  for (int k = 0; k < n; k += 4) {
+    f32x4_t v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = reinterpret_cast<const f32x4_t*>(boards + (UP ? min(k + q, at.waves - 1) : max(at.waves - 1 - k - q, 0)) * pitch)[at.lc];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (k + q < n) h[0] = fmaf(v[q][0], h[0], v[q][1]), h[1] = fmaf(v[q][2], h[1], v[q][3]);
+  }
+  m.apply(h);
+}
+
+__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((amdgpu_waves_per_eu(7))) void gated_scan_rows_kernel(ScanArgs p) {
+  constexpr int kWave = 2 * kRows;  // of LDS: x, gates
+  extern __shared__ __align__(16) char lds[];
+  const HalfPlace at;
+  char *const xs = lds + at.wave * kWave, *const gs = xs + kRows;
+  const int first = at.wave * kStep, mine = first + at.run * kTokens;
+  const Tile tile(p, true);
+  const int b = tile.b, c0 = tile.cg * 2 * kHalf, width = min(2 * kHalf, p.D - c0), c = c0 + 2 * at.lc;
+  const bool has = c < p.D;
+  const uint32_t to = __builtin_amdgcn_readfirstlane(lds_offset(xs));
+  fetch_rows(static_cast<const uint16_t*>(p.g[0]) + b * p.gb + c0, p.gl, first, p.L, width, at.lane, to + kRows);
+  fetch_rows(static_cast<const uint16_t*>(p.x) + b * p.xb + c0, p.xl, first, p.L, width, at.lane, to);
+  float h[2], a[kTokens][2];
+  load_state(h, p.h0, p, b, c, has);
+  Pair x[kTokens], raw[kTokens];
+  wait_vmem<0>();
+  take_rows(gs, at, raw), take_rows(xs, at, x);
+  if (first + kStep > p.L) cut_rows(p.L - mine, raw), cut_rows(p.L - mine, x);  // (the last wave)
+  factors(raw, a);
+  wait_lds();  // (before a map takes the gates' place)
+  Map<2> m = fold_run<true>(a, x);
+  fold_halves<true>(m, at, gs);
+  __syncthreads();
+  enter_halves<true>(h, m, at, lds + kRows, kWave);
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) {
+    float y[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) h[i] = fmaf(a[t][i], h[i], x[t].get(i)), y[i] = p.scale * h[i];
+    put_row(xs, at, t, y);
+  }
+  if (p.hT && at.wave == at.waves - 1 && at.run == 1 && has) store_state(p.hT, h, p, b, c);
+  wait_lds();
+  send_rows(xs, p.o, p, b, first, c0, width, at.lane);
+}
+
+template <bool BOTH>
+__global__ __launch_bounds__(64 * kMaxWaves) void gated_scan_rows_bwd_kernel(ScanArgs p) {
+  constexpr int ways = BOTH ? 2 : 1, kWave = (2 + ways) * kRows;  // of LDS: x, the output's gradient, gates
+  extern __shared__ __align__(16) char lds[];
+  const HalfPlace at;
+  char *const xs = lds + at.wave * kWave, *const ds = xs + kRows, *const gs = ds + kRows;
+  const int first = at.wave * kStep, mine = first + at.run * kTokens;
+  const Tile tile(p, true);
+  const int b = tile.b, c0 = tile.cg * 2 * kHalf, width = min(2 * kHalf, p.D - c0), c = c0 + 2 * at.lc;
+  const bool has = c < p.D;
+  const uint32_t to = __builtin_amdgcn_readfirstlane(lds_offset(xs));
+#pragma unroll
+  for (int w = 0; w < ways; ++w) fetch_rows(static_cast<const uint16_t*>(p.g[w]) + b * p.gb + c0, p.gl, first, p.L, width, at.lane, to + (2 + w) * kRows);
+  fetch_rows(static_cast<const uint16_t*>(p.x) + b * p.xb + c0, p.xl, first, p.L, width, at.lane, to);
+  fetch_rows(static_cast<const uint16_t*>(p.d_o) + (long long)b * p.L * p.D + c0, p.D, first, p.L, width, at.lane, to + kRows);
+  Pair x[kTokens], dy[kTokens];
+  float a[ways][kTokens][2];
+  wait_vmem<0>();
+  {
+    Pair raw[ways][kTokens];
+#pragma unroll
+    for (int w = 0; w < ways; ++w) take_rows(gs + w * kRows, at, raw[w]);
+    take_rows(xs, at, x), take_rows(ds, at, dy);
+    if (first + kStep > p.L) {  // (the last wave)
+#pragma unroll
+      for (int w = 0; w < ways; ++w) cut_rows(p.L - mine, raw[w]);
+      cut_rows(p.L - mine, x), cut_rows(p.L - mine, dy);
+    }
+#pragma unroll
+    for (int w = 0; w < ways; ++w) factors(raw[w], a[w]);
+  }
+  wait_lds();  // (before maps take the gates' place)
+  Map<2> along[ways], against[ways];
+#pragma unroll
+  for (int w = 0; w < ways; ++w) {
+    char* const board = gs + w * kRows;
+    along[w] = w ? fold_run<false>(a[w], x) : fold_run<true>(a[w], x);
+    against[w] = w ? fold_back<true>(a[w], dy, p.scale, along[w]) : fold_back<false>(a[w], dy, p.scale, along[w]);
+    if (w) fold_halves<false>(along[w], at, board), fold_halves<true>(against[w], at, board + kHalfBoard);
+    else fold_halves<true>(along[w], at, board), fold_halves<false>(against[w], at, board + kHalfBoard);
+  }
+  __syncthreads();
+  float dx[kTokens][2];
+#pragma unroll
+  for (int w = 0; w < ways; ++w) {
+    const char* const board = lds + (2 + w) * kRows;
+    float h[2], d[2], u[kTokens][2];
+    load_state(h, w ? nullptr : p.h0, p, b, c, has);
+    load_state(d, w ? nullptr : p.dhT, p, b, c, has);
+    if (w) enter_halves<false>(h, along[w], at, board, kWave), enter_halves<true>(d, against[w], at, board + kHalfBoard, kWave);
+    else enter_halves<true>(h, along[w], at, board, kWave), enter_halves<false>(d, against[w], at, board + kHalfBoard, kWave);
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int t = w == 0 ? k : kTokens - 1 - k;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) u[t][i] = a[w][t][i] * h[i], h[i] = u[t][i] + x[t].get(i);
+    }
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int t = w == 0 ? kTokens - 1 - k : k;
+      float dg[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float dh = fmaf(p.scale, dy[t].get(i), d[i]);
+        dx[t][i] = w == 0 ? dh : dx[t][i] + dh;
+        dg[i] = dh * u[t][i];
+        d[i] = a[w][t][i] * dh;
+      }
+      put_row(xs, at, t, dg);
+    }
+    if (w == 0 && p.dh0 && at.wave == 0 && at.run == 0 && has) store_state(p.dh0, d, p, b, c);
+    wait_lds();
+    send_rows(xs, p.dg[w], p, b, first, c0, width, at.lane);
+    wait_lds();  // (before the next rows take these rows' place)
+  }
+#pragma unroll
+  for (int t = 0; t < kTokens; ++t) put_row(xs, at, t, dx[t]);
+  wait_lds();
+  send_rows(xs, p.dx, p, b, first, c0, width, at.lane);
 }
 
 // ---- one token
@@ -489,7 +704,8 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const TX* x, const
 // ---- host side
 
 struct Cut {
-  int waves, chunks, chunk, groups;
+  bool pairs;
+  int tokens, waves, chunks, chunk, groups;
 };
 // Whether N channels move at once: whole ones of them in every row, on boundaries of their size (a null pointer stands on any)
 inline bool whole(int n, int D, long long a, long long b, long long c, long long d) { return D % n == 0 && (a | b | c | d) % n == 0; }
@@ -499,9 +715,9 @@ bool on(int n, int dtype, P... p) {
   return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...);
 }
 
-inline Cut cut(int B, int L, int D, bool pairs) {
-  Cut k;
-  const int tile = kLanes * (pairs ? 2 : 1), run = kRuns * kTokens;  // channels of a workgroup, tokens of a wave
+inline Cut cut(int L, int D, bool pairs, int tokens) {
+  Cut k{pairs, tokens};
+  const int tile = kLanes * (pairs ? 2 : 1), run = kRuns * tokens;  // channels of a workgroup, tokens of a wave
   k.groups = (D + tile - 1) / tile;
   const int waves = (L + run - 1) / run;
   k.chunks = (waves + kMaxWaves - 1) / kMaxWaves;
@@ -511,40 +727,78 @@ inline Cut cut(int B, int L, int D, bool pairs) {
   return k;
 }
 
-template <typename TX, typename TG, bool BOTH, int N>
+// Sequences of 513 to 1024 tokens are one workgroup's with 16 tokens a thread, where 8 make two chunks of them and read everything twice; for both directions with
+// one channel a lane, which leaves the registers for it.  us, 64 x 1024 x 384: causal 51.8 -> 35.4, its gradients 104 -> 60, both 94 -> 68, gradients 154 -> 109.  Many
+// chunks of a causal gradient gain too (65536 x 1024: 278 -> 252; 4 x 2305 x 384, fewer workgroups than fill the chip: 19.0 -> 21.8).
+inline Cut cut_for(int B, int L, int D, bool pairs, bool both, bool bwd) {
+  const Cut few = cut(L, D, pairs, kTokens);
+  if (few.chunks == 1) return few;
+  if (L <= 16 * kRuns * kMaxWaves) return cut(L, D, pairs && !both, 16);
+  const Cut wide = cut(L, D, pairs, 16);
+  return bwd && !both && (long long)B * wide.groups * wide.chunks >= 1024 ? wide : few;
+}
+
+template <typename TX, typename TG, bool BOTH, int N, int TOKENS>
 void start(const ScanArgs& p, bool bwd, bool fold, dim3 grid, dim3 block, hipStream_t stream) {
+  const size_t lds = block.x / 64 * Board<N>::kBytes * (BOTH ? 2 : 1) * (bwd ? 2 : 1) * (!fold && p.chunks > 1 ? 2 : 1);  // (at most 64 KB)
   if (bwd) {
-    if (fold) hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, true, N>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, false, N>), grid, block, 0, stream, p);
+    if (fold) hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, true, N, TOKENS>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((gated_scan_bwd_kernel<TX, TG, BOTH, false, N, TOKENS>), grid, block, lds, stream, p);
   } else {
-    if (fold) hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, true, N>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, false, N>), grid, block, 0, stream, p);
+    if (fold) hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, true, N, TOKENS>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((gated_scan_kernel<TX, TG, BOTH, false, N, TOKENS>), grid, block, lds, stream, p);
   }
 }
 template <typename TX, typename TG>
-void start(const ScanArgs& p, bool bwd, bool fold, bool pairs, dim3 grid, dim3 block, hipStream_t stream) {
+void start(const ScanArgs& p, bool bwd, bool fold, const Cut& k, dim3 grid, dim3 block, hipStream_t stream) {
   if (p.g[1]) {
-    if (pairs) start<TX, TG, true, 2>(p, bwd, fold, grid, block, stream);
-    else start<TX, TG, true, 1>(p, bwd, fold, grid, block, stream);
+    if (k.tokens == 16) start<TX, TG, true, 1, 16>(p, bwd, fold, grid, block, stream);
+    else if (k.pairs) start<TX, TG, true, 2, 8>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, true, 1, 8>(p, bwd, fold, grid, block, stream);
+  } else if (k.tokens == 8) {
+    if (k.pairs) start<TX, TG, false, 2, 8>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, false, 1, 8>(p, bwd, fold, grid, block, stream);
   } else {
-    if (pairs) start<TX, TG, false, 2>(p, bwd, fold, grid, block, stream);
-    else start<TX, TG, false, 1>(p, bwd, fold, grid, block, stream);
+    if (k.pairs) start<TX, TG, false, 2, 16>(p, bwd, fold, grid, block, stream);
+    else start<TX, TG, false, 1, 16>(p, bwd, fold, grid, block, stream);
   }
 }
+// Whether and how bf16 sequences go by whole rows: 0, or launched
+inline int start_rows(ScanArgs p, bool bwd, int B, hipStream_t stream) {
+  const bool lies = p.L <= kRowsTokens && whole(8, p.D, p.xb, p.xl, p.gb, p.gl) && on(8, VIG_BF16, p.x, p.g[0], p.g[1], p.d_o, p.o, p.dx, p.dg[0], p.dg[1]);
+  if (!lies || (!bwd && p.g[1])) return 0;
+  p.groups = (p.D + 2 * kHalf - 1) / (2 * kHalf), p.chunks = 1, p.chunk = p.L;
+  const long long groups = (long long)B * p.groups;
+  // Few workgroups finish sooner as the smaller ones of the other kernels (4 x 196 x 192, gradients of both directions 5.6 us for 7.6), and lanes behind
+  // the last channel work for nothing (500 x 100 x 200: 38 for 52).
+  if (groups < 256 || groups > 0x7fffffffLL || p.groups * 2 * kHalf * 8 > p.D * 9) return 0;
+  const int waves = (p.L + kStep - 1) / kStep;
+  const size_t lds = (size_t)waves * kRows * (bwd ? p.g[1] ? 4 : 3 : 2);
+  static bool allowed[3][64];
+  const void* const kernel = !bwd ? (const void*)gated_scan_rows_kernel : p.g[1] ? (const void*)gated_scan_rows_bwd_kernel<true> : (const void*)gated_scan_rows_bwd_kernel<false>;
+  if (!allow_lds(kernel, kMaxWaves * kRows * (bwd ? p.g[1] ? 4 : 3 : 2), allowed[!bwd ? 0 : p.g[1] ? 2 : 1])) return 0;
+  const dim3 grid((unsigned)groups), block(64 * waves);
+  if (!bwd) hipLaunchKernelGGL(gated_scan_rows_kernel, grid, block, lds, stream, p);
+  else if (p.g[1]) hipLaunchKernelGGL(gated_scan_rows_bwd_kernel<true>, grid, block, lds, stream, p);
+  else hipLaunchKernelGGL(gated_scan_rows_bwd_kernel<false>, grid, block, lds, stream, p);
+  return 1;
+}
+
 int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t stream) {
+  if (io_dtype == VIG_BF16 && gate_dtype == VIG_BF16 && start_rows(p, bwd, B, stream)) return hipGetLastError() == hipSuccess ? VIG_OK : VIG_ELAUNCH;
   const bool pairs = whole(2, p.D, p.xb, p.xl, p.gb, p.gl) && on(2, io_dtype, p.x, p.d_o, p.o, p.dx) && on(2, gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
-  const Cut k = cut(B, p.L, p.D, pairs);
+  const Cut k = cut_for(B, p.L, p.D, pairs, p.g[1] != nullptr, bwd);
   p.groups = k.groups, p.chunks = k.chunks, p.chunk = k.chunk;
   const long long groups = (long long)B * k.groups * k.chunks;
   if (groups > 0x7fffffffLL) return VIG_ENOTSUP;
   const dim3 grid((unsigned)groups), block(64 * k.waves);
   for (int fold = k.chunks > 1; fold >= 0; --fold) {
     if (io_dtype == VIG_BF16) {
-      if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, pairs, grid, block, stream);
-      else start<uint16_t, float>(p, bwd, fold, pairs, grid, block, stream);
+      if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, k, grid, block, stream);
+      else start<uint16_t, float>(p, bwd, fold, k, grid, block, stream);
     } else {
-      if (gate_dtype == VIG_BF16) start<float, uint16_t>(p, bwd, fold, pairs, grid, block, stream);
-      else start<float, float>(p, bwd, fold, pairs, grid, block, stream);
+      if (gate_dtype == VIG_BF16) start<float, uint16_t>(p, bwd, fold, k, grid, block, stream);
+      else start<float, float>(p, bwd, fold, k, grid, block, stream);
     }
     if (hipGetLastError() != hipSuccess) return VIG_ELAUNCH;
   }
@@ -553,9 +807,9 @@ int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t 
 
 }  // namespace
 
-// Bytes for the chunks' maps, whichever way the rows lie (rows that move one channel at a time have the more chunks).
+// Bytes for the chunks' maps, whichever way the rows lie.
 size_t gated_scan_workspace(int B, int L, int D, bool both, bool bwd) {
-  const int chunks = std::max(cut(B, L, D, false).chunks, cut(B, L, D, true).chunks);
+  const int chunks = std::max(cut_for(B, L, D, false, both, bwd).chunks, cut_for(B, L, D, true, both, bwd).chunks);
   return chunks > 1 ? (size_t)B * (both ? 2 : 1) * (bwd ? 2 : 1) * chunks * D * 2 * sizeof(float) : 0;
 }
 
