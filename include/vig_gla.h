@@ -851,15 +851,16 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
  * state_bits 32: exp_avg = m and exp_avg_sq = v in fp32 (avg_scale, sq_scale are not read).
  * state_bits 8: m and r = sqrt(v) as e4m3 values times a scale for each 256 elements of a tensor (avg_scale[j], sq_scale[j]:
  * ceil(n[j] / 256) floats, the block's largest magnitude / 448).  A block that takes in a value that is not finite is NaN from then on.
- * States in 8 bits and bf16 parameters are rounded stochastically.  The element's word: w = mix(number ^ key), number = 256 * (blocks of 256 of
- * the tensors in front) + element (its bits past 32 times 0x9E3779B9 are added to the key), key = mix(mix(mix(seed) + (seed >> 32)) + t) in
+ * States in 8 bits and bf16 parameters are rounded stochastically.  The element's word: w = mix(number ^ key), number = first[j] +
+ * element (NULL: 256 * (blocks of 256 of the tensors in front) + element; its bits past 32 times 0x9E3779B9 are added to the key): a list that is part
+ * of a larger one, on one of several ranks say, is rounded as the whole would be where first[] goes on from the others, key = mix(mix(mix(seed) + (seed >> 32)) + t) in
  * 32-bit words, mix(x): x ^= x >> 16, x *= 0x6A09E667, x ^= x >> 15, x *= 0xBB67AE85, x ^= x >> 16.  m is rounded up in magnitude where the lower half of w
  * reaches past what the step lacks, r by the upper half (never from above 0 to 0), a bf16 parameter by the upper half of 0x9E3779B9 w.
- * Tensors that are written may not overlap one another or a gradient (VIG_EINVAL).  Up to 2^40 elements in all.
+ * Tensors that are written may not overlap one another or a gradient (VIG_EINVAL).  Up to 2^40 elements in all, numbers up to 2^40 too.
  */
 int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq, float* const* avg_scale,
-                   float* const* sq_scale, const long long* n, const int* param_dtype, const int* grad_dtype, int count, int state_bits,
-                   double lr, double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,
+                   float* const* sq_scale, const long long* n, const long long* first, const int* param_dtype, const int* grad_dtype, int count,
+                   int state_bits, double lr, double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,
                    const long long* step_on_device, const float* grad_scale, unsigned long long seed, void* stream);
 /*
  * norm[0] = sqrt of the sum of squares of all elements of `count` tensors (added up in fp64, in a fixed order), and, where `scale` is not NULL,

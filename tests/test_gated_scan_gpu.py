@@ -401,6 +401,28 @@ def test_on_another_stream_and_in_graphs():
             assert all(torch.equal(a, b) for a, b in zip(out, eager)), turn
 
 
+@pytest.mark.parametrize("both", [False, True])
+def test_more_sequences_than_a_launch_takes(both):
+    """Seventy million sequences of two tokens: a launch takes 2^32 threads."""
+    B = 70_000_000
+    announce(f"gated scan of {B} sequences both={both}")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen, dtype=F32).to(BF16)  # noqa: E731
+    x, g, do = r(B, 2, 1), -r(2 * B if both else B, 2, 1).abs(), r(B, 2, 1)
+    h0, dh = (None, None) if both else (torch.randn(B, 1, device="cuda", generator=gen), torch.randn(B, 1, device="cuda", generator=gen))
+    given = [t.requires_grad_() for t in ((x, g) if both else (x, g, h0))]
+    o, h = vig_amd.bid_gated_scan(*given) if both else vig_amd.gated_scan(*given, True)
+    got = torch.autograd.grad((o,) if both else (o, h), given, (do,) if both else (do, dh))
+    with torch.no_grad():
+        for some in (slice(0, 1000), slice(67_108_000, 67_110_000), slice(B - 1000, B)):
+            gates = torch.cat([g[:B][some], g[B:][some]]) if both else g[some]
+            want = reference(x[some], gates, None if both else h0[some], both, do[some], None if both else dh[some])
+            close(o[some], want["o"], "o"), close(got[0][some], want["dx"], "dx")
+            close(torch.cat([got[1][:B][some], got[1][B:][some]]) if both else got[1][some], want["dg"], "dg")
+            if not both:
+                close(h[some], want["final"], "final"), close(got[2][some], want["dh0"], "dh0")
+
+
 def test_offsets_past_32_bits():
     """70000 tokens of 32768 channels: the last rows lie past 2^32 bytes, the last elements past 2^31."""
     L, D = 70000, 32768

@@ -31,11 +31,10 @@ def key_of(seed, t):
     return mix((mix((mix(seed & M32) + (seed >> 32)) & M32) + t) & M32)
 
 
-def words(first_block, n, key):
+def words(first, n, key):
     """The random words of n elements, in Python's integers where a product passes 63 bits."""
-    x = torch.arange(n, dtype=torch.int64) + 256 * first_block
-    assert int(x[-1]) < 1 << 32
-    x = x ^ key
+    x = torch.arange(n, dtype=torch.int64) + first
+    x = (x & M32) ^ ((key + (x >> 32) * 0x9E3779B9) & M32)
     for shift, factor in ((16, 0x6A09E667), (15, 0xBB67AE85)):
         x = x ^ (x >> shift)
         x = (x * (factor & 0xFFFF) + (((x & 0xFFFF) * (factor >> 16) & 0xFFFF) << 16)) & M32
@@ -105,14 +104,14 @@ class Case:
         kw = {"step": t, "lr": LR, "betas": (B1, B2), "eps": EPS, "weight_decay": DECAY} | more
         vig_amd.adamw_step(self.p, self.g, self.m, self.v, self.ms, self.vs, **kw)
 
-    def check(self, before, t, seed=0, clip=1.0, lr=LR):
+    def check(self, before, t, seed=0, clip=1.0, lr=LR, numbers=None):
         after, first = self.held(), 0
         for j, n in enumerate(self.sizes):
             if n == 0:
                 continue
             p, g = before["p"][j], before["g"][j] * clip
-            w = words(first, n, key_of(seed, t))
-            first += -(-n // 256)
+            w = words(first if numbers is None else numbers[j], n, key_of(seed, t))
+            first += -(-n // 256) * 256
             if self.bits8:
                 spread = lambda s: s.repeat_interleave(256)[:n]  # noqa: E731
                 m, root = before["m"][j] * spread(before["ms"][j]), before["v"][j] * spread(before["vs"][j])
@@ -174,6 +173,28 @@ def test_more_tensors_than_a_launch_takes(bits8):
         before = c.held()
         c.step(t, grad_scale=torch.tensor(0.25, device="cuda"))
         c.check(before, t, clip=0.25)
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+def test_numbers_of_elements(bits8, monkeypatch):
+    """A list rounded as part of a larger one: numbers in any order, past 32 bits, and across that border within a lane's elements."""
+    sizes = [1000, 5000, 300, 9000]
+    numbers = [5, (1 << 32) - 4001, 1 << 39, 77]
+    for way in range(2):
+        if way:
+            monkeypatch.setattr(_ext, "calls", lambda: None)
+        c = Case(sizes, (BF16, F32), (F32,), bits8, 6)
+        for t in (1, 2):
+            before = c.held()
+            c.step(t, seed=3, first=numbers)
+            c.check(before, t, seed=3, numbers=numbers)
+    monkeypatch.undo()
+    whole, parts = Case([700, 300, 5000], (BF16,), (F32,), bits8, 2), Case([700, 300, 5000], (BF16,), (F32,), bits8, 2)
+    whole.step(1)
+    for some, first in ((slice(0, 1), [0]), (slice(1, 3), [768, 1280])):  # (behind blocks of 256)
+        lists = [t[some] if t is not None else None for t in (parts.p, parts.g, parts.m, parts.v, parts.ms, parts.vs)]
+        vig_amd.adamw_step(*lists, step=1, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=DECAY, first=first)
+    assert all(torch.equal(a, b) for a, b in zip(whole.p, parts.p)) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(whole.m + whole.v, parts.m + parts.v))
 
 
 def test_empty_tensors_and_lists():

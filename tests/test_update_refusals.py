@@ -31,7 +31,7 @@ def test_scan(lib):
                 dict(gb=5 * P, h0=4 * P), dict(gb=5 * P, hT=4 * P), dict(h0=4 * P + 2), dict(h0=4 * P, hT=4 * P), dict(xs=_strides(72, 7)), dict(gs=_strides(72, 0)), dict(xs=_strides(-1, 8)),
                 dict(L=5000, ws=P + 8, n=1 << 30)):
         assert fwd(**bad) == INVALID, bad
-    for unbuilt in (dict(io=2), dict(gd=-1), dict(D=(1 << 19) + 1), dict(L=(1 << 30) + 1), dict(xs=_strides(0, (1 << 19) + 1)), dict(B=1 << 30, D=1 << 10)):
+    for unbuilt in (dict(io=2), dict(gd=-1), dict(D=(1 << 19) + 1), dict(L=(1 << 30) + 1), dict(xs=_strides(0, (1 << 19) + 1)), dict(B=1, L=1 << 30, D=1 << 19, ws=4 * P, n=1 << 62)):
         assert fwd(**unbuilt) == UNBUILT, unbuilt
     need = lib.vig_gated_scan_fwd_workspace(2, 5000, 8, 0)
     assert need > 0 and lib.vig_gated_scan_fwd_workspace(2, 5000, 8, 1) == 2 * need and lib.vig_gated_scan_bwd_workspace(2, 5000, 8, 1) == 4 * need
@@ -55,18 +55,19 @@ def test_scan(lib):
         assert step(**unbuilt) == UNBUILT, unbuilt
 
 
-def _update(lib, p, g, m, v, n, ms=None, vs=None, types=None, bits=32, step=1, b1=0.9, b2=0.999, eps=1e-8, scale=None, step_at=None, lr_at=None):
+def _update(lib, p, g, m, v, n, ms=None, vs=None, types=None, bits=32, step=1, b1=0.9, b2=0.999, eps=1e-8, scale=None, step_at=None, lr_at=None, first=None):
     ptr = lambda a: (ctypes.c_void_p * len(a))(*a)  # noqa: E731
     dt = (ctypes.c_int * len(p))(*(types or [0] * len(p)))
-    return lib.vig_adamw_many(ptr(p), ptr(g), ptr(m), ptr(v), ptr(ms) if ms else None, ptr(vs) if vs else None, (ctypes.c_longlong * len(p))(*n), dt, dt, len(p), bits, 1e-3, b1, b2, eps,
+    return lib.vig_adamw_many(ptr(p), ptr(g), ptr(m), ptr(v), ptr(ms) if ms else None, ptr(vs) if vs else None, (ctypes.c_longlong * len(p))(*n), (ctypes.c_longlong * len(p))(*first) if first else None, dt, dt, len(p), bits, 1e-3, b1, b2, eps,
                               0.0, step, lr_at, step_at, scale, 0, None)
 
 
 def test_adamw(lib):
     good = ([P, 2 * P], [3 * P, 4 * P], [5 * P, 6 * P], [7 * P, 8 * P], [100, 300])
-    for bad in (dict(step=0), dict(b1=1.0), dict(b1=-0.1), dict(b1=float("nan")), dict(b2=1.0), dict(b2=float("nan")), dict(eps=-1.0), dict(eps=float("nan")), dict(bits=8), dict(scale=P + 2), dict(step_at=P + 4),
+    for bad in (dict(step=0), dict(b1=1.0), dict(b1=-0.1), dict(b1=float("nan")), dict(b2=1.0), dict(b2=float("nan")), dict(eps=-1.0), dict(eps=float("nan")), dict(bits=8), dict(scale=P + 2), dict(step_at=P + 4), dict(first=[0, -1]),
                 dict(lr_at=P + 1)):
         assert _update(lib, *good, **bad) == INVALID, bad
+    assert _update(lib, *good, first=[0, (1 << 40) + 1]) == UNBUILT
     assert _update(lib, *good, bits=16) == _update(lib, *good, types=[0, 2]) == UNBUILT
     change = lambda k, v: [list(x) if i != k else v for i, x in enumerate(good)]  # noqa: E731
     assert _update(lib, *change(4, [100, -1])) == INVALID
@@ -77,7 +78,7 @@ def test_adamw(lib):
     scales = dict(ms=[9 * P, 10 * P], vs=[11 * P, 12 * P], bits=8)
     for more in (dict(ms=[9 * P, None]), dict(vs=[11 * P + 1, 12 * P]), dict(ms=[9 * P, 11 * P]), dict(vs=[5 * P + 96, 12 * P])):
         assert _update(lib, *good, **(scales | more)) == INVALID, more
-    assert lib.vig_adamw_many(None, None, None, None, None, None, None, None, None, 1, 32, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, None, None, 0, None) == INVALID
+    assert lib.vig_adamw_many(None, None, None, None, None, None, None, None, None, None, 1, 32, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, None, None, 0, None) == INVALID
 
 
 def test_grad_norm(lib):

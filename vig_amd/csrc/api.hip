@@ -1182,7 +1182,7 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
 }
 
 int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq, float* const* avg_scale,
-                   float* const* sq_scale, const long long* n, const int* param_dtype, const int* grad_dtype, int count, int state_bits, double lr,
+                   float* const* sq_scale, const long long* n, const long long* first, const int* param_dtype, const int* grad_dtype, int count, int state_bits, double lr,
                    double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,
                    const long long* step_on_device, const float* grad_scale, unsigned long long seed, void* stream) {
   if (!param || !grad || !exp_avg || !exp_avg_sq || !n || !param_dtype || !grad_dtype || count <= 0) return VIG_EINVAL;
@@ -1195,7 +1195,8 @@ int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp
   long long blocks = 0;
   for (int j = 0; j < count; ++j) {
     if (!dtype_ok(param_dtype[j]) || !dtype_ok(grad_dtype[j])) return VIG_ENOTSUP;
-    if (n[j] < 0) return VIG_EINVAL;
+    if (n[j] < 0 || (first && first[j] < 0)) return VIG_EINVAL;
+    if (first && first[j] > vig::kUpdateElements) return VIG_ENOTSUP;
     if (n[j] > vig::kUpdateElements || (blocks += (n[j] + 255) / 256) > vig::kUpdateElements / 256) return VIG_ENOTSUP;
     if (n[j] == 0) continue;
     if (!param[j] || !grad[j] || !exp_avg[j] || !exp_avg_sq[j] || (bits8 && (!avg_scale[j] || !sq_scale[j]))) return VIG_EINVAL;
@@ -1203,7 +1204,7 @@ int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp
     if (!bits8 && (!on_element(exp_avg[j], 4) || !on_element(exp_avg_sq[j], 4))) return VIG_EINVAL;
     if (bits8 && (!on_element(avg_scale[j], 4) || !on_element(sq_scale[j], 4))) return VIG_EINVAL;
   }
-  const vig::AdamW a{param, grad, exp_avg, exp_avg_sq, avg_scale, sq_scale, n, param_dtype, grad_dtype, count, state_bits, lr, beta1, beta2, eps, weight_decay, step,
+  const vig::AdamW a{param, grad, exp_avg, exp_avg_sq, avg_scale, sq_scale, n, first, param_dtype, grad_dtype, count, state_bits, lr, beta1, beta2, eps, weight_decay, step,
                      lr_on_device, step_on_device, grad_scale, seed};
   try {
     if (!apart(a)) return VIG_EINVAL;

@@ -16,6 +16,7 @@
 #include "common.h"
 #include "launch.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace vig {
 namespace {
@@ -26,6 +27,7 @@ constexpr int kTokens = 8;                 // of a thread, where a comment does 
 constexpr int kLanes = 16;                 // that take a token's channels
 constexpr int kRuns = 64 / kLanes;         // of tokens in a wave
 constexpr int kMaxWaves = 16;
+constexpr unsigned kMostThreads = 0xffffff00u;  // of a launch
 
 // N consecutive channels of one token as stored
 template <typename T, int N> struct Piece;
@@ -771,7 +773,7 @@ inline int start_rows(ScanArgs p, bool bwd, int B, hipStream_t stream) {
   const long long groups = (long long)B * p.groups;
   // Few workgroups finish sooner as the smaller ones of the other kernels (4 x 196 x 192, gradients of both directions 5.6 us for 7.6), and lanes behind
   // the last channel work for nothing (500 x 100 x 200: 38 for 52).
-  if (groups < 256 || groups > 0x7fffffffLL || p.groups * 2 * kHalf * 8 > p.D * 9) return 0;
+  if (groups < 256 || groups * (64 * kMaxWaves) > kMostThreads || p.groups * 2 * kHalf * 8 > p.D * 9) return 0;
   const int waves = (p.L + kStep - 1) / kStep;
   const size_t lds = (size_t)waves * kRows * (bwd ? p.g[1] ? 4 : 3 : 2);
   static bool allowed[3][64];
@@ -784,14 +786,8 @@ inline int start_rows(ScanArgs p, bool bwd, int B, hipStream_t stream) {
   return 1;
 }
 
-int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t stream) {
-  if (io_dtype == VIG_BF16 && gate_dtype == VIG_BF16 && start_rows(p, bwd, B, stream)) return hipGetLastError() == hipSuccess ? VIG_OK : VIG_ELAUNCH;
-  const bool pairs = whole(2, p.D, p.xb, p.xl, p.gb, p.gl) && on(2, io_dtype, p.x, p.d_o, p.o, p.dx) && on(2, gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
-  const Cut k = cut_for(B, p.L, p.D, pairs, p.g[1] != nullptr, bwd);
-  p.groups = k.groups, p.chunks = k.chunks, p.chunk = k.chunk;
-  const long long groups = (long long)B * k.groups * k.chunks;
-  if (groups > 0x7fffffffLL) return VIG_ENOTSUP;
-  const dim3 grid((unsigned)groups), block(64 * k.waves);
+int run_some(ScanArgs& p, bool bwd, int B, const Cut& k, int io_dtype, int gate_dtype, hipStream_t stream) {
+  const dim3 grid((unsigned)B * (unsigned)(k.groups * k.chunks)), block(64 * k.waves);
   for (int fold = k.chunks > 1; fold >= 0; --fold) {
     if (io_dtype == VIG_BF16) {
       if (gate_dtype == VIG_BF16) start<uint16_t, uint16_t>(p, bwd, fold, k, grid, block, stream);
@@ -801,6 +797,29 @@ int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t 
       else start<float, float>(p, bwd, fold, k, grid, block, stream);
     }
     if (hipGetLastError() != hipSuccess) return VIG_ELAUNCH;
+  }
+  return VIG_OK;
+}
+
+int run(ScanArgs& p, bool bwd, int B, int io_dtype, int gate_dtype, hipStream_t stream) {
+  if (io_dtype == VIG_BF16 && gate_dtype == VIG_BF16 && start_rows(p, bwd, B, stream)) return hipGetLastError() == hipSuccess ? VIG_OK : VIG_ELAUNCH;
+  const bool pairs = whole(2, p.D, p.xb, p.xl, p.gb, p.gl) && on(2, io_dtype, p.x, p.d_o, p.o, p.dx) && on(2, gate_dtype, p.g[0], p.g[1], p.dg[0], p.dg[1]);
+  const Cut k = cut_for(B, p.L, p.D, pairs, p.g[1] != nullptr, bwd);
+  p.groups = k.groups, p.chunks = k.chunks, p.chunk = k.chunk;
+  // a launch takes 2^32 threads at most: more batch elements go by several (each element's chunks alone have to fit)
+  const long long most = (long long)kMostThreads / (64 * k.waves) / ((long long)k.groups * k.chunks);
+  if (most < 1) return VIG_ENOTSUP;
+  const size_t sx = io_dtype == VIG_BF16 ? 2 : 4, sg = gate_dtype == VIG_BF16 ? 2 : 4;
+  const size_t dense = (size_t)p.L * p.D, maps = (size_t)(p.g[1] ? 2 : 1) * (bwd ? 2 : 1) * k.chunks * p.D * 2;
+  for (long long b = 0; b < B; b += most) {
+    ScanArgs q = p;
+    auto at = [](auto& t, size_t bytes) { t = t ? (std::remove_reference_t<decltype(t)>)((uintptr_t)t + bytes) : t; };
+    at(q.x, b * p.xb * sx), at(q.g[0], b * p.gb * sg), at(q.g[1], b * p.gb * sg), at(q.d_o, b * dense * sx), at(q.o, b * dense * sx), at(q.dx, b * dense * sx);
+    at(q.dg[0], b * dense * sg), at(q.dg[1], b * dense * sg), at(q.maps, k.chunks > 1 ? b * maps * sizeof(float) : 0);
+    for (auto* t : {&q.h0, &q.dhT}) at(*t, b * p.D * sizeof(float));
+    for (auto* t : {&q.hT, &q.dh0}) at(*t, b * p.D * sizeof(float));
+    const int rc = run_some(q, bwd, (int)std::min(most, B - b), k, io_dtype, gate_dtype, stream);
+    if (rc != VIG_OK) return rc;
   }
   return VIG_OK;
 }

@@ -153,7 +153,7 @@ struct AdamW {
   void* const* exp_avg_sq;
   float* const* avg_scale;  // states in 8 bits: a scale for each block of 256
   float* const* sq_scale;
-  const long long* n;
+  const long long *n, *first;  // first: number of a tensor's first element; null: tensors behind one another in whole blocks
   const int *param_dtype, *grad_dtype;
   int count, state_bits;
   double lr, beta1, beta2, eps, weight_decay;
@@ -163,7 +163,7 @@ struct AdamW {
   const float* grad_scale;           // null: 1
   unsigned long long seed;
 };
-constexpr long long kUpdateElements = 1LL << 40;  // of a list: its blocks of 256 are numbered in 32 bits
+constexpr long long kUpdateElements = 1LL << 40;  // of a list, and their numbers
 int launch_adamw(const AdamW& a, hipStream_t stream);
 size_t grad_norm_workspace(const long long* n, int count);
 int launch_grad_norm(const void* const* g, const long long* n, const int* dtype, int count, float max_norm, float* norm, float* scale, void* workspace,

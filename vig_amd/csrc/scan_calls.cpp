@@ -178,10 +178,10 @@ bool alike(const Tensor& a, const Tensor& b) {
 }  // namespace
 
 // adamw(params, grads, moments, moments, scales or None, scales or None, step (int or tensor), lr (float or tensor), beta1, beta2, eps, weight_decay, grad_scale or None,
-// seed): True, or None where ops.py has to see to an argument
+// seed, first numbers or None): True, or None where ops.py has to see to an argument
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 14, "adamw takes 14 arguments");
+  TORCH_CHECK_TYPE(n == 15, "adamw takes 15 arguments");
   List p, g, m, v, ms, vs;
   const bool bits8 = a[4] != Py_None;
   if (!tensors(a[0], p) || !tensors(a[1], g) || !tensors(a[2], m) || !tensors(a[3], v)) Py_RETURN_NONE;
@@ -206,6 +206,13 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const unsigned long long seed = PyLong_AsUnsignedLongLongMask(a[13]);
   if (PyErr_Occurred()) return nullptr;
+  std::vector<long long> first;
+  if (a[14] != Py_None) {
+    if (!PyList_CheckExact(a[14]) || PyList_GET_SIZE(a[14]) != (Py_ssize_t)count) Py_RETURN_NONE;
+    first.resize(count);
+    for (size_t j = 0; j < count; ++j) first[j] = PyLong_AsLongLong(PyList_GET_ITEM(a[14], j));
+    if (PyErr_Occurred()) return nullptr;
+  }
   std::vector<void*> pp(count), mp(count), vp(count);
   std::vector<const void*> gp(count);
   std::vector<float*> msp(bits8 ? count : 0), vsp(bits8 ? count : 0);
@@ -225,7 +232,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     msp[j] = ms[j]->data_ptr<float>(), vsp[j] = vs[j]->data_ptr<float>();
   }
   const c10::DeviceGuard guard(dev);
-  const int rc = vig_adamw_many(pp.data(), gp.data(), mp.data(), vp.data(), msp.data(), vsp.data(), sizes.data(), pd.data(), gd.data(), (int)count, bits8 ? 8 : 32, x[0],
+  const int rc = vig_adamw_many(pp.data(), gp.data(), mp.data(), vp.data(), msp.data(), vsp.data(), sizes.data(), first.empty() ? nullptr : first.data(), pd.data(), gd.data(), (int)count, bits8 ? 8 : 32, x[0],
                                 x[1], x[2], x[3], x[4], step, lr_t.defined() ? lr_t.const_data_ptr<float>() : nullptr,
                                 step_t.defined() ? reinterpret_cast<const long long*>(step_t.const_data_ptr<int64_t>()) : nullptr,
                                 scale_t.defined() ? scale_t.const_data_ptr<float>() : nullptr, seed, stream_of(*p[0]));

@@ -24,6 +24,7 @@ namespace {
 constexpr int kPiece = 2048;
 constexpr int kNormPiece = 8192;
 constexpr int kNormJobs = 192;
+constexpr unsigned kMostPieces = 0xffffffu;  // of a launch: it takes 2^32 threads at most
 
 // A launch's table: at most 4 KB of arguments in all.
 template <bool BITS8> struct UpdateJobs;
@@ -35,7 +36,7 @@ template <> struct UpdateJobs<false> {
   void* v[kMost];
   unsigned n[kMost];      // elements
   unsigned upto[kMost];   // pieces up to and with this tensor's
-  unsigned block[kMost];  // number of the tensor's first block of 256 in the whole list
+  unsigned first[kMost];  // number of the tensor's first element, from the launch's on
 };
 template <> struct UpdateJobs<true> {
   static constexpr int kMost = 64;
@@ -45,7 +46,7 @@ template <> struct UpdateJobs<true> {
   void* v[kMost];
   float* ms[kMost];
   float* vs[kMost];
-  unsigned n[kMost], upto[kMost], block[kMost];
+  unsigned n[kMost], upto[kMost], first[kMost];
 };
 
 struct UpdateScalars {
@@ -238,7 +239,7 @@ __device__ __forceinline__ int tensor_of(const unsigned* upto, unsigned count, u
 
 template <typename TP, typename TG, bool BITS8>
 __global__ __launch_bounds__(256) void adamw_kernel(UpdateJobs<BITS8> by_value, UpdateScalars s, const float* grad_scale, unsigned count, uint32_t key, unsigned long long seed,
-                                                    UpdateOnDevice dev) {
+                                                    unsigned long long from, UpdateOnDevice dev) {
   constexpr int E = BITS8 ? 8 : 4, kTurns = kPiece / (256 * E);
   const UpdateJobs<BITS8>* jobs = arguments<UpdateJobs<BITS8>>();
   const unsigned piece = blockIdx.x;
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(UpdateJobs<BITS8> by_value, 
   const unsigned first = (piece - (j ? jobs->upto[j - 1] : 0u)) * kPiece, n = jobs->n[j];
   void *const p = jobs->p[j], *const m = jobs->m[j], *const v = jobs->v[j];
   const void* const g = jobs->g[j];
-  const unsigned block0 = jobs->block[j];
+  const unsigned long long number0 = from + jobs->first[j];
   float P[kTurns][E], G[kTurns][E], M[kTurns][E], V[kTurns][E];
   auto load = [&](auto full) {
     constexpr bool FULL = decltype(full)::value;
@@ -294,11 +295,16 @@ __global__ __launch_bounds__(256) void adamw_kernel(UpdateJobs<BITS8> by_value, 
       float root[E];
       uint32_t word[E];
       if constexpr (BITS8 || sizeof(TP) == 2) {
-        // (numbers of elements in the whole list pass 32 bits: the upper ones go into the key)
-        const unsigned long long number = (unsigned long long)block0 * 256u + i;
-        const uint32_t k2 = key + (uint32_t)(number >> 32) * kGolden;
+        // (numbers of elements pass 32 bits: the upper ones go into the key)
+        const unsigned long long number = number0 + i;
+        const uint32_t low32 = (uint32_t)number, k2 = key + (uint32_t)(number >> 32) * kGolden;
 #pragma unroll
-        for (int e = 0; e < E; ++e) word[e] = mix(((uint32_t)number + e) ^ k2);
+        for (int e = 0; e < E; ++e) word[e] = mix((low32 + e) ^ k2);
+        if (low32 > ~0u - (E - 1)) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (low32 + e < low32) word[e] = mix((low32 + e) ^ (k2 + kGolden));
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) word[e] = 0u;
@@ -432,10 +438,11 @@ int launch_grad_norm(const void* const* g, const long long* n, const int* dtype,
     const size_t size = dtype[j] == VIG_BF16 ? 2 : 4;
     for (long long at = 0; at < n[j]; at += kMost) {
       const unsigned part = (unsigned)(n[j] - at < kMost ? n[j] - at : kMost);
-      if (used == kNormJobs || pieces >= 0x10000000u) {
+      const unsigned more = (part + kNormPiece - 1) / kNormPiece;
+      if (used == kNormJobs || pieces + more > kMostPieces) {
         if (!flush()) return VIG_ELAUNCH;
       }
-      pieces += (part + kNormPiece - 1) / kNormPiece;
+      pieces += more;
       jobs.g[used] = static_cast<const char*>(g[j]) + at * size, jobs.n[used] = part;
       jobs.upto[used++] = pieces | (dtype[j] == VIG_BF16 ? 0x80000000u : 0u);
     }
@@ -458,9 +465,10 @@ static int launch_adamw_of(const AdamW& a, hipStream_t stream) {
   for (int types = 0; types < 4; ++types) {
     UpdateJobs<BITS8> jobs;
     unsigned used = 0, pieces = 0;
+    unsigned long long from = 0;  // number of the launch's first element
     auto flush = [&]() {
       if (!used) return true;
-      auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(pieces), dim3(256), 0, stream, jobs, s, a.grad_scale, used, key, a.seed, dev); };
+      auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(pieces), dim3(256), 0, stream, jobs, s, a.grad_scale, used, key, a.seed, from, dev); };
       if (types == 0) start(adamw_kernel<float, float, BITS8>);
       else if (types == 1) start(adamw_kernel<float, uint16_t, BITS8>);
       else if (types == 2) start(adamw_kernel<uint16_t, float, BITS8>);
@@ -474,14 +482,17 @@ static int launch_adamw_of(const AdamW& a, hipStream_t stream) {
       const size_t sp = a.param_dtype[j] == VIG_BF16 ? 2 : 4, sg = a.grad_dtype[j] == VIG_BF16 ? 2 : 4, sm = BITS8 ? 1 : 4;
       for (long long at = 0; mine && at < a.n[j]; at += kMost) {
         const unsigned part = (unsigned)(a.n[j] - at < kMost ? a.n[j] - at : kMost);
-        if (used == UpdateJobs<BITS8>::kMost || pieces >= 0x10000000u) {
+        const unsigned long long number = (a.first ? (unsigned long long)a.first[j] : 256 * block) + at;
+        const unsigned more = (part + kPiece - 1) / kPiece;
+        if (used == UpdateJobs<BITS8>::kMost || pieces + more > kMostPieces || (used && (number < from || number - from > 0xffffffffULL))) {
           if (!flush()) return VIG_ELAUNCH;
         }
-        pieces += (part + kPiece - 1) / kPiece;
+        pieces += more;
         jobs.p[used] = static_cast<char*>(a.param[j]) + at * sp, jobs.g[used] = static_cast<const char*>(a.grad[j]) + at * sg;
         jobs.m[used] = static_cast<char*>(a.exp_avg[j]) + at * sm, jobs.v[used] = static_cast<char*>(a.exp_avg_sq[j]) + at * sm;
         if constexpr (BITS8) jobs.ms[used] = a.avg_scale[j] + at / 256, jobs.vs[used] = a.sq_scale[j] + at / 256;
-        jobs.n[used] = part, jobs.upto[used] = pieces, jobs.block[used++] = (unsigned)(block + at / 256);
+        if (!used) from = number;
+        jobs.n[used] = part, jobs.upto[used] = pieces, jobs.first[used++] = (unsigned)(number - from);
       }
       block += (unsigned long long)(a.n[j] + 255) / 256;
     }

@@ -1245,7 +1245,7 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
                avg_scales: Optional[Sequence[torch.Tensor]] = None, sq_scales: Optional[Sequence[torch.Tensor]] = None, *, step, lr=1e-3,
                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, grad_scale: Optional[torch.Tensor] = None,
-               seed: int = 0) -> None:
+               seed: int = 0, first: Optional[Sequence[int]] = None) -> None:
     """One AdamW step over lists of tensors, in place, in a few launches whatever their number:
 
         m <- b1 m + (1-b1) g,  v <- b2 v + (1-b2) g^2,  p <- p (1 - lr decay) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps),  g = grad_scale grad
@@ -1254,22 +1254,23 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     the states are held in 8 bits: exp_avgs m and exp_avg_sqs sqrt(v) as torch.float8_e4m3fn, times avg_scales[j], sq_scales[j], a
     float32 number for each 256 elements of tensor j (ceil(n/256) of them); all zeros is where they begin.  A block that takes in a value that is not finite is
     NaN from then on.  States in 8 bits and bf16 parameters are rounded stochastically, by a word made of seed, step and the element's
-    number in the list: the same calls give the same bits.
+    number: the same calls give the same bits.  Numbers go on from tensor to tensor in whole blocks of 256, or from first[j] in tensor j: a list that is part of a
+    larger one (a rank's share of the parameters) is rounded as the whole would be.
     step counts from 1; it and lr may be int64 and float32 numbers on the device (a captured step).  grad_scale: a float32 number there, as grad_norm gives it; NaN
     leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient."""
     params, grads, exp_avgs, exp_avg_sqs = (list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
-    avg_scales, sq_scales = (None if t is None else list(t) for t in (avg_scales, sq_scales))
+    avg_scales, sq_scales, first = (None if t is None else list(t) for t in (avg_scales, sq_scales, first))
     if not params:
         return
     calls = _ext.calls()
-    if calls is not None and calls.adamw(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed):
+    if calls is not None and calls.adamw(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed, first):
         return
     lib = _lib.load()
     bits8 = avg_scales is not None
     if bits8 != (sq_scales is not None):
         raise ValueError("states in 8 bits take scales for both moments")
     lists = [params, grads, exp_avgs, exp_avg_sqs] + ([avg_scales, sq_scales] if bits8 else [])
-    if any(len(t) != len(params) for t in lists):
+    if any(len(t) != len(params) for t in lists + ([first] if first is not None else [])):
         raise ValueError("lists of different lengths")
     _check_cuda(*(t for some in lists for t in some))
     dev = params[0].device
@@ -1296,11 +1297,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     n, p_dt, g_dt = _longs([t.numel() for t in params]), _ints([_dt(t) for t in params]), _ints([_dt(t) for t in kept])
     with torch.cuda.device(dev):
         rc = lib.vig_adamw_many(_pointers(params), _pointers(kept), _pointers(exp_avgs), _pointers(exp_avg_sqs), _pointers(lists[4]) if bits8 else None,
-                                _pointers(lists[5]) if bits8 else None, n, p_dt, g_dt, len(params), 8 if bits8 else 32, 0.0 if on_device(lr) else float(lr),
+                                _pointers(lists[5]) if bits8 else None, n, _longs(first) if first is not None else None, p_dt, g_dt, len(params), 8 if bits8 else 32, 0.0 if on_device(lr) else float(lr),
                                 betas[0], betas[1], eps, weight_decay, 1 if on_device(step) else step, on_device(lr), on_device(step), on_device(grad_scale),
                                 seed & (2 ** 64 - 1), _stream_ptr(params[0]))
     if rc == _lib.VIG_EINVAL:
-        raise ValueError("tensors that are written overlap one another or a gradient (a parameter twice in the list?)")
+        raise ValueError("tensors that are written overlap one another or a gradient (a parameter twice in the list?), or a first number is negative")
     _lib.check(rc, "vig_adamw_many")
     torch.autograd.graph.increment_version([t for some in [lists[0]] + lists[2:] for t in some if not t.is_inference()])
 
