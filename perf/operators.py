@@ -356,7 +356,9 @@ def _own(state):
     if case["clip"]:
         norm, scale = vig_amd.grad_norm(state["g"], max_norm=MAX_NORM)
     moments = (state["m"], state["v"]) if case["bits"] == 32 else (state["m"], state["r"], state["ms"], state["rs"])
-    vig_amd.adamw_step(state["p"], state["g"], *moments, step=state["t"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, grad_scale=scale, seed=SEED)
+    # (elements are numbered by their places in the flat buffers; tensors in whole blocks of 256 are so by themselves)
+    first = [t.storage_offset() for t in state["p"]] if case["tight"] and case["p"] == "bf16" else None
+    vig_amd.adamw_step(state["p"], state["g"], *moments, step=state["t"], lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, grad_scale=scale, seed=SEED, first=first)
     return {k: v for k, v in state["flat"].items() if k != "g"} | ({} if norm is None else {"norm": norm})
 
 
