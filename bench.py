@@ -124,22 +124,25 @@ def _enable_gemm_tuning(tune_gemm):
         return False
 
 
-def train_step_throughput(dev, batch=128, warmup=3, iters=10, tune_gemm=True):
+def train_step_throughput(dev, batch=128, warmup=3, iters=10, tune_gemm=True, optimizer="torch"):
     """ViG-S training steps (forward, cross-entropy, backward, AdamW update) on synthetic images: the differentiable
     path of the shell, whose kernels between the GEMMs are the library's in both directions.  fp32 as the reference's
-    configs train (vig-s.yaml: AMP off), and bf16 autocast."""
+    configs train (vig-s.yaml: AMP off), and bf16 autocast.  optimizer: torch's AdamW, or the library's ("library", "library-8bit")."""
     import torch
 
-    from vig_amd import layers
+    from vig_amd import layers, optim
 
     tuned = _enable_gemm_tuning(tune_gemm)
-    out = {"batch": batch, "iters": iters, "gemm_solution_tuning": "torch.cuda.tunable" if tuned else None}
+    out = {"batch": batch, "iters": iters, "optimizer": optimizer, "gemm_solution_tuning": "torch.cuda.tunable" if tuned else None}
     images = torch.randn(batch, 3, 224, 224, device=dev)
     target = torch.randint(0, 1000, (batch,), device=dev)
     for name, amp in (("fp32", False), ("bf16_autocast", True)):
         torch.manual_seed(0)
         model = layers.vig_small().to(dev).train()
-        opt = torch.optim.AdamW(model.parameters(), lr=1e-4)
+        if optimizer == "torch":
+            opt = torch.optim.AdamW(model.parameters(), lr=1e-4)
+        else:
+            opt = optim.AdamW(model.parameters(), lr=1e-4, state_bits=8 if optimizer == "library-8bit" else 32)
 
         def step():
             opt.zero_grad(set_to_none=True)
@@ -301,6 +304,8 @@ def main():
                     help="also time ViG-S training steps (differentiable path of the shell; fp32 and bf16 autocast)")
     ap.add_argument("--train-only", action="store_true",
                     help="time only the ViG-S training steps and print their JSON line (clean kernel traces)")
+    ap.add_argument("--optimizer", choices=("torch", "library", "library-8bit"), default="torch",
+                    help="with --train / --train-only: torch's AdamW (as ever) or the library's, with states in 32 or in 8 bits")
     ap.add_argument("--no-graph", action="store_true",
                     help="with --model: eager forwards only (no HIP graph capture, no batch-16 latency)")
     ap.add_argument("--unfused-gate", action="store_true",
@@ -330,7 +335,7 @@ def main():
     torch.cuda.set_device(dev)
 
     if args.train_only:
-        res = train_step_throughput(dev, tune_gemm=not args.no_gemm_tuning)
+        res = train_step_throughput(dev, tune_gemm=not args.no_gemm_tuning, optimizer=args.optimizer)
         print(json.dumps({"metric": "ViG-S training step images/sec @224^2 (forward + backward + AdamW)",
                           "value": res["bf16_autocast"]["images_per_s"], "unit": "images/s", "n_gpus": 1,
                           "ms_per_step": res["bf16_autocast"]["ms_per_step"], "higher_is_better": True,
@@ -492,7 +497,7 @@ def main():
         out["long_sequence"] = others["cfg3"]  # the 4096-token workload: the second named target
     if want_model:
         if args.train:
-            out["vig_s_train_step"] = train_step_throughput(dev, tune_gemm=not args.no_gemm_tuning)
+            out["vig_s_train_step"] = train_step_throughput(dev, tune_gemm=not args.no_gemm_tuning, optimizer=args.optimizer)
         out["vig_s_forward"] = model_throughput(dev, tune_gemm=not args.no_gemm_tuning, use_graph=not args.no_graph)
     if not args.no_cpu:
         out["cpu_baseline"] = cpu_baseline(s, 1000 + args.config)

@@ -4,6 +4,7 @@
 // are 720 addresses, sizes and types, which Python reads in 0.4 ms, twice what the kernels take.
 #include "host_calls.h"
 
+#include <deque>
 #include <vector>
 
 namespace vig_host {
@@ -219,9 +220,18 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::vector<long long> sizes(count);
   std::vector<int> pd(count), gd(count);
   const auto state = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(dev);
+  std::deque<Tensor> copies;  // (its elements stay where they are)
   for (size_t j = 0; j < count; ++j) {
-    for (const Tensor* t : {p[j], g[j], m[j], v[j]})
+    for (const Tensor* t : {p[j], m[j], v[j]})
       if (!simple(*t) || t->device() != dev || !alike(*t, *p[j])) Py_RETURN_NONE;
+    if (!simple(*g[j]) || g[j]->device() != dev || g[j]->sizes() != p[j]->sizes()) Py_RETURN_NONE;
+    if (!alike(*g[j], *p[j])) {  // (a convolution's weight gradient, channels last)
+      copies.push_back(at::empty_like(*p[j], p[j]->options().dtype(g[j]->scalar_type())));
+      copies.back().copy_(g[j]->detach());
+      g[j] = &copies.back();
+    }
     if (m[j]->scalar_type() != state || v[j]->scalar_type() != state) Py_RETURN_NONE;
     sizes[j] = p[j]->numel(), pd[j] = dtype_code(*p[j]), gd[j] = dtype_code(*g[j]);
     if (pd[j] < 0 || gd[j] < 0) Py_RETURN_NONE;
@@ -231,7 +241,6 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!simple(*t) || t->device() != dev || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != (sizes[j] + 255) / 256) Py_RETURN_NONE;
     msp[j] = ms[j]->data_ptr<float>(), vsp[j] = vs[j]->data_ptr<float>();
   }
-  const c10::DeviceGuard guard(dev);
   const int rc = vig_adamw_many(pp.data(), gp.data(), mp.data(), vp.data(), msp.data(), vsp.data(), sizes.data(), first.empty() ? nullptr : first.data(), pd.data(), gd.data(), (int)count, bits8 ? 8 : 32, x[0],
                                 x[1], x[2], x[3], x[4], step, lr_t.defined() ? lr_t.const_data_ptr<float>() : nullptr,
                                 step_t.defined() ? reinterpret_cast<const long long*>(step_t.const_data_ptr<int64_t>()) : nullptr,
