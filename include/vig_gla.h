@@ -815,8 +815,8 @@ int vig_sum_jobs_run(vig_sum_jobs* jobs, void* stream);
  * behind the last token.
  * x_strides, g_strides: elements between batch elements and between tokens, e.g. of the columns of a projection's rows
  * (NULL: dense); both gate tensors lie alike.  Tensors begin on any element (the exception to the 16-byte rule, as those of the update
- * below are; the workspace keeps it).  Any B, L >= 1 and D >= 1 with D and the token strides up to 524288 and L up to 2^30; four channels
- * move at once where D, the strides and the addresses are whole quads of elements.  Sums and states are held in fp32 and their order is fixed.
+ * below are; the workspace keeps it).  Any B, L >= 1 and D >= 1 with D and the token strides up to 262144 and L up to 2^30; lanes
+ * move two channels at once where D, the strides and the addresses are whole pairs, and many short bf16 sequences 16 bytes where they are whole eights.  Sums and states are held in fp32 and their order is fixed.
  * Outputs may not overlap inputs.  `workspace`: vig_gated_scan_fwd_workspace(...) bytes (0: may be NULL).
  */
 size_t vig_gated_scan_fwd_workspace(int B, int L, int D, int both);
@@ -850,7 +850,7 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
  * t = *step_on_device or, where that is NULL, step >= 1; lr likewise *lr_on_device or lr.  grad_scale NULL: 1; a NaN there leaves every tensor as it is.
  * state_bits 32: exp_avg = m and exp_avg_sq = v in fp32 (avg_scale, sq_scale are not read).
  * state_bits 8: m and r = sqrt(v) as e4m3 values times a scale for each 256 elements of a tensor (avg_scale[j], sq_scale[j]:
- * ceil(n[j] / 256) floats, the block's largest magnitude / 448).  A block that takes in a value that is not finite is NaN from then on.
+ * ceil(n[j] / 256) floats, the block's largest magnitude / 448; where v is below fp32's normal range, r lies between 0 and its root).  A block that takes in a value that is not finite is NaN from then on.
  * States in 8 bits and bf16 parameters are rounded stochastically.  The element's word: w = mix(number ^ key), number = first[j] +
  * element (NULL: 256 * (blocks of 256 of the tensors in front) + element; its bits past 32 times 0x9E3779B9 are added to the key): a list that is part
  * of a larger one, on one of several ranks say, is rounded as the whole would be where first[] goes on from the others, key = mix(mix(mix(seed) + (seed >> 32)) + t) in

@@ -402,6 +402,37 @@ def test_on_another_stream_and_in_graphs():
 
 
 @pytest.mark.parametrize("both", [False, True])
+def test_the_widest_rows(both):
+    """1024 rows of 262144 channels in fp32, 2^30 bytes of one workgroup's reach; then a few channels of such rows."""
+    L, D = 1024, 1 << 18
+    announce(f"gated scan of {D} channels both={both}")
+    x, g, h0, do, dh = draw(1, L, D, F32, F32, both, 1, state=not both)
+    some = slice(D - 70, D)
+    for cut in (slice(None), some):
+        given = [t[..., cut].detach().requires_grad_() for t in ((x, g) if both else (x, g, h0))]
+        o, h = vig_amd.bid_gated_scan(*given) if both else vig_amd.gated_scan(*given, True)
+        got = torch.autograd.grad((o,) if both else (o, h), given, (do[..., cut],) if both else (do[..., cut], dh[:, cut]))
+        want = reference(x[..., some], g[..., some], None if both else h0[:, some], both, do[..., some], None if both else dh[:, some])
+        close(o[..., -70:], want["o"], "o"), close(got[0][..., -70:], want["dx"], "dx"), close(got[1][..., -70:], want["dg"], "dg")
+    with pytest.raises(Exception):
+        vig_amd.gated_scan(torch.zeros(1, 2, D + 1, device="cuda"), torch.zeros(1, 2, D + 1, device="cuda"))
+
+
+def test_no_second_derivative(monkeypatch):
+    x, g, h0, _, _ = draw(1, 9, 4, F32, F32, False, 1, state=True)
+    for way in range(2):
+        if way:
+            monkeypatch.setattr(_ext, "calls", lambda: None)
+        x = x.detach().requires_grad_()
+        o, _ = vig_amd.gated_scan(x, g, h0)
+        (dx,) = torch.autograd.grad(o.square().sum(), x, create_graph=True)
+        want = reference(x, g, h0, False, 2 * o)["dx"]
+        close(dx.detach(), (want[0], want[1] + 4 * U * want[0].abs().max()), "first")
+        with pytest.raises(RuntimeError):
+            dx.sum().backward()
+
+
+@pytest.mark.parametrize("both", [False, True])
 def test_more_sequences_than_a_launch_takes(both):
     """Seventy million sequences of two tokens: a launch takes 2^32 threads."""
     B = 70_000_000

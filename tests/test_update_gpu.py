@@ -462,6 +462,45 @@ def test_optimiser_keeps_its_state(bits, tmp_path):
     assert all(torch.equal(p, q) for p, q in zip(ours, other))
 
 
+def test_optimiser_becomes_capturable_and_back():
+    """The number of steps goes with the state, whichever way it is counted."""
+    w = torch.linspace(-1, 1, 5000, device="cuda")
+    make = lambda c, p: optim.AdamW([p], lr=1e-2, capturable=c)  # noqa: E731
+    want, ours = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    ref, opt = make(False, want), make(False, ours)
+    for i in range(6):
+        if i in (2, 4):  # to be captured from now on, and back
+            state = opt.state_dict()
+            state["param_groups"][0]["capturable"] = i == 2
+            opt = make(i == 2, ours)
+            opt.load_state_dict(state)
+        for o, p in ((ref, want), (opt, ours)):
+            p.grad = torch.cos(w * (i + 1))
+            o.step()
+    # (the two ways to the corrections agree but for a rounding a step)
+    assert float((want - ours).detach().abs().max()) <= 6 * 4 * U
+
+
+def test_refused_on_the_gpu():
+    c = Case([300, 20], (F32,), (F32,), False, 2)
+    cpu = torch.zeros(300)
+    for bad in (lambda: vig_amd.adamw_step([c.p[0], c.p[0]], c.g[:1] * 2, [c.m[0], c.m[0]], [c.v[0], c.v[0]], step=1), lambda: c.step(0), lambda: c.step(1, grad_scale=0.5),
+                lambda: c.step(torch.tensor(1)), lambda: c.step(1, lr=torch.tensor(0.1)), lambda: c.step(1, betas=(1.0, 0.9)), lambda: c.step(1, eps=-1.0), lambda: c.step(1, first=[0]),
+                lambda: c.step(1, first=[0, -1]), lambda: vig_amd.adamw_step(c.p, c.g, c.m, c.v[:1], step=1), lambda: vig_amd.adamw_step(c.p[:1], [cpu], c.m[:1], c.v[:1], step=1),
+                lambda: vig_amd.adamw_step(c.p, c.g, c.p, c.v, step=1), lambda: vig_amd.adamw_step(c.p, c.p, c.m, c.v, step=1),
+                lambda: vig_amd.adamw_step(c.p, c.g, [t.bfloat16() for t in c.m], c.v, step=1), lambda: vig_amd.adamw_step(c.p, c.g, c.m, c.v, c.ms, [torch.zeros(1, device="cuda")], step=1),
+                lambda: vig_amd.adamw_step([t.half() for t in c.p], c.g, c.m, c.v, step=1), lambda: vig_amd.adamw_step([c.p[0][::2]], [c.g[0][::2]], [c.m[0][::2]], [c.v[0][::2]], step=1),
+                lambda: vig_amd.grad_norm([c.g[0], cpu]), lambda: vig_amd.grad_norm([c.g[0].half()]), lambda: vig_amd.grad_norm(c.g, float("nan"))):
+        before = c.held()
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            bad()
+        after = c.held()
+        assert all(torch.equal(a, b) for k in ("p", "g", "m", "v") for a, b in zip(before[k], after[k]))
+    norm, _ = vig_amd.grad_norm([c.g[0][::2], c.g[1].expand(3, 20)])  # (gaps and repeats are copied)
+    want = math.sqrt(float(c.g[0][::2].double().square().sum()) + 3 * float(c.g[1].double().square().sum()))
+    assert abs(float(norm) - want) <= 2 * U * want
+
+
 def test_weight_copies_of_the_layers_follow():
     torch.manual_seed(0)
     norm = layers.RMSNorm(384).cuda()

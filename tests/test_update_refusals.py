@@ -31,7 +31,7 @@ def test_scan(lib):
                 dict(gb=5 * P, h0=4 * P), dict(gb=5 * P, hT=4 * P), dict(h0=4 * P + 2), dict(h0=4 * P, hT=4 * P), dict(xs=_strides(72, 7)), dict(gs=_strides(72, 0)), dict(xs=_strides(-1, 8)),
                 dict(L=5000, ws=P + 8, n=1 << 30)):
         assert fwd(**bad) == INVALID, bad
-    for unbuilt in (dict(io=2), dict(gd=-1), dict(D=(1 << 19) + 1), dict(L=(1 << 30) + 1), dict(xs=_strides(0, (1 << 19) + 1)), dict(B=1, L=1 << 30, D=1 << 19, ws=4 * P, n=1 << 62)):
+    for unbuilt in (dict(io=2), dict(gd=-1), dict(D=(1 << 18) + 1), dict(L=(1 << 30) + 1), dict(xs=_strides(0, (1 << 18) + 1)), dict(B=1, L=1 << 30, D=1 << 18, ws=4 * P, n=1 << 62)):
         assert fwd(**unbuilt) == UNBUILT, unbuilt
     need = lib.vig_gated_scan_fwd_workspace(2, 5000, 8, 0)
     assert need > 0 and lib.vig_gated_scan_fwd_workspace(2, 5000, 8, 1) == 2 * need and lib.vig_gated_scan_bwd_workspace(2, 5000, 8, 1) == 4 * need

@@ -703,6 +703,8 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(const TX* x, const
   store_some(h + at, v), store_some(o + at, v);
 }
 
+static_assert(16LL * kRuns * kMaxWaves * kScanRow * 4 <= kBeyond, "byte offsets of a workgroup's rows");
+
 // ---- host side
 
 struct Cut {

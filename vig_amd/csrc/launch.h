@@ -131,8 +131,8 @@ struct GatedScan {
   float out_scale;
   int io_dtype, gate_dtype;
 };
-// Widest row and largest distance between rows, in elements: a workgroup's rows stay within 2^30 bytes of its first.
-constexpr long long kScanRow = 1 << 19;
+// Widest row and largest distance between rows, in elements: a workgroup's 1024 rows stay within 2^30 bytes of its first.
+constexpr long long kScanRow = 1 << 18;
 size_t gated_scan_workspace(int B, int L, int D, bool both, bool bwd);
 int launch_gated_scan(const GatedScan& s, hipStream_t stream);
 struct GatedScanStep {

@@ -4,6 +4,8 @@
 // are 720 addresses, sizes and types, which Python reads in 0.4 ms, twice what the kernels take.
 #include "host_calls.h"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <deque>
 #include <vector>
 
@@ -14,7 +16,7 @@ namespace {
 Tensor rows(const Tensor& t) {
   const int64_t d = t.dim(), pitch = t.stride(d - 2);
   const bool side = t.size(d - 1) == 1 || t.stride(d - 1) == 1;
-  return side && (t.size(d - 2) == 1 || (pitch >= t.size(d - 1) && pitch <= (1 << 19))) ? t : t.contiguous();
+  return side && (t.size(d - 2) == 1 || (pitch >= t.size(d - 1) && pitch <= (1 << 18))) ? t : t.contiguous();
 }
 // (batch, token) strides; a row alone is as far from the next as it is wide
 struct Strides {
@@ -32,7 +34,7 @@ bool scan_call(const Tensor& x, const Tensor& g, const Tensor& h0, bool both) {
   if (!simple(x) || !simple(g) || x.dim() != 3 || g.dim() != 3 || g.device() != x.device()) return false;
   if (g.size(0) != x.size(0) * (both ? 2 : 1) || g.size(1) != x.size(1) || g.size(2) != x.size(2)) return false;
   if (dtype_code(x) < 0 || dtype_code(g) < 0) return false;
-  if (x.numel() == 0 || x.size(0) > (1 << 30) || x.size(1) > (1 << 30) || x.size(2) > (1 << 19)) return false;
+  if (x.numel() == 0 || x.size(0) > (1 << 30) || x.size(1) > (1 << 30) || x.size(2) > (1 << 18)) return false;
   if (h0.defined() && (both || !simple(h0) || h0.device() != x.device() || h0.scalar_type() != at::kFloat || h0.dim() != 2 || h0.size(0) != x.size(0) ||
                        h0.size(1) != x.size(2)))
     return false;
@@ -89,6 +91,15 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                                 dh0.defined() ? dh0.data_ptr<float>() : nullptr, need ? ws.data_ptr() : nullptr, need, B, L, D, sx.v, sg.v,
                                 (float)ctx->saved_data["scale"].toDouble(), dtype_code(x), dtype_code(g), stream_of(x)),
              "vig_gated_scan_bwd");
+    if (at::GradMode::is_enabled()) {  // (create_graph: the gradients' own gradients are refused when they are asked for, and not left out of a sum)
+      variable_list found;
+      for (Tensor* t : {&dx, &dg, &dh0})
+        if (t->defined()) found.push_back(t->set_requires_grad(true));
+      const auto refuse = std::make_shared<torch::autograd::DelayedError>("gated_scan has no second derivative", (int64_t)found.size());
+      found = (*refuse)(variable_list(found));
+      dx = found[0], dg = found[1];
+      if (dh0.defined()) dh0 = found[2];
+    }
     return {dx, dg, dh0, Tensor(), Tensor(), Tensor()};
   }
 };
@@ -185,6 +196,7 @@ PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 15, "adamw takes 15 arguments");
   List p, g, m, v, ms, vs;
   const bool bits8 = a[4] != Py_None;
+  if (bits8 != (a[5] != Py_None)) Py_RETURN_NONE;
   if (!tensors(a[0], p) || !tensors(a[1], g) || !tensors(a[2], m) || !tensors(a[3], v)) Py_RETURN_NONE;
   if (bits8 && (!tensors(a[4], ms) || !tensors(a[5], vs))) Py_RETURN_NONE;
   const size_t count = p.size();

@@ -1186,6 +1186,7 @@ class _GatedScanFunction(torch.autograd.Function):
         return _gated_scan_raw(x, g, h0, both, want_final)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_final):
         lib = _lib.load()
         x, g, h0 = ctx.saved_tensors
@@ -1274,6 +1275,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError("lists of different lengths")
     _check_cuda(*(t for some in lists for t in some))
     dev = params[0].device
+    if grad_scale is not None and not isinstance(grad_scale, torch.Tensor):
+        raise TypeError("grad_scale must be a float32 number on the tensors' device, as grad_norm gives it")
     for name, t, dtype in (("step", step, torch.int64), ("lr", lr, torch.float32), ("grad_scale", grad_scale, torch.float32)):
         if isinstance(t, torch.Tensor) and (t.dtype != dtype or t.numel() != 1 or t.device != dev):
             raise ValueError(f"{name} must be one {dtype} number on the tensors' device")

@@ -90,7 +90,9 @@ class AdamW(torch.optim.Optimizer):
         if str(device) not in counts:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: run one step outside of the capture first")
-            counts[str(device)] = torch.zeros((), dtype=torch.int64, device=device)
+            # (steps that were counted one by one, before the group became capturable)
+            done = max((self.state[p]["step"] for p in group["params"] if p.device == device and p in self.state), default=0)
+            counts[str(device)] = torch.full((), done, dtype=torch.int64, device=device)
         return counts[str(device)].add_(1)
 
     def load_state_dict(self, state_dict):
@@ -105,3 +107,6 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             if "step_on_device" in group:
                 group["step_on_device"] = {k: v.to(k).clone() for k, v in group["step_on_device"].items()}
+                for p in group["params"]:
+                    if p in self.state and str(p.device) in group["step_on_device"]:
+                        self.state[p]["step"] = int(group["step_on_device"][str(p.device)])
