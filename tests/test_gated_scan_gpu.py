@@ -418,6 +418,30 @@ def test_the_widest_rows(both):
         vig_amd.gated_scan(torch.zeros(1, 2, D + 1, device="cuda"), torch.zeros(1, 2, D + 1, device="cuda"))
 
 
+def test_a_capture_with_a_leaf_that_an_eager_graph_holds():
+    """Refused while the graph lives; captured and replayed once it is gone."""
+    x, g, h0, do, dh = draw(2, 70, 10, F32, F32, False, 3, state=True)
+    leaves = [t.detach().requires_grad_() for t in (x, g, h0)]
+    alive = vig_amd.gated_scan(*leaves)[0]
+    want = torch.autograd.grad(alive, leaves, do, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still holds a leaf"):
+        with torch.cuda.graph(graph):
+            vig_amd.gated_scan(*leaves)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, _ = vig_amd.gated_scan(*leaves)
+        got = torch.autograd.grad(o, leaves, do)
+    for _ in range(3):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_second_derivative(monkeypatch):
     x, g, h0, _, _ = draw(1, 9, 4, F32, F32, False, 1, state=True)
     for way in range(2):

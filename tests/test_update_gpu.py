@@ -3,6 +3,7 @@
 Bounds.  u = 2^-24.  A moment is two products and a sum of constants rounded once: off by at most 4 u of the sum of its terms' magnitudes (g's square and the clip's
 product add 3 u of that term).  The parameter's step has eight more roundings: 12 u of itself, its moment's relative error and half of the square's.  A rounding to 8 or
 16 bits by given random bits is a function Q that never falls: what lies within d of x ends between Q(x - d) and Q(x + d), which differ for few."""
+import copy
 import math
 
 import pytest
@@ -479,6 +480,42 @@ def test_optimiser_becomes_capturable_and_back():
             o.step()
     # (the two ways to the corrections agree but for a rounding a step)
     assert float((want - ours).detach().abs().max()) <= 6 * 4 * U
+
+
+def test_optimiser_counts_where_it_is_told():
+    """Captured, not captured, saved and captured again, by the group's own entry or a loaded state: the count goes on."""
+    w = torch.linspace(-1, 1, 5000, device="cuda")
+    p = torch.nn.Parameter(w.clone())
+    opt = optim.AdamW([p], lr=1e-2)
+    for i, capturable in enumerate((True, True, False, False, True, False)):
+        opt.param_groups[0]["capturable"] = capturable
+        p.grad = w.cos()
+        opt.step()
+        state = opt.state_dict()
+        opt = optim.AdamW([p], lr=1e-2)
+        opt.load_state_dict(state)
+        counted = opt.param_groups[0].get("step_on_device", {"": opt.state[p]["step"]})
+        assert [int(v) for v in counted.values()] == [i + 1]
+        assert capturable == ("step_on_device" in opt.param_groups[0])
+
+
+def test_optimiser_copied_and_taken_over_from_torch():
+    w = torch.linspace(-1, 1, 5000, device="cuda")
+    want, ours = torch.nn.Parameter(w.clone()), torch.nn.Parameter(w.clone())
+    ref, opt = torch.optim.AdamW([want], lr=1e-2), optim.AdamW([ours], lr=1e-2, max_norm=1e9, seed=5)
+    for i in range(6):
+        for o, q in ((ref, want), (opt, ours)):
+            q.grad = torch.cos(w * (i + 1))
+            o.step()
+        if i == 1:
+            opt.load_state_dict(ref.state_dict())
+        if i == 3:
+            opt, ours = copy.deepcopy((opt, ours))
+            assert opt.max_norm == 1e9 and opt.seed == 5
+    # (each side's step is off by a few roundings of the parameter, at most 1, and of a move of at most lr (1 + its part of the moments' roundings))
+    assert float((want - ours).detach().abs().max()) <= 6 * 8 * U
+    with pytest.raises(ValueError):
+        opt.load_state_dict(torch.optim.AdamW([want], amsgrad=True).state_dict())
 
 
 def test_refused_on_the_gpu():

@@ -4,6 +4,7 @@
 // are 720 addresses, sizes and types, which Python reads in 0.4 ms, twice what the kernels take.
 #include "host_calls.h"
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <deque>
@@ -106,6 +107,16 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 
 bool records(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// A leaf's gradient is added up on the stream of the graph that first used it, as long as one lives.  Where that is the default stream a captured backward pass would
+// wait there, which breaks the capture in a destructor and ends the process: refused before anything is recorded.
+void refuse_held_leaf(const Tensor& t) {
+  if (!records(t) || !t.is_leaf()) return;
+  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!held || !held->stream()) return;
+  TORCH_CHECK(held->stream()->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
+              "gated_scan: a graph recorded on the default stream still holds a leaf that is captured here; drop that graph (its outputs) or detach the leaf first");
+}
+
 // What was written behind autograd's back: tensors saved for a backward pass notice.
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -124,6 +135,8 @@ PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double out_scale = both ? 0.5 : 1.0;
   Tensor o, final;
   if (at::GradMode::is_enabled() && (records(x) || records(g) || records(h0))) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      for (const Tensor* t : {&x, &g, &h0}) refuse_held_leaf(*t);
     const auto out = GatedScan::apply(x, g, h0.defined() ? std::optional<Tensor>(h0) : std::nullopt, both, want, out_scale);
     o = out[0];
     if (want) final = out[1];

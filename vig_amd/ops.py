@@ -1067,7 +1067,8 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     x has; a token of x = 0, g = 0 changes nothing (padding), g = -inf starts a new sequence behind the last one (packed
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
     and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
-    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd)."""
+    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once.  In a graph capture, leaves that
+    a graph recorded on the default stream still holds are refused: their gradients would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
 
 
@@ -1147,7 +1148,7 @@ def _gated_scan(x, g, initial_state, both, want_final):
 def _scan_rows(t):
     """t as it lies where its channels stand side by side in rows that do not overlap, else packed."""
     side = t.shape[-1] == 1 or t.stride(-1) == 1
-    return t if side and (t.shape[-2] == 1 or t.shape[-1] <= t.stride(-2) <= 1 << 19) else t.contiguous()
+    return t if side and (t.shape[-2] == 1 or t.shape[-1] <= t.stride(-2) <= 1 << 18) else t.contiguous()
 
 
 def _scan_strides(t):

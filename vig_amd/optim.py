@@ -34,6 +34,9 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm, self.seed, self.grad_norm = max_norm, seed, None
         super().__init__(params, {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay, "state_bits": state_bits, "capturable": capturable})
 
+    def __getstate__(self):
+        return super().__getstate__() | {"max_norm": self.max_norm, "seed": self.seed, "grad_norm": None}
+
     def _state_of(self, p, group):
         state = self.state[p]
         if not state:
@@ -59,6 +62,8 @@ class AdamW(torch.optim.Optimizer):
             if grads:
                 self.grad_norm, scale = ops.grad_norm(grads, self.max_norm)
         for group, params in todo:
+            if not group["capturable"]:
+                self._count_here(group)
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and not lr.is_cuda:
                 lr = float(lr)
@@ -95,8 +100,17 @@ class AdamW(torch.optim.Optimizer):
             counts[str(device)] = torch.full((), done, dtype=torch.int64, device=device)
         return counts[str(device)].add_(1)
 
+    def _count_here(self, group):
+        """Steps that the device has counted so far, back to the parameters' own numbers."""
+        counts = group.pop("step_on_device", {})
+        for p in group["params"]:
+            if p in self.state and str(p.device) in counts:
+                self.state[p]["step"] = int(counts[str(p.device)])
+
     def load_state_dict(self, state_dict):
-        """As torch.optim's, but states keep the types they were saved in (8 bits among them)."""
+        """As torch.optim's, but states keep the types they were saved in (8 bits among them).  Takes torch.optim.AdamW's too."""
+        if any(group.get("amsgrad") or group.get("maximize") for group in state_dict["param_groups"]):
+            raise ValueError("AdamW has neither amsgrad nor maximize")
         super().load_state_dict(state_dict)
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
@@ -104,9 +118,12 @@ class AdamW(torch.optim.Optimizer):
             for name, value in state_dict["state"].get(i, {}).items():
                 if isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device).clone(memory_format=torch.preserve_format)
+            if "step" in self.state.get(p, {}):
+                self.state[p]["step"] = int(self.state[p]["step"])
         for group in self.param_groups:
+            for name in ("state_bits", "capturable"):
+                group.setdefault(name, self.defaults[name])
             if "step_on_device" in group:
                 group["step_on_device"] = {k: v.to(k).clone() for k, v in group["step_on_device"].items()}
-                for p in group["params"]:
-                    if p in self.state and str(p.device) in group["step_on_device"]:
-                        self.state[p]["step"] = int(group["step_on_device"][str(p.device)])
+                if not group["capturable"]:
+                    self._count_here(group)
