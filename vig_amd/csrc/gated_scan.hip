@@ -13,6 +13,11 @@
 // Backward: dh_t = do_t + e^{g_{t+1}} dh_{t+1}; with D_t = e^{g_t} dh_t, what token t hands back, the walk against the direction is D -> e^{g_t} (do_t + D), an
 // affine map again, and dx_t = dh_t, dg_t = dh_t u_t with u_t = e^{g_t} h_{t-1} from the walk along it, recomputed in 32 bits from x and g (the stored
 // output is rounded, and for both directions holds their sum).
+//
+// Measured, bf16 (a large copy: 5.3 TB/s of reads and writes).  One workgroup a sequence, 128 x 196 x 384: both directions 14.8 us, 5.2 TB/s, with the last calls' tensors in the
+// 256 MB cache, 21.7 and 3.6 past it, causal 13.5 past it, 4.3, gradients of both 33 to 36, 4.3 to 4.7, where the arithmetic of four maps begins to count.  Chunks, 65536 x 1024: folding 63 us, 4.2 TB/s (loads alone in this pattern of 64-byte rows 53, in rows of 128
+// bytes 48; with the next rows on their way during the arithmetic no less, and more registers a thread, 143 to 158 us for both launches), walking 82, 4.9; fp32, 4 x 2305 x 333: 7 and 10,
+// gradients 10 and 15, of 420 workgroups each.
 #include "common.h"
 #include "launch.h"
 #include <algorithm>
@@ -688,6 +693,7 @@ __device__ __forceinline__ void store_some(uint16_t* p, const float (&x)[4]) {
   *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
 }
 
+// 14 bytes a channel in bf16, and nothing to wait for but memory: 2048 x 1024 5.8 us, 5.0 TB/s; one sequence of 384 channels 1.4 us, less than its launch.
 template <typename TX, typename TG, int N>
 __global__ __launch_bounds__(256) void gated_scan_step_kernel(const TX* x, const TG* g, float* h, TX* o, unsigned n, unsigned per_row, long long xl, long long gl, int D) {
   const unsigned id = blockIdx.x * 256u + threadIdx.x;

@@ -7,7 +7,7 @@
 // Both are bound by memory: every tensor is read once, what changes is written once, 16 bytes a lane.  A launch takes a table of tensors in its
 // arguments (nothing is copied to the device, so that a captured launch holds all it needs); a workgroup takes one piece of 2048 elements
 // (norm: 8192) and finds its tensor by comparing its number with the tensors' last pieces, one a lane.  Measured (us, TB/s; a large copy by torch: 5.3): fp32, 89 M parameters 417,
-// 6.0; in 8 bits beside fp32 282, 5.1, beside bf16 187, 4.8, where the arithmetic (75 instructions an element) comes near the memory's time; norm of 89 M bf16 32, 5.5.
+// 6.0; in 8 bits beside fp32 282, 5.1, beside bf16 165 to 187, 4.8 to 5.4, where the arithmetic (75 instructions an element) comes near the memory's time; norm of 89 M bf16 32, 5.5.
 //
 // 8 bits: blocks of 256 elements, counted from each tensor's first, hold m and r = sqrt(v) as e4m3 values times a scale of max / 448.  (The root: v spans
 // twice the octaves that e4m3 has.)  Rounding is stochastic: by the nearest value a moment would stand still, as a step of e4m3 is 6 to 12 % and b2 moves v
