@@ -418,6 +418,19 @@ def test_the_widest_rows(both):
         vig_amd.gated_scan(torch.zeros(1, 2, D + 1, device="cuda"), torch.zeros(1, 2, D + 1, device="cuda"))
 
 
+@pytest.mark.parametrize("native", [True, False])
+def test_inference_mode(native, monkeypatch):
+    if not native:
+        monkeypatch.setattr(_ext, "calls", lambda: None)
+    x, g, h0, _, _ = draw(3, 5, 12, F32, F32, False, 7, state=True)
+    with torch.inference_mode():
+        h = h0.clone()
+        o = torch.stack([vig_amd.gated_scan_step(x[:, t], g[:, t], h) for t in range(5)], 1)
+        whole, last = vig_amd.gated_scan(x.clone(), g, h0, True)
+    want = reference(x, g, h0, False)
+    close(o, want["o"], "steps"), close(whole, want["o"], "o"), close(h, want["final"], "state"), close(last, want["final"], "state")
+
+
 def test_a_capture_with_a_leaf_that_an_eager_graph_holds():
     """Refused while the graph lives; captured and replayed once it is gone."""
     x, g, h0, do, dh = draw(2, 70, 10, F32, F32, False, 3, state=True)

@@ -1105,7 +1105,8 @@ def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> to
     with torch.cuda.device(x.device):
         rc = lib.vig_gated_scan_step(x.data_ptr(), g.data_ptr(), state.data_ptr(), o.data_ptr(), B, D, pitch(x), pitch(g), io_dt, g_dt, _stream_ptr(x))
     _lib.check(rc, "vig_gated_scan_step")
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return o
 
 
