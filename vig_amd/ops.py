@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -931,6 +932,14 @@ def observed() -> bool:
     return torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() > 0
 
 
+def _recorded() -> bool:
+    """Whether a trace is among those that observe: what it does not see is missing from what it computes later."""
+    if torch._C._get_tracing_state() is not None:
+        return True
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor") if torch._C._len_torch_dispatch_stack() else None
+    return fx is not None and fx.get_proxy_mode() is not None
+
+
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x @ weight.T (+ bias): vig_linear_fwd for bf16 rows at the sizes where it is the better choice, torch's product
     otherwise.  Inference only (no autograd node of its own)."""
@@ -1067,7 +1076,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     x has; a token of x = 0, g = 0 changes nothing (padding), g = -inf starts a new sequence behind the last one (packed
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
     and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
-    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once.  In a graph capture, leaves that
+    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once.  A trace holds it as an operator.  In a graph capture, leaves that
     a graph recorded on the default stream still holds are refused: their gradients would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
 
@@ -1087,7 +1096,6 @@ def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> to
         o = calls.gated_scan_step(x, g, state)
         if o is not None:
             return o
-    lib = _lib.load()
     _check_cuda(x, g, state)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, g, state)):
         raise ValueError("gated_scan_step updates its state in place and records no gradient; use gated_scan")
@@ -1095,7 +1103,15 @@ def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> to
         raise ValueError("x, g and state must be [B,D]")
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("state must be a contiguous float32 tensor (it is updated in place)")
-    io_dt, g_dt = _dt(x), _dt(g)
+    _dt(x), _dt(g)
+    if observed():
+        return torch.ops.vig_amd.gated_scan_step(x, g, state)
+    return _gated_scan_step_launch(x, g, state)
+
+
+def _gated_scan_step_launch(x, g, state):
+    lib = _lib.load()
+    _check_cuda(x, g, state)
     B, D = x.shape
     o = torch.empty(B, D, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
@@ -1103,7 +1119,7 @@ def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> to
     x, g = _scan_rows(x), _scan_rows(g)
     pitch = lambda t: D if B == 1 else t.stride(0)  # noqa: E731
     with torch.cuda.device(x.device):
-        rc = lib.vig_gated_scan_step(x.data_ptr(), g.data_ptr(), state.data_ptr(), o.data_ptr(), B, D, pitch(x), pitch(g), io_dt, g_dt, _stream_ptr(x))
+        rc = lib.vig_gated_scan_step(x.data_ptr(), g.data_ptr(), state.data_ptr(), o.data_ptr(), B, D, pitch(x), pitch(g), _dt(x), _dt(g), _stream_ptr(x))
     _lib.check(rc, "vig_gated_scan_step")
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)
@@ -1161,7 +1177,17 @@ def _second_gates(g, both):
 
 
 def _gated_scan_raw(x, g, h0, both, want_final):
+    if observed():
+        if both:
+            return torch.ops.vig_amd.bid_gated_scan_fwd(x, g), None
+        o, h = torch.ops.vig_amd.gated_scan_fwd(x, g, h0)
+        return o, h if want_final else None
+    return _gated_scan_launch(x, g, h0, both, want_final)
+
+
+def _gated_scan_launch(x, g, h0, both, want_final):
     lib = _lib.load()
+    _check_cuda(x, g, h0)
     x, g = _scan_rows(x), _scan_rows(g)
     h0 = h0.contiguous() if h0 is not None else None
     B, L, D = x.shape
@@ -1190,25 +1216,33 @@ class _GatedScanFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_final):
-        lib = _lib.load()
         x, g, h0 = ctx.saved_tensors
-        x, g, both = _scan_rows(x), _scan_rows(g), ctx.both
-        h0 = h0.contiguous() if h0 is not None else None
-        B, L, D = x.shape
-        dense = lambda dtype, n: torch.empty(n, L, D, dtype=dtype, device=x.device)  # noqa: E731
-        d_o = d_o.contiguous() if d_o is not None else torch.zeros_like(dense(x.dtype, B))
-        d_final = d_final.contiguous() if d_final is not None else None
-        dx, dg = dense(x.dtype, B), dense(g.dtype, 2 * B if both else B)
-        dh0 = torch.empty_like(h0) if h0 is not None and ctx.needs_input_grad[2] else None
-        need = lib.vig_gated_scan_bwd_workspace(B, L, D, int(both))
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-        with torch.cuda.device(x.device):
-            rc = lib.vig_gated_scan_bwd(ptr(x), ptr(g), _second_gates(g, both), ptr(h0), ptr(d_o), ptr(d_final), ptr(dx), ptr(dg), _second_gates(dg, both),
-                                        ptr(dh0), ptr(ws), need, B, L, D, _scan_strides(x), _scan_strides(g), 0.5 if both else 1.0, _dt(x), _dt(g),
-                                        _stream_ptr(x))
-        _lib.check(rc, "vig_gated_scan_bwd")
-        return dx, dg, dh0, None, None
+        d_o = d_o if d_o is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+        wanted = h0 is not None and ctx.needs_input_grad[2]
+        if observed():
+            dx, dg, dh0 = torch.ops.vig_amd.gated_scan_bwd(x, g, h0, d_o, d_final, ctx.both)
+        else:
+            dx, dg, dh0 = _gated_scan_backward(x, g, h0, d_o, d_final, ctx.both, wanted)
+        return dx, dg, dh0 if wanted else None, None, None
+
+
+def _gated_scan_backward(x, g, h0, d_o, d_final, both, want_state):
+    lib = _lib.load()
+    _check_cuda(x, g, h0, d_o, d_final)
+    x, g, d_o = _scan_rows(x), _scan_rows(g), d_o.contiguous()
+    h0, d_final = (t.contiguous() if t is not None else None for t in (h0, d_final))
+    B, L, D = x.shape
+    dx, dg = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, g))
+    dh0 = torch.empty_like(h0) if want_state else None
+    need = lib.vig_gated_scan_bwd_workspace(B, L, D, int(both))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    with torch.cuda.device(x.device):
+        rc = lib.vig_gated_scan_bwd(ptr(x), ptr(g), _second_gates(g, both), ptr(h0), ptr(d_o), ptr(d_final), ptr(dx), ptr(dg), _second_gates(dg, both),
+                                    ptr(dh0), ptr(ws), need, B, L, D, _scan_strides(x), _scan_strides(g), 0.5 if both else 1.0, _dt(x), _dt(g),
+                                    _stream_ptr(x))
+    _lib.check(rc, "vig_gated_scan_bwd")
+    return dx, dg, dh0
 
 
 # ---------------------------------------------------------------------------
@@ -1229,6 +1263,14 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -
         r = calls.grad_norm(grads, max_norm)
         if r is not None:
             return r
+    _check_cuda(*grads)
+    if observed():
+        norm, scale = torch.ops.vig_amd.grad_norm([t.detach() for t in grads], float(max_norm or 0.0))
+        return norm, scale if max_norm is not None else None
+    return _grad_norm_launch(grads, max_norm)
+
+
+def _grad_norm_launch(grads, max_norm):
     lib = _lib.load()
     _check_cuda(*grads)
     grads = [t.detach() if _gapless(t) else t.detach().contiguous() for t in grads]
@@ -1260,7 +1302,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     number: the same calls give the same bits.  Numbers go on from tensor to tensor in whole blocks of 256, or from first[j] in tensor j: a list that is part of a
     larger one (a rank's share of the parameters) is rounded as the whole would be.
     step counts from 1; it and lr may be int64 and float32 numbers on the device (a captured step).  grad_scale: a float32 number there, as grad_norm gives it; NaN
-    leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient."""
+    leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient, and is refused in a trace."""
     params, grads, exp_avgs, exp_avg_sqs = (list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
     avg_scales, sq_scales, first = (None if t is None else list(t) for t in (avg_scales, sq_scales, first))
     if not params:
@@ -1268,6 +1310,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     calls = _ext.calls()
     if calls is not None and calls.adamw(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, step, lr, betas[0], betas[1], eps, weight_decay, grad_scale, seed, first):
         return
+    if _recorded():
+        raise RuntimeError("adamw_step changes lists of tensors in place and cannot be recorded in a trace")
     lib = _lib.load()
     bits8 = avg_scales is not None
     if bits8 != (sq_scales is not None):
@@ -1331,3 +1375,54 @@ def _longs(v):
 
 def _ints(v):
     return (ctypes.c_int * len(v))(*v)
+
+
+# ---------------------------------------------------------------------------
+# the same as operators, for whoever records them
+# ---------------------------------------------------------------------------
+# A trace keeps the operators that it sees, and the calls above launch their kernels outside of the dispatcher: a trace of them would hold outputs that nothing writes.
+# Where somebody observes, they go through these instead (torch.ops.vig_amd.*, as the other kernels' in csrc/torch_ext.cpp), whose state and factor are always computed.
+
+_operators = torch.library.Library("vig_amd", "FRAGMENT")
+
+
+def _operator(schema, shapes):
+    def made(launch):
+        _operators.define(schema)
+        name = schema.split("(", 1)[0]
+        _operators.impl(name, launch, "CompositeExplicitAutograd")
+        _operators.impl(name, shapes, "Meta")
+        return launch
+
+    return made
+
+
+def _state_like(x):
+    return x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32)
+
+
+@_operator("gated_scan_fwd(Tensor x, Tensor g, Tensor? initial_state) -> (Tensor, Tensor)", lambda x, g, h0: (x.new_empty(x.shape), _state_like(x)))
+def _gated_scan_operator(x, g, h0):
+    return _gated_scan_launch(x, g, h0, False, True)
+
+
+@_operator("bid_gated_scan_fwd(Tensor x, Tensor g) -> Tensor", lambda x, g: x.new_empty(x.shape))
+def _bid_gated_scan_operator(x, g):
+    return _gated_scan_launch(x, g, None, True, False)[0]
+
+
+@_operator("gated_scan_bwd(Tensor x, Tensor g, Tensor? initial_state, Tensor d_o, Tensor? d_final, bool both) -> (Tensor, Tensor, Tensor)",
+           lambda x, g, h0, d_o, d_final, both: (x.new_empty(x.shape), g.new_empty(g.shape), _state_like(x) if h0 is not None else x.new_empty(0, dtype=torch.float32)))
+def _gated_scan_bwd_operator(x, g, h0, d_o, d_final, both):
+    dx, dg, dh0 = _gated_scan_backward(x, g, h0, d_o, d_final, both, h0 is not None)
+    return dx, dg, dh0 if dh0 is not None else x.new_empty(0, dtype=torch.float32)
+
+
+@_operator("gated_scan_step(Tensor x, Tensor g, Tensor(a!) state) -> Tensor", lambda x, g, state: x.new_empty(x.shape))
+def _gated_scan_step_operator(x, g, state):
+    return _gated_scan_step_launch(x, g, state)
+
+
+@_operator("grad_norm(Tensor[] grads, float max_norm) -> (Tensor, Tensor)", lambda grads, max_norm: tuple(grads[0].new_empty((), dtype=torch.float32) for _ in range(2)))
+def _grad_norm_operator(grads, max_norm):
+    return _grad_norm_launch(grads, max_norm)
