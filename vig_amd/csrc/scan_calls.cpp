@@ -105,6 +105,8 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
   }
 };
 
+// a tensor of forward-mode differentiation, whose tangent a launch would drop
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool records(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // A leaf's gradient is added up on the stream of the graph that first used it, as long as one lives.  Where that is the default stream a captured backward pass would
@@ -131,7 +133,7 @@ PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!is_tensor(a[0]) || !is_tensor(a[1]) || !(a[2] == Py_None || is_tensor(a[2]))) Py_RETURN_NONE;
   const Tensor &x = THPVariable_Unpack(a[0]), &g = THPVariable_Unpack(a[1]), h0 = tensor_arg(a[2]);
   const bool both = PyObject_IsTrue(a[3]), want = PyObject_IsTrue(a[4]);
-  if (!scan_call(x, g, h0, both) || (both && want) || observed()) Py_RETURN_NONE;
+  if (!scan_call(x, g, h0, both) || (both && want) || observed() || dual(x) || dual(g) || dual(h0)) Py_RETURN_NONE;
   const double out_scale = both ? 0.5 : 1.0;
   Tensor o, final;
   if (at::GradMode::is_enabled() && (records(x) || records(g) || records(h0))) {
@@ -164,7 +166,7 @@ PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor &x = THPVariable_Unpack(a[0]), &g = THPVariable_Unpack(a[1]), &h = THPVariable_Unpack(a[2]);
   if (!simple(x) || !simple(g) || !simple(h) || x.dim() != 2 || g.sizes() != x.sizes() || h.sizes() != x.sizes() || g.device() != x.device() ||
       h.device() != x.device() || dtype_code(x) < 0 || dtype_code(g) < 0 || h.scalar_type() != at::kFloat || !h.is_contiguous() || x.numel() == 0 ||
-      x.numel() >= (1LL << 31) - 256 || observed())
+      x.numel() >= (1LL << 31) - 256 || observed() || dual(x) || dual(g) || dual(h))
     Py_RETURN_NONE;
   if (at::GradMode::is_enabled() && (records(x) || records(g) || records(h))) Py_RETURN_NONE;
   const c10::DeviceGuard guard(x.device());

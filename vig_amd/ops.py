@@ -17,6 +17,7 @@ import sys
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ext, _lib
 
@@ -1076,7 +1077,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     x has; a token of x = 0, g = 0 changes nothing (padding), g = -inf starts a new sequence behind the last one (packed
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
     and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
-    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once.  A trace holds it as an operator.  In a graph capture, leaves that
+    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once; forward-mode derivatives are refused.  A trace holds it as an operator.  In a graph capture, leaves that
     a graph recorded on the default stream still holds are refused: their gradients would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
 
@@ -1099,6 +1100,7 @@ def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> to
     _check_cuda(x, g, state)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, g, state)):
         raise ValueError("gated_scan_step updates its state in place and records no gradient; use gated_scan")
+    _refuse_tangents("gated_scan_step", x, g, state)
     if x.dim() != 2 or g.shape != x.shape or state.shape != x.shape:
         raise ValueError("x, g and state must be [B,D]")
     if state.dtype != torch.float32 or not state.is_contiguous():
@@ -1152,6 +1154,7 @@ def _gated_scan(x, g, initial_state, both, want_final):
     if initial_state is not None and tuple(initial_state.shape) != (B, D):
         raise ValueError(f"initial_state must be [B,D] = {(B, D)}; got {tuple(initial_state.shape)}")
     _dt(x), _dt(g)
+    _refuse_tangents("gated_scan", x, g, initial_state)
     if x.numel() == 0:  # nothing happens to the state
         state = initial_state if initial_state is not None else torch.zeros(B, D, dtype=torch.float32, device=x.device)
         return x.clone(), state.clone() if want_final else None
@@ -1160,6 +1163,11 @@ def _gated_scan(x, g, initial_state, both, want_final):
     else:
         o, h = _gated_scan_raw(x, g, initial_state, both, want_final)
     return o, h
+
+
+def _refuse_tangents(name, *ts):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _scan_rows(t):
@@ -1252,7 +1260,7 @@ def _gated_scan_backward(x, g, h0, d_o, d_final, both, want_state):
 def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(norm, scale) of a list of tensors on one device as fp32 numbers there: the root of the sum of all squares (added up in fp64, in a fixed order) and, where
     max_norm is given, min(1, max_norm / (norm + 1e-6)), the factor that clips to it; NaN where the norm is not finite, with which
-    adamw_step leaves everything as it is.  Nothing waits for the GPU."""
+    adamw_step leaves everything as it is.  Nothing waits for the GPU.  Records no gradient of any mode."""
     grads = list(grads)
     if not grads:
         raise ValueError("no tensors")
@@ -1302,7 +1310,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     number: the same calls give the same bits.  Numbers go on from tensor to tensor in whole blocks of 256, or from first[j] in tensor j: a list that is part of a
     larger one (a rank's share of the parameters) is rounded as the whole would be.
     step counts from 1; it and lr may be int64 and float32 numbers on the device (a captured step).  grad_scale: a float32 number there, as grad_norm gives it; NaN
-    leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient, and is refused in a trace."""
+    leaves every tensor as it is.  The tensors that are written must not overlap one another or a gradient.  Records no gradient of any mode, and is refused in a trace."""
     params, grads, exp_avgs, exp_avg_sqs = (list(t) for t in (params, grads, exp_avgs, exp_avg_sqs))
     avg_scales, sq_scales, first = (None if t is None else list(t) for t in (avg_scales, sq_scales, first))
     if not params:
