@@ -4,8 +4,9 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import vig_amd
+from vig_amd import _ext
 
-from .test_recorded_calls import device, inputs  # noqa: F401
+from .test_recorded_calls import device, formula, inputs  # noqa: F401
 from .util import announce
 
 
@@ -29,3 +30,79 @@ def test_no_forward_derivative(call, which, leaf, device):  # noqa: F811
         with pytest.raises((RuntimeError, ValueError)):
             run(given | {which: forward_ad.make_dual(at, torch.ones_like(at))})
     assert bool(torch.isfinite(want).all())
+
+
+class OnGpu(torch.Tensor):
+    """A tensor in host memory that says it is on the GPU."""
+    is_cuda = property(lambda self: True)
+
+
+def kinds(made):
+    """The forms of a call: names of its leaves -> the call."""
+    x, g, h = made
+    heads = [t.detach()[:, None].requires_grad_() for t in (x, g, h)]
+    half = h.detach().bfloat16().requires_grad_()
+    return {
+        "plain": ([x, g, h], lambda: vig_amd.gated_scan(x, g, h)),
+        "heads": (heads, lambda: vig_amd.gated_scan(*heads)),
+        "heads, rows alone": (heads[:1], lambda: vig_amd.gated_scan(heads[0], heads[1].detach())),
+        "state in bf16": ([half], lambda: vig_amd.gated_scan(x.detach(), g.detach(), half)),
+        "both": ([x], lambda: vig_amd.bid_gated_scan(x, torch.cat([g, g]).detach())),
+    }
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("kind", ["plain", "heads", "heads, rows alone", "state in bf16", "both"])
+def test_leaves_are_looked_at_before_a_capture(kind, native, monkeypatch, request):
+    """The caller's own leaves, not what is made of them on the way, are asked for; where nothing can be asked, the call is refused."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    seen = []
+
+    class Calls:
+        gated_scan = staticmethod(lambda *a: None)
+
+        @staticmethod
+        def refuse_held_leaves(*ts):
+            seen.extend(ts)
+            raise RuntimeError("held")
+
+    request.getfixturevalue("formula")
+    monkeypatch.setattr(_ext, "calls", lambda: Calls if native else None)
+    leaves, call = kinds([t.as_subclass(OnGpu).detach().requires_grad_() for t in inputs("cpu", 1)])[kind]
+    with pytest.raises(RuntimeError, match="held" if native else "capture"):
+        call()
+    assert [id(t) for t in seen] == ([id(t) for t in leaves] if native else [])
+    with torch.no_grad():
+        call()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("kind", ["heads", "heads, rows alone", "state in bf16", "both"])
+def test_captures_of_held_leaves(kind, native, monkeypatch):
+    """Refused while an eager graph lives, whichever form the leaf comes in; captured and replayed once it is gone."""
+    announce(f"held leaves: {kind}, native {native}")
+    if not native:
+        monkeypatch.setattr(_ext, "calls", lambda: None)
+    leaves, call = kinds([t.requires_grad_() for t in inputs("cuda", 1, L=70)])[kind]
+    alive = call()[0]
+    d = torch.randn_like(alive)
+    want = torch.autograd.grad(alive, leaves, d, retain_graph=True)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()
+    if not native:
+        return
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call()[0], leaves, d)
+    for _ in range(3):
+        for t in got:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

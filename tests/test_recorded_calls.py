@@ -79,17 +79,23 @@ class Formula:
         return 0
 
 
+@pytest.fixture
+def formula(monkeypatch):
+    """The formula in place of the library, for tensors in host memory."""
+    lib = Formula()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_check_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_stream_ptr", lambda t: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+
+
 @pytest.fixture(params=["cpu", pytest.param("cuda", marks=pytest.mark.gpu), pytest.param("ctypes", marks=pytest.mark.gpu)])
 def device(request, monkeypatch):
     if request.param != "cuda":
         monkeypatch.setattr(_ext, "calls", lambda: None)
     if request.param != "cpu":
         return "cuda"
-    lib = Formula()
-    monkeypatch.setattr(_lib, "load", lambda: lib)
-    monkeypatch.setattr(ops, "_check_cuda", lambda *ts: None)
-    monkeypatch.setattr(ops, "_stream_ptr", lambda t: 0)
-    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    request.getfixturevalue("formula")
     return "cpu"
 
 

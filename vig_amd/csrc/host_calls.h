@@ -102,6 +102,7 @@ PyObject* stem_norm(PyObject*, PyObject* const* a, Py_ssize_t n);
 
 // the methods of scan_calls.cpp
 PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* refuse_held_leaves(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n);

@@ -166,6 +166,7 @@ PyMethodDef kMethods[] = {
     {"stem_conv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(stem_conv)), METH_FASTCALL, nullptr},
     {"stem_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(stem_norm)), METH_FASTCALL, nullptr},
     {"gated_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_scan)), METH_FASTCALL, nullptr},
+    {"refuse_held_leaves", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(refuse_held_leaves)), METH_FASTCALL, nullptr},
     {"gated_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_scan_step)), METH_FASTCALL, nullptr},
     {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL, nullptr},

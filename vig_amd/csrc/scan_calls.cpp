@@ -157,6 +157,17 @@ PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// refuse_held_leaves(tensors): raises for a leaf that a capture must not take (the caller has asked whether there is one)
+PyObject* refuse_held_leaves(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    TORCH_CHECK_TYPE(is_tensor(a[i]), "refuse_held_leaves takes tensors");
+    refuse_held_leaf(THPVariable_Unpack(a[i]));
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // gated_scan_step(x [B, D], g, state fp32, in place): o; None: not of that kind
 PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS

@@ -1078,7 +1078,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
     and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
     the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once; forward-mode derivatives are refused.  A trace holds it as an operator.  In a graph capture, leaves that
-    a graph recorded on the default stream still holds are refused: their gradients would be added up on that stream."""
+    a graph recorded on the default stream still holds are refused where a gradient is recorded (not under no_grad): it would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
 
 
@@ -1136,9 +1136,11 @@ def _gated_scan(x, g, initial_state, both, want_final):
         h0 = initial_state.reshape(B * H, D) if initial_state is not None and tuple(initial_state.shape) == (B, H, D) else initial_state
         if initial_state is not None and h0 is initial_state:
             raise ValueError(f"initial_state must be [B,H,D] = {(B, H, D)}; got {tuple(initial_state.shape)}")
+        _refuse_held_leaves(x, g, initial_state)
         o, h = _gated_scan(x.reshape(B * H, L, D), g.reshape(g.shape[0] * H, L, D), h0, both, want_final)
         return o.view(B, H, L, D), h.view(B, H, D) if h is not None else None
-    if initial_state is not None:
+    if initial_state is not None and initial_state.dtype != torch.float32:
+        _refuse_held_leaves(initial_state)
         initial_state = initial_state.float()
     calls = _ext.calls()
     if calls is not None:  # one native call for what the kernels take; None: not of that kind
@@ -1155,6 +1157,7 @@ def _gated_scan(x, g, initial_state, both, want_final):
         raise ValueError(f"initial_state must be [B,D] = {(B, D)}; got {tuple(initial_state.shape)}")
     _dt(x), _dt(g)
     _refuse_tangents("gated_scan", x, g, initial_state)
+    _refuse_held_leaves(x, g, initial_state)
     if x.numel() == 0:  # nothing happens to the state
         state = initial_state if initial_state is not None else torch.zeros(B, D, dtype=torch.float32, device=x.device)
         return x.clone(), state.clone() if want_final else None
@@ -1163,6 +1166,18 @@ def _gated_scan(x, g, initial_state, both, want_final):
     else:
         o, h = _gated_scan_raw(x, g, initial_state, both, want_final)
     return o, h
+
+
+def _refuse_held_leaves(*ts):
+    """Before leaves of the caller are taken into a captured call in another form than their own (the native call looks at what it is given by itself): a leaf whose
+    gradient would be added up on the default stream ends the process there.  Which stream that is only the native module can tell."""
+    leaves = [t for t in ts if t is not None and t.is_cuda and t.requires_grad and t.is_leaf]
+    if not (leaves and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()):
+        return
+    calls = _ext.calls()
+    if calls is None:
+        raise RuntimeError("gated_scan: a gradient of leaves is recorded in a capture by the native calls only (vig_amd/lib/vig_host.so); detach the leaves or run without gradients")
+    calls.refuse_held_leaves(*leaves)
 
 
 def _refuse_tangents(name, *ts):
