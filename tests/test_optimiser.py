@@ -1,0 +1,58 @@
+"""What optim.AdamW asks of the update and keeps beside it, with the update replaced by a record of its calls (no GPU is needed)."""
+import copy
+
+import pytest
+import torch
+
+from vig_amd import ops, optim
+
+F32, BF16, E4M3 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The calls of adamw_step as dicts, made to move the moments by one: what lies there is seen to be carried on."""
+    seen = []
+
+    def step(params, grads, avgs, sqs, avg_scales=None, sq_scales=None, **kw):
+        kw["step"] = int(kw["step"])
+        seen.append({"params": list(params), "avgs": list(avgs), "scales": avg_scales, **kw})
+        for t in avgs + sqs:
+            if t.dtype == F32:
+                t += 1
+
+    monkeypatch.setattr(ops, "adamw_step", step)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return seen
+
+
+def params(*shapes, dtype=F32):
+    return [torch.nn.Parameter(torch.zeros(s, dtype=dtype)) for s in shapes]
+
+
+def give(*ps):
+    for p in ps:
+        p.grad = torch.ones_like(p)
+
+
+def counts(calls):
+    """The count each parameter was last updated with."""
+    return {id(p): c["step"] for c in calls for p in c["params"]}
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("lies", [torch.contiguous_format, torch.channels_last])
+def test_states_of_torch_in_bf16(bits, lies, calls):
+    """torch holds the moments of bf16 parameters in bf16; they are fp32 here, lying as the parameter does."""
+    theirs, ours = (params((6, 5, 32, 8), (7,), dtype=BF16) for _ in range(2))
+    ours[0].data = ours[0].data.to(memory_format=lies)
+    ref, opt = torch.optim.AdamW(theirs), optim.AdamW(ours, state_bits=bits)
+    give(*theirs), give(*ours)
+    ref.step()
+    opt.load_state_dict(ref.state_dict())
+    opt.step()
+    assert counts(calls) == {id(p): 2 for p in ours}
+    for p, q in zip(theirs, ours):
+        for name in ("exp_avg", "exp_avg_sq"):
+            got = opt.state[q][name]
+            assert got.dtype == F32 and got.stride() == q.stride() and torch.equal(got, ref.state[p][name].float() + 1)

@@ -107,8 +107,9 @@ class AdamW(torch.optim.Optimizer):
             if p in self.state and str(p.device) in counts:
                 self.state[p]["step"] = int(counts[str(p.device)])
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """As torch.optim's, but states keep the types they were saved in (8 bits among them).  Takes torch.optim.AdamW's too."""
+        """As torch.optim's, but states keep the types they were saved in (8 bits among them; others are fp32).  Takes torch.optim.AdamW's too."""
         if any(group.get("amsgrad") or group.get("maximize") for group in state_dict["param_groups"]):
             raise ValueError("AdamW has neither amsgrad nor maximize")
         super().load_state_dict(state_dict)
@@ -116,7 +117,10 @@ class AdamW(torch.optim.Optimizer):
         params = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(ids, params):
             for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor):
+                if name in ("exp_avg", "exp_avg_sq") and value.dtype != torch.float8_e4m3fn and value.shape == p.shape:
+                    # (torch holds them in the parameter's type; they lie as the parameter does, whichever way it lay when they were saved)
+                    self.state[p][name] = torch.empty_like(p, dtype=torch.float32).copy_(value)
+                elif isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device).clone(memory_format=torch.preserve_format)
             if "step" in self.state.get(p, {}):
                 self.state[p]["step"] = int(self.state[p]["step"])
