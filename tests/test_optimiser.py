@@ -22,7 +22,6 @@ def calls(monkeypatch):
                 t += 1
 
     monkeypatch.setattr(ops, "adamw_step", step)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return seen
 
 
@@ -56,3 +55,42 @@ def test_states_of_torch_in_bf16(bits, lies, calls):
         for name in ("exp_avg", "exp_avg_sq"):
             got = opt.state[q][name]
             assert got.dtype == F32 and got.stride() == q.stride() and torch.equal(got, ref.state[p][name].float() + 1)
+
+
+def capture(monkeypatch, on=True):
+    monkeypatch.setattr(optim, "_capturing", lambda: on)
+
+
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_captures_that_replay_something_else(max_norm, calls, monkeypatch):
+    """Refused before anything is counted, made or recorded: a count on the host, and a state that the capture would make (and clear in each replay)."""
+    norms = []
+    monkeypatch.setattr(ops, "grad_norm", lambda grads, most: norms.append(len(grads)) or (None, None))
+    a, b, c = params((5000,), (3,), (4,))
+    opt = optim.AdamW([{"params": [a, b], "capturable": True}, {"params": [c]}], max_norm=max_norm)
+
+    def refused(words):
+        before = copy.deepcopy(opt.state_dict())
+        done = len(calls), len(norms)
+        capture(monkeypatch)
+        with pytest.raises(RuntimeError, match=words):
+            opt.step()
+        capture(monkeypatch, False)
+        after = opt.state_dict()
+        assert (len(calls), len(norms)) == done and str(after) == str(before)
+
+    give(a)
+    refused("outside of the capture")  # nothing has been there yet
+    opt.step()
+    give(c)
+    refused("capturable")
+    c.grad = None
+    give(b)
+    refused("outside of the capture")  # b has no state yet
+    opt.step()
+    capture(monkeypatch)
+    opt.step()
+    assert counts(calls)[id(a)] == 3
+    a.grad = b.grad = None
+    opt.step()  # (nothing to do)
+    assert counts(calls)[id(a)] == 3

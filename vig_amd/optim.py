@@ -10,6 +10,10 @@ from . import ops
 LEAST_8_BIT = 4096  # elements from which on a tensor's states are held in 8 bits: below, they weigh nothing beside its launch
 
 
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay; moments without amsgrad) in a few launches for all parameters together.
 
@@ -18,7 +22,7 @@ class AdamW(torch.optim.Optimizer):
     max_norm clips the gradients of all parameters, which must lie on one device, to that norm; `grad_norm` holds it afterwards, as a
     number on the device.  A step whose norm is not finite changes no parameter and no moment (it does count).
     capturable=True counts the steps of a parameter group on the device, so that step() can be captured into a graph and
-    replayed: run one step outside of the capture first, and give lr as a float32 tensor there if it is to change between replays.
+    replayed (without it a captured step is refused): run one step outside of the capture first, with gradients of the same parameters, and give lr as a float32 tensor there if it is to change between replays.
     Parameters' version counters are moved, so that copies of weights kept by the layers are renewed."""
 
     def __init__(self, params, lr=1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
@@ -56,6 +60,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         todo = [(group, [p for p in group["params"] if p.grad is not None]) for group in self.param_groups]
+        if _capturing():
+            self._check_capture(todo)
         scale = None
         if self.max_norm is not None:
             grads = [p.grad for _, params in todo for p in params]
@@ -89,12 +95,19 @@ class AdamW(torch.optim.Optimizer):
                 ops.adamw_step(*lists, step=t, lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, seed=self.seed)
         return loss
 
+    def _check_capture(self, todo):
+        """Before anything is recorded: a count on the host would be the same in each replay, and a state made here would be cleared by each."""
+        for group, params in todo:
+            if params and not group["capturable"]:
+                raise RuntimeError("AdamW: a parameter group whose step is captured has to be capturable")
+            counts = group.get("step_on_device", {})
+            if any(not self.state.get(p) or str(p.device) not in counts for p in params):
+                raise RuntimeError("AdamW: run one step outside of the capture first, with gradients of the same parameters")
+
     def _count(self, group, device):
         """The group's number of steps on the device, one further."""
         counts = group.setdefault("step_on_device", {})
         if str(device) not in counts:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW: run one step outside of the capture first")
             # (steps that were counted one by one, before the group became capturable)
             done = max((self.state[p]["step"] for p in group["params"] if p.device == device and p in self.state), default=0)
             counts[str(device)] = torch.full((), done, dtype=torch.int64, device=device)
