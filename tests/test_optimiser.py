@@ -94,3 +94,27 @@ def test_captures_that_replay_something_else(max_norm, calls, monkeypatch):
     a.grad = b.grad = None
     opt.step()  # (nothing to do)
     assert counts(calls)[id(a)] == 3
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+@pytest.mark.parametrize("name", ["cpu", "cuda:7"])
+def test_counts_of_another_device(name, capturable, calls):
+    """A checkpoint of a device that is not here, or that holds the parameters no longer: the count goes on where they are."""
+    ps = params((5000,), (3,))
+    opt = optim.AdamW(ps, capturable=True, state_bits=8)
+    give(*ps)
+    for _ in range(3):
+        opt.step()
+    state = copy.deepcopy(opt.state_dict())
+    group = state["param_groups"][0]
+    group["step_on_device"] = {name: v for v in group["step_on_device"].values()}
+    for s in state["state"].values():  # (as states were saved whose steps the group alone counted)
+        s["step"] = 0
+    group["capturable"] = capturable
+    others = params((5000,), (3,))
+    opt = optim.AdamW(others)
+    opt.load_state_dict(state)
+    assert ("step_on_device" in opt.param_groups[0]) == capturable
+    give(*others)
+    opt.step()
+    assert counts(calls)[id(others[0])] == counts(calls)[id(others[1])] == 4

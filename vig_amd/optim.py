@@ -88,7 +88,7 @@ class AdamW(torch.optim.Optimizer):
                 if t is None:
                     t = counted.get(device)
                     if t is None:
-                        t = counted[device] = self._count(group, device)
+                        t = counted[device] = self._count_of(group, device).add_(1)
                 lists = [[p for p, _ in some], [p.grad for p, _ in some]] + [[s[name] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
                 if bits8:
                     lists += [[s[name + "_scale"] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
@@ -104,14 +104,14 @@ class AdamW(torch.optim.Optimizer):
             if any(not self.state.get(p) or str(p.device) not in counts for p in params):
                 raise RuntimeError("AdamW: run one step outside of the capture first, with gradients of the same parameters")
 
-    def _count(self, group, device):
-        """The group's number of steps on the device, one further."""
+    def _count_of(self, group, device):
+        """The group's number of steps on the device."""
         counts = group.setdefault("step_on_device", {})
         if str(device) not in counts:
             # (steps that were counted one by one, before the group became capturable)
             done = max((self.state[p]["step"] for p in group["params"] if p.device == device and p in self.state), default=0)
             counts[str(device)] = torch.full((), done, dtype=torch.int64, device=device)
-        return counts[str(device)].add_(1)
+        return counts[str(device)]
 
     def _count_here(self, group):
         """Steps that the device has counted so far, back to the parameters' own numbers."""
@@ -140,7 +140,9 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             for name in ("state_bits", "capturable"):
                 group.setdefault(name, self.defaults[name])
-            if "step_on_device" in group:
-                group["step_on_device"] = {k: v.to(k).clone() for k, v in group["step_on_device"].items()}
-                if not group["capturable"]:
-                    self._count_here(group)
+            counts = group.pop("step_on_device", {})  # (by the devices of the program that saved them, which these parameters need not be on)
+            for p in group["params"]:
+                if counts and p in self.state:
+                    self.state[p]["step"] = int(counts[str(p.device)] if str(p.device) in counts else max(counts.values()))
+                    if group["capturable"]:
+                        self._count_of(group, p.device)
