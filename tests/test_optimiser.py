@@ -118,3 +118,74 @@ def test_counts_of_another_device(name, capturable, calls):
     give(*others)
     opt.step()
     assert counts(calls)[id(others[0])] == counts(calls)[id(others[1])] == 4
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_each_parameter_counts_its_own_steps(capturable, calls):
+    """One that joins late begins at 1, one that misses a step stands still in it, whether counted on the device, on the host, or saved and loaded in between."""
+    a, b, c = ps = params((5000,), (3,), (6,))
+    opt = optim.AdamW(ps, capturable=capturable)
+    want = dict.fromkeys(map(id, ps), 0)
+
+    def step(*some):
+        for p in ps:
+            p.grad = torch.ones_like(p) if any(p is q for q in some) else None
+        del calls[:]
+        opt.step()
+        for p in some:
+            want[id(p)] += 1
+        assert counts(calls) == {id(p): want[id(p)] for p in some}
+
+    step(a, c), step(a, c)
+    step(a, b, c)  # b joins
+    step(b, c)  # a misses one
+    step(a, b, c)
+    assert len(calls) == 3 and want == {id(a): 4, id(b): 3, id(c): 5}
+    assert [int(opt.state[p]["step"]) for p in ps] == [4, 3, 5]
+    opt.param_groups[0]["capturable"] = not capturable
+    step(a, b, c)
+    saved = copy.deepcopy(opt.state_dict())
+    assert ("step_on_device" in saved["param_groups"][0]) != capturable
+    opt = optim.AdamW(ps)
+    opt.load_state_dict(saved)
+    step(a, b, c), step(b)
+    opt.param_groups[0]["capturable"] = capturable
+    step(a, b, c)
+    opt, ps = copy.deepcopy((opt, ps))
+    a, b, c = ps
+    want = dict(zip(map(id, ps), want.values()))
+    step(a, b, c), step(a, c), step(a, b, c)
+    assert list(want.values()) == [10, 9, 11]
+
+
+def test_parameters_that_a_graph_counts_together(calls, monkeypatch):
+    """A replay moves one number for all of them: to count them apart is refused, before anything is counted or made, until the states are loaded anew."""
+    a, b = ps = params((5000,), (3,))
+    opt = optim.AdamW(ps, capturable=True)
+    give(a, b)
+    opt.step()
+    capture(monkeypatch)
+    opt.step()
+    a.grad = None
+    with pytest.raises(RuntimeError, match="gradients of the same parameters"):  # (in a capture, the number would be copied in each replay)
+        opt.step()
+    capture(monkeypatch, False)
+    before = str(opt.state_dict()), len(calls)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    assert (str(opt.state_dict()), len(calls)) == before
+    give(a)
+    opt.step()
+    assert counts(calls) == {id(a): 3, id(b): 3}
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    a.grad = None
+    opt.step()
+    assert counts(calls) == {id(a): 3, id(b): 4}
+    # both ways have been there before the captures: two graphs, each with what it counts
+    give(a)
+    opt.step()
+    capture(monkeypatch)
+    opt.step()
+    a.grad = None
+    opt.step()
+    assert counts(calls) == {id(a): 5, id(b): 7}

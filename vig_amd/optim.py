@@ -21,8 +21,9 @@ class AdamW(torch.optim.Optimizer):
     root), rounded stochastically; bf16 parameters are rounded stochastically too (vig_amd.adamw_step says how).  Two runs with the same `seed` give the same bits.
     max_norm clips the gradients of all parameters, which must lie on one device, to that norm; `grad_norm` holds it afterwards, as a
     number on the device.  A step whose norm is not finite changes no parameter and no moment (it does count).
-    capturable=True counts the steps of a parameter group on the device, so that step() can be captured into a graph and
+    capturable=True counts a parameter group's steps on the device, so that step() can be captured into a graph and
     replayed (without it a captured step is refused): run one step outside of the capture first, with gradients of the same parameters, and give lr as a float32 tensor there if it is to change between replays.
+    Each parameter counts the steps in which it had a gradient; those that a graph counts together have to go on together.
     Parameters' version counters are moved, so that copies of weights kept by the layers are renewed."""
 
     def __init__(self, params, lr=1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
@@ -62,63 +63,109 @@ class AdamW(torch.optim.Optimizer):
         todo = [(group, [p for p in group["params"] if p.grad is not None]) for group in self.param_groups]
         if _capturing():
             self._check_capture(todo)
+        elif self._captured and any(self._shared(group, params) & {id(t) for t in self._captured} for group, params in todo if group["capturable"]):
+            raise RuntimeError("AdamW: parameters whose steps a captured step counts together have gradients in different steps; load the states anew to count them apart")
         scale = None
         if self.max_norm is not None:
             grads = [p.grad for _, params in todo for p in params]
             if grads:
                 self.grad_norm, scale = ops.grad_norm(grads, self.max_norm)
         for group, params in todo:
-            if not group["capturable"]:
-                self._count_here(group)
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and not lr.is_cuda:
                 lr = float(lr)
+            if group["capturable"]:
+                self._count_there(group, params)
+            else:
+                self._count_here(group)
             calls = {}
             for p in params:
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW takes no sparse gradients")
                 state = self._state_of(p, group)
                 if group["capturable"]:
-                    t = None
+                    t = id(state["step"])
                 else:
                     t = state["step"] = state["step"] + 1
                 calls.setdefault((p.device, t, "exp_avg_scale" in state), []).append((p, state))
-            counted = {}
-            for (device, t, bits8), some in calls.items():
-                if t is None:
-                    t = counted.get(device)
-                    if t is None:
-                        t = counted[device] = self._count_of(group, device).add_(1)
+            for (_, _, bits8), some in calls.items():
                 lists = [[p for p, _ in some], [p.grad for p, _ in some]] + [[s[name] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
                 if bits8:
                     lists += [[s[name + "_scale"] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
-                ops.adamw_step(*lists, step=t, lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, seed=self.seed)
+                ops.adamw_step(*lists, step=some[0][1]["step"], lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, seed=self.seed)
         return loss
 
+    # Steps are counted for each parameter: state["step"] is a number on the host or, in a capturable group, one on the device, the same tensor for all that have had
+    # gradients in the same steps.  group["step_on_device"] lists those.
+
+    _captured = ()  # counts that a captured step moves
+
     def _check_capture(self, todo):
-        """Before anything is recorded: a count on the host would be the same in each replay, and a state made here would be cleared by each."""
+        """Before anything is recorded: a count on the host would be the same in each replay, and a state or a count made here would be made anew by each."""
         for group, params in todo:
             if params and not group["capturable"]:
                 raise RuntimeError("AdamW: a parameter group whose step is captured has to be capturable")
-            counts = group.get("step_on_device", {})
-            if any(not self.state.get(p) or str(p.device) not in counts for p in params):
+            if any(not self.state.get(p) or not isinstance(self.state[p]["step"], torch.Tensor) for p in params) or self._shared(group, params):
                 raise RuntimeError("AdamW: run one step outside of the capture first, with gradients of the same parameters")
+        self._captured += tuple({id(t): t for _, params in todo for t in (self.state[p]["step"] for p in params)}.values())
 
-    def _count_of(self, group, device):
-        """The group's number of steps on the device."""
-        counts = group.setdefault("step_on_device", {})
-        if str(device) not in counts:
-            # (steps that were counted one by one, before the group became capturable)
-            done = max((self.state[p]["step"] for p in group["params"] if p.device == device and p in self.state), default=0)
-            counts[str(device)] = torch.full((), done, dtype=torch.int64, device=device)
-        return counts[str(device)]
+    def _shared(self, group, params):
+        """The counts (by id) of parameters some of which have a gradient and some have none."""
+        if len(params) == len(group["params"]):
+            return set()
+        left = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p) and isinstance(self.state[p]["step"], torch.Tensor)}
+        return left & {id(self.state[p]["step"]) for p in params if self.state.get(p)}
+
+    def _count_there(self, group, params):
+        """The parameters' counts on the device, one further."""
+        for p in params:
+            self._state_of(p, group)
+        self._move_there(group)
+        apart, shared = {}, self._shared(group, params)
+        for p in params:
+            t = self.state[p]["step"]
+            if id(t) in shared:
+                if id(t) not in apart:
+                    apart[id(t)] = t.clone()
+                self.state[p]["step"] = apart[id(t)]
+        if apart:
+            self._list_counts(group)
+        for t in {id(t): t for t in (self.state[p]["step"] for p in params)}.values():
+            t.add_(1)
+
+    def _move_there(self, group):
+        """Counts on the host, as those of states just made, onto the device."""
+        made = {}
+        for p in group["params"]:
+            state = self.state.get(p)
+            if state and not isinstance(state["step"], torch.Tensor):
+                key = (p.device, state["step"])
+                if key not in made:
+                    made[key] = torch.full((), state["step"], dtype=torch.int64, device=p.device)
+                state["step"] = made[key]
+        if made:
+            self._list_counts(group)
+
+    def _list_counts(self, group):
+        group["step_on_device"] = listed = {}
+        for t in {id(t): t for t in (self.state[p]["step"] for p in group["params"] if self.state.get(p))}.values():
+            name, k = str(t.device), 1
+            while name in listed:
+                k += 1
+                name = f"{t.device} {k}"
+            listed[name] = t
 
     def _count_here(self, group):
-        """Steps that the device has counted so far, back to the parameters' own numbers."""
-        counts = group.pop("step_on_device", {})
+        """Steps that the device has counted so far, back to numbers on the host."""
+        if group.pop("step_on_device", None) is None:
+            return
+        known = {}
         for p in group["params"]:
-            if p in self.state and str(p.device) in counts:
-                self.state[p]["step"] = int(counts[str(p.device)])
+            t = self.state[p]["step"] if self.state.get(p) else 0
+            if isinstance(t, torch.Tensor):
+                if id(t) not in known:
+                    known[id(t)] = (int(t), t)
+                self.state[p]["step"] = known[id(t)][0]
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
@@ -126,23 +173,27 @@ class AdamW(torch.optim.Optimizer):
         if any(group.get("amsgrad") or group.get("maximize") for group in state_dict["param_groups"]):
             raise ValueError("AdamW has neither amsgrad nor maximize")
         super().load_state_dict(state_dict)
+        self._captured = ()
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
+        alone = set()  # parameters whose count is their group's
         for i, p in zip(ids, params):
             for name, value in state_dict["state"].get(i, {}).items():
                 if name in ("exp_avg", "exp_avg_sq") and value.dtype != torch.float8_e4m3fn and value.shape == p.shape:
                     # (torch holds them in the parameter's type; they lie as the parameter does, whichever way it lay when they were saved)
                     self.state[p][name] = torch.empty_like(p, dtype=torch.float32).copy_(value)
+                elif name == "step":
+                    self.state[p][name] = int(value)
+                    if not isinstance(value, torch.Tensor):
+                        alone.add(p)
                 elif isinstance(value, torch.Tensor):
                     self.state[p][name] = value.detach().to(p.device).clone(memory_format=torch.preserve_format)
-            if "step" in self.state.get(p, {}):
-                self.state[p]["step"] = int(self.state[p]["step"])
         for group in self.param_groups:
             for name in ("state_bits", "capturable"):
                 group.setdefault(name, self.defaults[name])
             counts = group.pop("step_on_device", {})  # (by the devices of the program that saved them, which these parameters need not be on)
             for p in group["params"]:
-                if counts and p in self.state:
+                if counts and p in alone:  # (a group's steps were once counted by one number for all)
                     self.state[p]["step"] = int(counts[str(p.device)] if str(p.device) in counts else max(counts.values()))
-                    if group["capturable"]:
-                        self._count_of(group, p.device)
+            if group["capturable"]:
+                self._move_there(group)
