@@ -189,3 +189,29 @@ def test_parameters_that_a_graph_counts_together(calls, monkeypatch):
     a.grad = None
     opt.step()
     assert counts(calls) == {id(a): 5, id(b): 7}
+
+
+def spans(calls):
+    """{parameter: its elements' numbers}"""
+    return {id(p): range(n, n + p.numel()) for c in calls for p, n in zip(c["params"], c["first"])}
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_no_two_elements_are_rounded_by_the_same_word(bits, capturable, calls):
+    """Numbers go on over groups and kinds of states, and stay a parameter's whichever others have gradients."""
+    a, b, c, d, e = ps = params((300,), (5000,), (4096,), (7,), (20, 300), dtype=BF16)
+    opt = optim.AdamW([{"params": [a, b]}, {"params": [c, d], "state_bits": 40 - bits}, {"params": [e], "capturable": not capturable}], state_bits=bits, capturable=capturable, seed=3)
+    give(*ps)
+    opt.step()
+    first = spans(calls)
+    assert len(first) == 5 and all(c["seed"] == 3 for c in calls)
+    taken = [set(range(r.start // 256, -(-r.stop // 256))) for r in first.values()]
+    assert all(r.start % 256 == 0 for r in first.values()) and sum(map(len, taken)) == len(set().union(*taken))
+    del calls[:]
+    a.grad = c.grad = None
+    opt.step()
+    opt.add_param_group({"params": params((9,), dtype=BF16)})
+    opt.step()
+    later = spans(calls)
+    assert sorted(later) == sorted(map(id, (b, d, e))) and all(first[k] == r for k, r in later.items())

@@ -77,3 +77,26 @@ def test_counts_of_a_captured_step(bits):
         # (the corrections of either way agree but for a rounding of 24 bits, which may turn codes of 8 bits over: a step of one is up to 1/8 of a moment, and a move is about lr)
         off = float((p - q).detach().abs().max())
         assert off <= (8 * 4 * 2.0 ** -24 * float(q.detach().abs().max()) if bits == 32 or p.numel() == 3 else 8 * 0.01 / 4)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_groups_of_equal_tensors_are_rounded_apart(bits):
+    """The same weights and gradients in two groups: the same update before the rounding, another one after it; and as one list whose numbers are given."""
+    announce(f"rounding over groups, states in {bits} bits")
+    w = made((5000,), dtype=torch.bfloat16)[0].detach()
+    ps = [torch.nn.Parameter(w.clone()) for _ in range(3)]
+    opt = optim.AdamW([{"params": ps[:1]}, {"params": ps[1:]}], lr=1e-3, state_bits=bits, seed=5)
+    for p in ps:
+        give(p)
+    opt.step()
+    step = torch.exp2(torch.floor(torch.log2(w.float().abs() * 1.01 + 2e-3)) - 7)  # of bf16, the larger one at a border
+    for p, q in ((ps[0], ps[1]), (ps[1], ps[2]), (ps[0], ps[2])):
+        off = (p - q).detach().float().abs()
+        # (a move of 1e-3 and a decay of 1e-5 are not bf16's steps of about 4e-3: most elements are rounded, one way or the other)
+        assert bool((off <= step).all()) and float((off > 0).float().mean()) > 0.05
+    alone = [torch.nn.Parameter(w.clone()) for _ in range(3)]
+    other = optim.AdamW(alone, lr=1e-3, state_bits=bits, seed=5)
+    for p in alone:
+        give(p)
+    other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, alone))

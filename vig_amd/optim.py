@@ -18,7 +18,7 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay; moments without amsgrad) in a few launches for all parameters together.
 
     state_bits=8 holds the moments of tensors of 4096 elements and more in 8 bits with a scale for each 256 (the second one as its
-    root), rounded stochastically; bf16 parameters are rounded stochastically too (vig_amd.adamw_step says how).  Two runs with the same `seed` give the same bits.
+    root), rounded stochastically; bf16 parameters are rounded stochastically too (vig_amd.adamw_step says how), by numbers that go on over all groups.  Two runs with the same `seed` give the same bits.
     max_norm clips the gradients of all parameters, which must lie on one device, to that norm; `grad_norm` holds it afterwards, as a
     number on the device.  A step whose norm is not finite changes no parameter and no moment (it does count).
     capturable=True counts a parameter group's steps on the device, so that step() can be captured into a graph and
@@ -70,6 +70,7 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for _, params in todo for p in params]
             if grads:
                 self.grad_norm, scale = ops.grad_norm(grads, self.max_norm)
+        numbers = None
         for group, params in todo:
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and not lr.is_cuda:
@@ -92,8 +93,23 @@ class AdamW(torch.optim.Optimizer):
                 lists = [[p for p, _ in some], [p.grad for p, _ in some]] + [[s[name] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
                 if bits8:
                     lists += [[s[name + "_scale"] for _, s in some] for name in ("exp_avg", "exp_avg_sq")]
-                ops.adamw_step(*lists, step=some[0][1]["step"], lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, seed=self.seed)
+                first = None
+                if bits8 or any(p.dtype == torch.bfloat16 for p, _ in some):  # (what is rounded by random words)
+                    numbers = numbers or self._numbers()
+                    first = [numbers[p] for p, _ in some]
+                ops.adamw_step(*lists, step=some[0][1]["step"], lr=lr, betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=scale, seed=self.seed,
+                               first=first)
         return loss
+
+    def _numbers(self):
+        """The number of each parameter's first element: they go on over all groups in blocks of 256, so that no two elements of a step are rounded by the same word,
+        and stay a parameter's own whichever others have gradients."""
+        numbers, n = {}, 0
+        for group in self.param_groups:
+            for p in group["params"]:
+                numbers[p] = n
+                n += -(-p.numel() // 256) * 256
+        return numbers
 
     # Steps are counted for each parameter: state["step"] is a number on the host or, in a capturable group, one on the device, the same tensor for all that have had
     # gradients in the same steps.  group["step_on_device"] lists those.
