@@ -1,10 +1,12 @@
 """Calls of the gated scan that have to be refused, on the GPU both ways and, with the library replaced by its formula, without one."""
+import os
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import vig_amd
-from vig_amd import _ext
+from vig_amd import _ext, _lib
 
 from .test_recorded_calls import device, formula, inputs  # noqa: F401
 from .util import announce
@@ -106,3 +108,38 @@ def test_captures_of_held_leaves(kind, native, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_sequences_longer_than_the_chunks_are_folded_for():
+    """Every chunk folds all in front of it: past 2^24 tokens the square of their number is refused."""
+    if not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("library not built here")
+    lib = _lib.load()
+    P, most = 1 << 20, 1 << 24
+    fwd = lambda L: lib.vig_gated_scan_fwd(P, 2 * P, None, None, 3 * P, None, None, 0, 1, L, 8, None, None, 1.0, 1, 1, None)  # noqa: E731
+    bwd = lambda L: lib.vig_gated_scan_bwd(P, 2 * P, None, None, 3 * P, None, 4 * P, 5 * P, None, None, None, 0, 1, L, 8, None, None, 1.0, 1, 1, None)  # noqa: E731
+    assert fwd(most) == bwd(most) == _lib.VIG_ENOSPC and lib.vig_gated_scan_fwd_workspace(1, most, 8, 1) > 0
+    assert fwd(most + 1) == bwd(most + 1) == _lib.VIG_ENOTSUP
+    assert lib.vig_gated_scan_fwd_workspace(1, most + 1, 8, 0) == lib.vig_gated_scan_bwd_workspace(1, most + 1, 8, 1) == 0
+
+
+@pytest.mark.gpu
+def test_the_longest_sequences():
+    """2^24 tokens that change nothing but for a few: sums of whole numbers, which are exact; one token more is refused."""
+    L, D = 1 << 24, 2
+    announce(f"gated scan of {L} tokens")
+    x = torch.zeros(1, L, D, device="cuda")
+    at = torch.tensor([0, 1, 511, 512, 70_000, 1 << 20, (1 << 23) + 5, L - 513, L - 1], device="cuda")
+    x[0, at, 0], x[0, at, 1] = torch.arange(1.0, 10.0, device="cuda"), 3.0
+    g, h0 = torch.zeros_like(x), torch.full((1, D), 5.0, device="cuda")
+    o, h = vig_amd.gated_scan(x, g, h0, True)
+    want = 5 + x.double().cumsum(1)
+    assert torch.equal(o.double(), want) and torch.equal(h.double(), want[:, -1])
+    x.requires_grad_()
+    o, _ = vig_amd.bid_gated_scan(x, torch.cat([g, g]))
+    back = x.detach().double().flip(1).cumsum(1).flip(1)
+    assert torch.equal(o.detach().double(), (want - 5 + back) / 2)
+    (dx,) = torch.autograd.grad(o, x, x.detach())
+    assert torch.equal(dx.double(), (want - 5 + back) / 2)
+    with pytest.raises(Exception):
+        vig_amd.gated_scan(torch.zeros(1, L + 1, 1, device="cuda"), torch.zeros(1, L + 1, 1, device="cuda"))

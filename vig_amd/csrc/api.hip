@@ -110,7 +110,7 @@ static bool aligned16(P... p) {
 }
 static int element_size(int dtype) { return dtype == VIG_BF16 ? 2 : 4; }
 static bool on_element(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
-static bool scan_sizes_ok(int B, int L, int D) { return B > 0 && L > 0 && D > 0 && L <= (1 << 30) && D <= vig::kScanRow; }
+static bool scan_sizes_ok(int B, int L, int D) { return B > 0 && L > 0 && D > 0 && L <= vig::kScanTokens && D <= vig::kScanRow; }
 // The arguments that the gated scan and its backward share: checked and put into `s`.
 static int scan_arguments(vig::GatedScan& s, void* workspace, int B, int L, int D, const long long* x_strides, const long long* g_strides, float out_scale,
                           int io_dtype, int gate_dtype) {

@@ -133,6 +133,9 @@ struct GatedScan {
 };
 // Widest row and largest distance between rows, in elements: a workgroup's 1024 rows stay within 2^30 bytes of its first.
 constexpr long long kScanRow = 1 << 18;
+// Most tokens.  Each chunk of a long sequence folds the maps of all others in front of it, so that the time grows with the square of the chunks: one causal bf16
+// sequence of 1024 channels takes 0.2 ms for 2^16 tokens, 4.8 for 2^20, one of 64 channels 0.2 for 2^20, 1.8 for 2^22, 23 for 2^24 (its rows alone: 1.2), and the next power four times that.
+constexpr int kScanTokens = 1 << 24;
 size_t gated_scan_workspace(int B, int L, int D, bool both, bool bwd);
 int launch_gated_scan(const GatedScan& s, hipStream_t stream);
 struct GatedScanStep {

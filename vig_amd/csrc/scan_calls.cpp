@@ -35,7 +35,7 @@ bool scan_call(const Tensor& x, const Tensor& g, const Tensor& h0, bool both) {
   if (!simple(x) || !simple(g) || x.dim() != 3 || g.dim() != 3 || g.device() != x.device()) return false;
   if (g.size(0) != x.size(0) * (both ? 2 : 1) || g.size(1) != x.size(1) || g.size(2) != x.size(2)) return false;
   if (dtype_code(x) < 0 || dtype_code(g) < 0) return false;
-  if (x.numel() == 0 || x.size(0) > (1 << 30) || x.size(1) > (1 << 30) || x.size(2) > (1 << 18)) return false;
+  if (x.numel() == 0 || x.size(0) > (1 << 30) || x.size(1) > (1 << 24) || x.size(2) > (1 << 18)) return false;
   if (h0.defined() && (both || !simple(h0) || h0.device() != x.device() || h0.scalar_type() != at::kFloat || h0.dim() != 2 || h0.size(0) != x.size(0) ||
                        h0.size(1) != x.size(2)))
     return false;

@@ -1076,7 +1076,8 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     The causal GLA ops' sibling whose state is one number a channel.  g: natural-log decays (<= 0), of any of the built dtypes whatever
     x has; a token of x = 0, g = 0 changes nothing (padding), g = -inf starts a new sequence behind the last one (packed
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
-    and behind the last token.  x and g may be columns of wider rows (read in place).  The state is held in fp32; the order of
+    and behind the last token.  x and g may be columns of wider rows (read in place; of four axes where heads and batch make one).  Up to 2^24 tokens, whose
+    time grows with the square of their number from about 2^18 on.  The state is held in fp32; the order of
     the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once; forward-mode derivatives are refused.  A trace holds it as an operator.  In a graph capture, leaves that
     a graph recorded on the default stream still holds are refused where a gradient is recorded (not under no_grad): it would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
