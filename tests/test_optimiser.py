@@ -215,3 +215,18 @@ def test_no_two_elements_are_rounded_by_the_same_word(bits, capturable, calls):
     opt.step()
     later = spans(calls)
     assert sorted(later) == sorted(map(id, (b, d, e))) and all(first[k] == r for k, r in later.items())
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_counts_that_move_while_one_stands_still(capturable, calls):
+    """Equal counts go to the device or back in a step that only one of their parameters takes."""
+    a, b = ps = params((5000,), (3,))
+    opt = optim.AdamW(ps, capturable=not capturable)
+    give(a, b)
+    opt.step(), opt.step()
+    opt.param_groups[0]["capturable"] = capturable
+    a.grad = None
+    opt.step()
+    give(a)
+    opt.step()
+    assert counts(calls) == {id(a): 3, id(b): 4}

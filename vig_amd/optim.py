@@ -75,16 +75,17 @@ class AdamW(torch.optim.Optimizer):
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and not lr.is_cuda:
                 lr = float(lr)
-            if group["capturable"]:
-                self._count_there(group, params)
+            states = [self._state_of(p, group) for p in params]
+            capturable = group["capturable"]
+            if capturable:
+                self._count_there(group, params, states)
             else:
                 self._count_here(group)
             calls = {}
-            for p in params:
+            for p, state in zip(params, states):
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW takes no sparse gradients")
-                state = self._state_of(p, group)
-                if group["capturable"]:
+                if capturable:
                     t = id(state["step"])
                 else:
                     t = state["step"] = state["step"] + 1
@@ -132,21 +133,20 @@ class AdamW(torch.optim.Optimizer):
         left = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p) and isinstance(self.state[p]["step"], torch.Tensor)}
         return left & {id(self.state[p]["step"]) for p in params if self.state.get(p)}
 
-    def _count_there(self, group, params):
+    def _count_there(self, group, params, states):
         """The parameters' counts on the device, one further."""
-        for p in params:
-            self._state_of(p, group)
-        self._move_there(group)
-        apart, shared = {}, self._shared(group, params)
-        for p in params:
-            t = self.state[p]["step"]
-            if id(t) in shared:
-                if id(t) not in apart:
-                    apart[id(t)] = t.clone()
-                self.state[p]["step"] = apart[id(t)]
-        if apart:
+        shared = self._shared(group, params)
+        if shared or not all(isinstance(s["step"], torch.Tensor) for s in states):
+            self._move_there(group)
+            shared, apart = self._shared(group, params), {}
+            for state in states:
+                t = state["step"]
+                if id(t) in shared:
+                    if id(t) not in apart:
+                        apart[id(t)] = t.clone()
+                    state["step"] = apart[id(t)]
             self._list_counts(group)
-        for t in {id(t): t for t in (self.state[p]["step"] for p in params)}.values():
+        for t in {id(s["step"]): s["step"] for s in states}.values():
             t.add_(1)
 
     def _move_there(self, group):
@@ -159,8 +159,6 @@ class AdamW(torch.optim.Optimizer):
                 if key not in made:
                     made[key] = torch.full((), state["step"], dtype=torch.int64, device=p.device)
                 state["step"] = made[key]
-        if made:
-            self._list_counts(group)
 
     def _list_counts(self, group):
         group["step_on_device"] = listed = {}
@@ -213,3 +211,4 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p]["step"] = int(counts[str(p.device)] if str(p.device) in counts else max(counts.values()))
             if group["capturable"]:
                 self._move_there(group)
+                self._list_counts(group)
