@@ -230,3 +230,16 @@ def test_counts_that_move_while_one_stands_still(capturable, calls):
     give(a)
     opt.step()
     assert counts(calls) == {id(a): 3, id(b): 4}
+
+
+def test_a_sparse_gradient_is_refused_before_anything_is_counted(calls, monkeypatch):
+    norms = []
+    monkeypatch.setattr(ops, "grad_norm", lambda grads, most: norms.append(1) or (None, None))
+    for capturable in (False, True):
+        a, b = ps = params((50,), (30, 2))
+        opt = optim.AdamW(ps, capturable=capturable, max_norm=1.0)
+        give(a)
+        b.grad = torch.ones_like(b).to_sparse()
+        with pytest.raises(RuntimeError, match="sparse"):
+            opt.step()
+        assert not opt.state[a] and not calls and not norms

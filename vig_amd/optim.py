@@ -61,6 +61,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         todo = [(group, [p for p in group["params"] if p.grad is not None]) for group in self.param_groups]
+        if any(p.grad.is_sparse for _, params in todo for p in params):
+            raise RuntimeError("AdamW takes no sparse gradients")
         if _capturing():
             self._check_capture(todo)
         elif self._captured and any(self._shared(group, params) & {id(t) for t in self._captured} for group, params in todo if group["capturable"]):
@@ -83,8 +85,6 @@ class AdamW(torch.optim.Optimizer):
                 self._count_here(group)
             calls = {}
             for p, state in zip(params, states):
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW takes no sparse gradients")
                 if capturable:
                     t = id(state["step"])
                 else:
