@@ -817,7 +817,8 @@ int vig_sum_jobs_run(vig_sum_jobs* jobs, void* stream);
  * (NULL: dense); both gate tensors lie alike.  Tensors begin on any element (the exception to the 16-byte rule, as those of the update
  * below are; the workspace keeps it).  Any B, L >= 1 and D >= 1 with D and the token strides up to 262144 and L up to 2^24 (VIG_ENOTSUP past them: from about 2^18 tokens on the time grows with
  * the square of L, 0.2 ms for a causal bf16 sequence of 64 channels and 2^20 tokens, 1.8 for 2^22, 23 for 2^24); lanes
- * move two channels at once where D, the strides and the addresses are whole pairs, and many short bf16 sequences 16 bytes where they are whole eights.  Sums and states are held in fp32 and their order is fixed.
+ * move two channels at once where D, the strides and the addresses are whole pairs, and many short bf16 sequences 16 bytes where they are whole eights.  Sums and states are held in fp32; their order is fixed by sizes,
+ * types and how the rows lie.
  * Outputs may not overlap inputs.  `workspace`: vig_gated_scan_fwd_workspace(...) bytes (0: may be NULL).
  */
 size_t vig_gated_scan_fwd_workspace(int B, int L, int D, int both);
@@ -835,7 +836,7 @@ int vig_gated_scan_bwd(const void* x, const void* g_fwd, const void* g_bwd, cons
                        size_t workspace_bytes, int B, int L, int D, const long long* x_strides, const long long* g_strides,
                        float out_scale, int io_dtype, int gate_dtype, void* stream);
 /*
- * One token of each of B sequences: state <- exp(g) state + x, o = state.  x, g [B, D] with rows x_stride, g_stride elements
+ * One token of each of B sequences: state <- exp(g) state + x, o = state.  state and o overlap nothing else.  x, g [B, D] with rows x_stride, g_stride elements
  * apart (0 = packed), state fp32 [B, D], o [B, D] of io_dtype.  B * D < 2^31 - 256.
  */
 int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int B, int D, long long x_stride, long long g_stride,

@@ -1078,7 +1078,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, initial_state: Optional[torch.T
     sequences).  A value that is not finite stays in its channel, past any gate.  initial_state and final_state: fp32 [B,D] ([B,H,D]), the state before the first
     and behind the last token.  x and g may be columns of wider rows (read in place; of four axes where heads and batch make one).  Up to 2^24 tokens, whose
     time grows with the square of their number from about 2^18 on.  The state is held in fp32; the order of
-    the sums is fixed.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once; forward-mode derivatives are refused.  A trace holds it as an operator.  In a graph capture, leaves that
+    the sums is fixed by sizes, types and how the rows lie.  Differentiable in x, g and initial_state, from o and final_state (vig_gated_scan_bwd), once; forward-mode derivatives are refused.  A trace holds it as an operator.  In a graph capture, leaves that
     a graph recorded on the default stream still holds are refused where a gradient is recorded (not under no_grad): it would be added up on that stream."""
     return _gated_scan(x, g, initial_state, False, bool(output_final_state))
 
@@ -1092,7 +1092,7 @@ def bid_gated_scan(x: torch.Tensor, g: torch.Tensor) -> Tuple[torch.Tensor, None
 
 def gated_scan_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     """gated_scan for one token of every sequence: state (fp32 [B,D], contiguous) <- e^g state + x in place, returned in x's dtype.
-    x, g: [B,D], or columns of wider rows.  Inference only."""
+    x, g: [B,D], or columns of wider rows, apart from state's memory.  Inference only."""
     calls = _ext.calls()
     if calls is not None:
         o = calls.gated_scan_step(x, g, state)
