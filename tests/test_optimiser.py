@@ -120,6 +120,30 @@ def test_counts_of_another_device(name, capturable, calls):
     assert counts(calls)[id(others[0])] == counts(calls)[id(others[1])] == 4
 
 
+def test_counts_of_several_devices(calls):
+    """Saved by a group on two devices, neither of which holds the parameters: the larger count, wherever the numbers lie."""
+    ps = params((5000,), (3,))
+    opt = optim.AdamW(ps, capturable=True)
+    give(*ps)
+    opt.step()
+    state = copy.deepcopy(opt.state_dict())
+
+    class There:
+        """A number on another device: it compares with nothing that lies elsewhere."""
+        def __init__(self, v):
+            self.v = v
+
+        def __int__(self):
+            return self.v
+
+    state["param_groups"][0]["step_on_device"] = {"cuda:6": There(3), "cuda:7": There(8)}
+    for s in state["state"].values():
+        s["step"] = 0
+    opt.load_state_dict(state)
+    opt.step()
+    assert set(counts(calls).values()) == {9}
+
+
 @pytest.mark.parametrize("capturable", [True, False])
 def test_each_parameter_counts_its_own_steps(capturable, calls):
     """One that joins late begins at 1, one that misses a step stands still in it, whether counted on the device, on the host, or saved and loaded in between."""

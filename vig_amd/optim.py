@@ -208,7 +208,7 @@ class AdamW(torch.optim.Optimizer):
             counts = group.pop("step_on_device", {})  # (by the devices of the program that saved them, which these parameters need not be on)
             for p in group["params"]:
                 if counts and p in alone:  # (a group's steps were once counted by one number for all)
-                    self.state[p]["step"] = int(counts[str(p.device)] if str(p.device) in counts else max(counts.values()))
+                    self.state[p]["step"] = int(counts[str(p.device)]) if str(p.device) in counts else max(map(int, counts.values()))
             if group["capturable"]:
                 self._move_there(group)
                 self._list_counts(group)
