@@ -843,6 +843,79 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
                         int io_dtype, int gate_dtype, void* stream);
 
 /*
+ * Selective state space scan: N numbers of state a channel, whose decays and inputs go by the token:
+ *
+ *   s_t = softplus(delta_t + delta_bias)            (delta_softplus 0: delta_t + delta_bias)
+ *   h_t[n] = exp(s_t A[n]) h_{t-1}[n] + s_t x_t B_t[n],   y_t = sum_n C_t[n] h_t[n] + D_skip x_t,   o_t = y_t silu(z_t)
+ *
+ * x, delta, z [batch, L, D], B, C [batch, L, G, N] (a group's for the D / G channels side by side), o dense, all of io_dtype; A [D, N], D_skip, delta_bias [D] fp32.
+ * D_skip, z (no gate), delta_bias may be NULL.  initial_state (NULL: zeros) and final_state (NULL: not wanted): fp32 [batch, D, N], in front of the first and
+ * behind the last token of the walk.  reverse: the walk goes from token L - 1 to token 0.  A token with a step of 0 (delta of -infinity in front of the softplus) and a
+ * finite x leaves the state as it is (padding).  N up to 64.
+ * *_strides: elements between batch elements and between tokens (B, C: and between groups), NULL: dense; channels, and a group's states, lie side by side.  Distances
+ * between tokens up to 262144.  Tensors begin on any element; `kept` and the workspaces on 16 bytes.
+ * kept: NULL, or vig_selective_scan_kept(...) bytes of states for vig_selective_scan_bwd.  Sums and states are held in fp32, in an order fixed by the sizes.
+ * Outputs may not overlap inputs.  VIG_ENOTSUP past 2^24 tokens, 2^18 channels, or 2^32 threads of a launch (batch times channels times N / 4 from about 2^32 on).
+ */
+size_t vig_selective_scan_fwd_workspace(int batch, int L, int D, int N, int G);
+size_t vig_selective_scan_kept(int batch, int L, int D, int N);
+int vig_selective_scan_fwd(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias,
+                           const float* initial_state, void* o, float* final_state, float* kept, void* workspace, size_t workspace_bytes, int batch, int L, int D, int N, int G,
+                           const long long* x_strides, const long long* delta_strides, const long long* B_strides, const long long* C_strides, const long long* z_strides,
+                           int delta_softplus, int reverse, int io_dtype, void* stream);
+/*
+ * Its gradients: d_o dense, d_final_state (NULL: zeros) -> dx, ddelta, dB, dC, dz (NULL exactly where z is), dense, of io_dtype, dA_dD_dbias: D N + 2 D floats, the gradients of
+ * A, D_skip and delta_bias behind one another (written whether or not the last two are given), and d_initial_state (NULL: not wanted).
+ */
+size_t vig_selective_scan_bwd_workspace(int batch, int L, int D, int N, int G);
+int vig_selective_scan_bwd(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias,
+                           const float* kept, const void* d_o, const float* d_final_state, void* dx, void* ddelta, void* dB, void* dC, void* dz, float* dA_dD_dbias,
+                           float* d_initial_state, void* workspace, size_t workspace_bytes, int batch, int L, int D, int N, int G, const long long* x_strides,
+                           const long long* delta_strides, const long long* B_strides, const long long* C_strides, const long long* z_strides, int delta_softplus, int reverse,
+                           int io_dtype, void* stream);
+/* One token of each of `batch` sequences, state fp32 [batch, D, N] in place; x, delta, z [batch, D] with rows *_stride elements apart (0: packed), B, C [batch, G, N] with strides of
+ * batch element and group (NULL: packed), o packed.  state and o overlap nothing else. */
+int vig_selective_scan_step(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias, float* state,
+                            void* o, int batch, int D, int N, int G, long long x_stride, long long delta_stride, const long long* B_strides, const long long* C_strides,
+                            long long z_stride, int delta_softplus, int io_dtype, void* stream);
+
+/*
+ * Causal convolution of W = 2, 3 or 4 taps along the tokens of each channel:
+ *
+ *   y_t = f(bias + sum_k weight[k] x_{t - W + 1 + k}),   f: silu, or nothing
+ *
+ * x [B, L, D] with x_strides (batch element, token; NULL: dense), weight [D, W] and bias [D] (NULL: none) fp32, y dense of io_dtype.  initial_state (NULL: zeros) holds the W - 1
+ * rows in front of the first token, final_state (NULL: not wanted) takes the last W - 1 rows: [B, W - 1, D] of io_dtype in the order of the walk, which goes from the last
+ * token to the first where `reverse` is set.  Tensors begin on any element.  Limits as the scan's.  Outputs may not overlap inputs.
+ */
+int vig_causal_conv1d_fwd(const void* x, const float* weight, const float* bias, const void* initial_state, void* y, void* final_state, int B, int L, int D, int W,
+                          const long long* x_strides, int silu, int reverse, int io_dtype, void* stream);
+/* dy dense, d_final_state (NULL: zeros) -> dx dense, d_initial_state (NULL: not wanted; also without an initial_state), dw_db: D W + D floats, the gradients of weight and bias
+ * behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes. */
+size_t vig_causal_conv1d_bwd_workspace(int B, int L, int D, int W);
+int vig_causal_conv1d_bwd(const void* x, const float* weight, const float* bias, const void* initial_state, const void* dy, const void* d_final_state, void* dx, void* d_initial_state,
+                          float* dw_db, void* workspace, size_t workspace_bytes, int B, int L, int D, int W, const long long* x_strides, int silu, int reverse, int io_dtype,
+                          void* stream);
+/* One token of each sequence: state [B, W - 1, D] in place, x [B, D] with rows x_stride elements apart (0: packed), y packed.  state and y overlap nothing else. */
+int vig_causal_conv1d_step(const void* x, const float* weight, const float* bias, void* state, void* y, int B, int D, int W, long long x_stride, int silu, int io_dtype, void* stream);
+
+/*
+ * Residual add and layer norm over rows of C elements (up to 16384):
+ *
+ *   sum = x + residual, rounded to sum_dtype;   y = (sum - mean) / sqrt(var + eps) * weight + bias
+ *
+ * x, y [rows, C] of io_dtype, residual and sum of sum_dtype (io_dtype, or fp32 beside bf16 rows), both NULL for the norm of x alone; weight, bias (NULL: none) fp32 [C]; stats
+ * (NULL: not wanted): 2 * rows floats, mean and 1 / sqrt(var + eps) of each row, which the backward takes.  All dense.  Tensors begin on any element.  rows up to 2^24.
+ */
+int vig_add_layernorm_fwd(const void* x, const void* residual, const float* weight, const float* bias, void* sum, void* y, float* stats, long long rows, int C, float eps,
+                          int io_dtype, int sum_dtype, void* stream);
+/* sum: as the forward left it (without a residual: x).  dy, and d_sum (NULL: zeros), what else came to the sum -> the sum's gradient as d_residual of sum_dtype and dx of io_dtype (each
+ * may be NULL), dw_db: 2 C floats, the gradients of weight and bias behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes. */
+size_t vig_add_layernorm_bwd_workspace(long long rows, int C);
+int vig_add_layernorm_bwd(const void* sum, const float* stats, const float* weight, const void* dy, const void* d_sum, void* d_residual, void* dx, float* dw_db, void* workspace,
+                          size_t workspace_bytes, long long rows, int C, int io_dtype, int sum_dtype, void* stream);
+
+/*
  * One AdamW step over `count` tensors, in place:
  *
  *   g' = *grad_scale g;  m <- beta1 m + (1 - beta1) g';  v <- beta2 v + (1 - beta2) g'^2

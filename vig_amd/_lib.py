@@ -122,6 +122,19 @@ SIGNATURES = {
     "vig_gated_scan_bwd_workspace": (_c_size_t, [_c_int] * 4),
     "vig_gated_scan_bwd": (_c_int, [_c_void_p] * 11 + [_c_size_t] + [_c_int] * 3 + [_c_void_p] * 2 + [_c_float, _c_int, _c_int, _c_void_p]),
     "vig_gated_scan_step": (_c_int, [_c_void_p] * 4 + [_c_int] * 2 + [_c_longlong] * 2 + [_c_int] * 2 + [_c_void_p]),
+    "vig_selective_scan_fwd_workspace": (_c_size_t, [_c_int] * 5),
+    "vig_selective_scan_kept": (_c_size_t, [_c_int] * 4),
+    "vig_selective_scan_fwd": (_c_int, [_c_void_p] * 13 + [_c_size_t] + [_c_int] * 5 + [_c_void_p] * 5 + [_c_int] * 3 + [_c_void_p]),
+    "vig_selective_scan_bwd_workspace": (_c_size_t, [_c_int] * 5),
+    "vig_selective_scan_bwd": (_c_int, [_c_void_p] * 19 + [_c_size_t] + [_c_int] * 5 + [_c_void_p] * 5 + [_c_int] * 3 + [_c_void_p]),
+    "vig_selective_scan_step": (_c_int, [_c_void_p] * 10 + [_c_int] * 4 + [_c_longlong] * 2 + [_c_void_p] * 2 + [_c_longlong] + [_c_int] * 2 + [_c_void_p]),
+    "vig_causal_conv1d_fwd": (_c_int, [_c_void_p] * 6 + [_c_int] * 4 + [_c_void_p] + [_c_int] * 3 + [_c_void_p]),
+    "vig_causal_conv1d_bwd_workspace": (_c_size_t, [_c_int] * 4),
+    "vig_causal_conv1d_bwd": (_c_int, [_c_void_p] * 10 + [_c_size_t] + [_c_int] * 4 + [_c_void_p] + [_c_int] * 3 + [_c_void_p]),
+    "vig_causal_conv1d_step": (_c_int, [_c_void_p] * 5 + [_c_int] * 3 + [_c_longlong] + [_c_int] * 2 + [_c_void_p]),
+    "vig_add_layernorm_fwd": (_c_int, [_c_void_p] * 7 + [_c_longlong, _c_int, _c_float] + [_c_int] * 2 + [_c_void_p]),
+    "vig_add_layernorm_bwd_workspace": (_c_size_t, [_c_longlong, _c_int]),
+    "vig_add_layernorm_bwd": (_c_int, [_c_void_p] * 9 + [_c_size_t, _c_longlong] + [_c_int] * 3 + [_c_void_p]),
     "vig_adamw_many": (_c_int, [_c_void_p] * 10 + [_c_int] * 2 + [_c_double] * 5 + [_c_longlong] + [_c_void_p] * 3 + [ctypes.c_ulonglong, _c_void_p]),
     "vig_grad_norm_workspace": (_c_size_t, [_c_void_p, _c_int]),
     "vig_grad_norm": (_c_int, [_c_void_p] * 3 + [_c_int, _c_float] + [_c_void_p] * 3 + [_c_size_t, _c_void_p]),

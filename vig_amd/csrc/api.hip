@@ -1181,6 +1181,205 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
   return vig::launch_gated_scan_step({x, g, state, o, B, D, x_stride, g_stride, io_dtype, gate_dtype}, (hipStream_t)stream);
 }
 
+// A token's rows of `width` elements: strides of batch element and token (null: dense), positive and not beyond what a tile's offsets hold.
+static bool token_strides(const long long* given, int L, int width, long long& b, long long& l) {
+  b = given ? given[0] : (long long)L * width, l = given ? given[1] : width;
+  return b >= 0 && l >= width && l <= vig::kScanRow;
+}
+static bool selective_sizes_ok(int batch, int L, int D, int N, int G) {
+  return scan_sizes_ok(batch, L, D) && N > 0 && N <= vig::kScanStates && G > 0 && D % G == 0 && (long long)G * N <= vig::kScanRow;
+}
+// The arguments that the selective scan and its backward share, checked and put into `p`.
+static int selective_arguments(vig::SelScanArgs& p, const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z,
+                               const float* delta_bias, const float* initial_state, const long long* x_strides, const long long* delta_strides, const long long* B_strides,
+                               const long long* C_strides, const long long* z_strides, int batch, int L, int D, int N, int G, int delta_softplus, int reverse, int io_dtype) {
+  if (!x || !delta || !A || !B || !C || batch <= 0 || L <= 0 || D <= 0 || N <= 0 || G <= 0 || D % G) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !selective_sizes_ok(batch, L, D, N, G)) return VIG_ENOTSUP;
+  p = {};
+  p.x.at = x, p.delta.at = delta, p.z.at = z, p.B.at = B, p.C.at = C, p.A = A, p.skip = D_skip, p.bias = delta_bias, p.h0 = initial_state;
+  p.batch = batch, p.L = L, p.D = D, p.N = N, p.G = G, p.softplus = delta_softplus != 0, p.reverse = reverse != 0;
+  if (!token_strides(x_strides, L, D, p.x.b, p.x.l) || !token_strides(delta_strides, L, D, p.delta.b, p.delta.l) || !token_strides(z_strides, L, D, p.z.b, p.z.l) ||
+      !token_strides(B_strides, L, G * N, p.B.b, p.B.l) || !token_strides(C_strides, L, G * N, p.C.b, p.C.l))
+    return VIG_EINVAL;
+  p.B.g = B_strides ? B_strides[2] : N, p.C.g = C_strides ? C_strides[2] : N;
+  if (G > 1 && (p.B.g < N || p.C.g < N || (G - 1) * p.B.g + N > p.B.l || (G - 1) * p.C.g + N > p.C.l)) return VIG_EINVAL;
+  for (const void* t : {x, delta, B, C, z})
+    if (!on_element(t, element_size(io_dtype))) return VIG_EINVAL;
+  for (const float* t : {A, D_skip, delta_bias, initial_state})
+    if (!on_element(t, 4)) return VIG_EINVAL;
+  return VIG_OK;
+}
+
+size_t vig_selective_scan_fwd_workspace(int batch, int L, int D, int N, int G) { return selective_sizes_ok(batch, L, D, N, G) ? vig::selective_scan_workspace(batch, L, D, N, G) : 0; }
+size_t vig_selective_scan_kept(int batch, int L, int D, int N) { return selective_sizes_ok(batch, L, D, N, 1) ? vig::selective_scan_kept(batch, L, D, N) : 0; }
+size_t vig_selective_scan_bwd_workspace(int batch, int L, int D, int N, int G) {
+  return selective_sizes_ok(batch, L, D, N, G) ? vig::selective_scan_bwd_workspace(batch, L, D, N, G) : 0;
+}
+
+int vig_selective_scan_fwd(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias,
+                           const float* initial_state, void* o, float* final_state, float* kept, void* workspace, size_t workspace_bytes, int batch, int L, int D, int N, int G,
+                           const long long* x_strides, const long long* delta_strides, const long long* B_strides, const long long* C_strides, const long long* z_strides,
+                           int delta_softplus, int reverse, int io_dtype, void* stream) {
+  vig::SelScanArgs p;
+  const int rc = selective_arguments(p, x, delta, A, B, C, D_skip, z, delta_bias, initial_state, x_strides, delta_strides, B_strides, C_strides, z_strides, batch, L, D, N, G,
+                                     delta_softplus, reverse, io_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!o || !on_element(o, element_size(io_dtype)) || !on_element(final_state, 4) || !aligned16(kept, workspace)) return VIG_EINVAL;
+  for (const void* t : {x, delta, B, C, z})
+    if (o == t) return VIG_EINVAL;
+  if (final_state && final_state == initial_state) return VIG_EINVAL;
+  const size_t need = vig::selective_scan_workspace(batch, L, D, N, G);
+  if (need && (!workspace || workspace_bytes < need)) return VIG_ENOSPC;
+  p.o = o, p.hT = final_state, p.kept = kept;
+  return vig::launch_selective_scan(p, workspace, io_dtype, (hipStream_t)stream);
+}
+
+int vig_selective_scan_bwd(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias,
+                           const float* kept, const void* d_o, const float* d_final_state, void* dx, void* ddelta, void* dB, void* dC, void* dz, float* dA_dD_dbias,
+                           float* d_initial_state, void* workspace, size_t workspace_bytes, int batch, int L, int D, int N, int G, const long long* x_strides,
+                           const long long* delta_strides, const long long* B_strides, const long long* C_strides, const long long* z_strides, int delta_softplus, int reverse,
+                           int io_dtype, void* stream) {
+  vig::SelScanArgs p;
+  const int rc = selective_arguments(p, x, delta, A, B, C, D_skip, z, delta_bias, nullptr, x_strides, delta_strides, B_strides, C_strides, z_strides, batch, L, D, N, G,
+                                     delta_softplus, reverse, io_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!kept || !d_o || !dx || !ddelta || !dB || !dC || !dz != !z || !dA_dD_dbias || !aligned16(kept, workspace)) return VIG_EINVAL;
+  const void* const outs[] = {dx, ddelta, dB, dC, dz, dA_dD_dbias, d_initial_state};
+  for (int i = 0; i < 7; ++i) {
+    if (!outs[i]) continue;
+    if (!on_element(outs[i], i < 5 ? element_size(io_dtype) : 4)) return VIG_EINVAL;
+    for (const void* t : {x, delta, B, C, z, d_o, (const void*)kept, (const void*)d_final_state, (const void*)A, (const void*)D_skip, (const void*)delta_bias})
+      if (outs[i] == t) return VIG_EINVAL;
+    for (int k = 0; k < i; ++k)
+      if (outs[i] == outs[k]) return VIG_EINVAL;
+  }
+  if (!on_element(d_o, element_size(io_dtype)) || !on_element(d_final_state, 4)) return VIG_EINVAL;
+  if (!workspace || workspace_bytes < vig::selective_scan_bwd_workspace(batch, L, D, N, G)) return VIG_ENOSPC;
+  p.kept = const_cast<float*>(kept), p.d_o = {d_o, (long long)L * D, D, 0}, p.dhT = d_final_state;
+  p.dx = dx, p.ddelta = ddelta, p.dB = dB, p.dC = dC, p.dz = dz, p.dparams = dA_dD_dbias, p.dh0 = d_initial_state;
+  return vig::launch_selective_scan_bwd(p, workspace, io_dtype, (hipStream_t)stream);
+}
+
+int vig_selective_scan_step(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias, float* state,
+                            void* o, int batch, int D, int N, int G, long long x_stride, long long delta_stride, const long long* B_strides, const long long* C_strides,
+                            long long z_stride, int delta_softplus, int io_dtype, void* stream) {
+  if (!x || !delta || !A || !B || !C || !state || !o || batch <= 0 || D <= 0 || N <= 0 || G <= 0 || D % G) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !selective_sizes_ok(batch, 1, D, N, G)) return VIG_ENOTSUP;
+  vig::SelScanStep s{x, delta, z, B, C, A, D_skip, delta_bias, state, o, batch, D, N, G, x_stride ? x_stride : D, delta_stride ? delta_stride : D, z_stride ? z_stride : D,
+                     {B_strides ? B_strides[0] : (long long)G * N, B_strides ? B_strides[1] : N}, {C_strides ? C_strides[0] : (long long)G * N, C_strides ? C_strides[1] : N},
+                     delta_softplus, io_dtype};
+  if (s.x_stride < D || s.delta_stride < D || s.z_stride < D || s.B_strides[0] < 0 || s.C_strides[0] < 0 || (G > 1 && (s.B_strides[1] < N || s.C_strides[1] < N))) return VIG_EINVAL;
+  for (const void* t : {x, delta, B, C, z, (const void*)o})
+    if (!on_element(t, element_size(io_dtype))) return VIG_EINVAL;
+  for (const float* t : {A, D_skip, delta_bias, (const float*)state})
+    if (!on_element(t, 4)) return VIG_EINVAL;
+  for (const void* t : {x, delta, B, C, z, (const void*)state})
+    if (o == t) return VIG_EINVAL;
+  for (const void* t : {x, delta, B, C, z, (const void*)A, (const void*)D_skip, (const void*)delta_bias})
+    if (state == t) return VIG_EINVAL;
+  return vig::launch_selective_scan_step(s, (hipStream_t)stream);
+}
+
+static bool conv_sizes_ok(int B, int L, int D, int W) { return scan_sizes_ok(B, L, D) && W >= 2 && W <= 4; }
+static int conv_arguments(vig::CausalConv& p, const void* x, const float* weight, const float* bias, const void* initial_state, int B, int L, int D, int W, const long long* x_strides,
+                          int silu, int reverse, int io_dtype) {
+  if (!x || !weight || B <= 0 || L <= 0 || D <= 0 || W <= 0) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !conv_sizes_ok(B, L, D, W)) return VIG_ENOTSUP;
+  p = {};
+  p.x = x, p.weight = weight, p.bias = bias, p.initial = initial_state, p.B = B, p.L = L, p.D = D, p.W = W, p.silu = silu != 0, p.reverse = reverse != 0;
+  if (!token_strides(x_strides, L, D, p.xb, p.xl)) return VIG_EINVAL;
+  return on_element(x, element_size(io_dtype)) && on_element(initial_state, element_size(io_dtype)) && on_element(weight, 4) && on_element(bias, 4) ? VIG_OK : VIG_EINVAL;
+}
+
+int vig_causal_conv1d_fwd(const void* x, const float* weight, const float* bias, const void* initial_state, void* y, void* final_state, int B, int L, int D, int W,
+                          const long long* x_strides, int silu, int reverse, int io_dtype, void* stream) {
+  vig::CausalConv p;
+  const int rc = conv_arguments(p, x, weight, bias, initial_state, B, L, D, W, x_strides, silu, reverse, io_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!y || !on_element(y, element_size(io_dtype)) || !on_element(final_state, element_size(io_dtype))) return VIG_EINVAL;
+  if (y == x || y == initial_state || y == final_state || (final_state && (final_state == x || final_state == initial_state))) return VIG_EINVAL;
+  p.y = y, p.final = final_state;
+  return vig::launch_causal_conv(p, io_dtype, (hipStream_t)stream);
+}
+
+size_t vig_causal_conv1d_bwd_workspace(int B, int L, int D, int W) { return conv_sizes_ok(B, L, D, W) ? vig::causal_conv_bwd_workspace(B, L, D, W) : 0; }
+
+int vig_causal_conv1d_bwd(const void* x, const float* weight, const float* bias, const void* initial_state, const void* dy, const void* d_final_state, void* dx, void* d_initial_state,
+                          float* dw_db, void* workspace, size_t workspace_bytes, int B, int L, int D, int W, const long long* x_strides, int silu, int reverse, int io_dtype,
+                          void* stream) {
+  vig::CausalConv p;
+  const int rc = conv_arguments(p, x, weight, bias, initial_state, B, L, D, W, x_strides, silu, reverse, io_dtype);
+  if (rc != VIG_OK) return rc;
+  const int size = element_size(io_dtype);
+  if (!dy || !dx || !on_element(dy, size) || !on_element(d_final_state, size) || !on_element(dx, size) || !on_element(d_initial_state, size) || !on_element(dw_db, 4) ||
+      !aligned16(workspace))
+    return VIG_EINVAL;
+  for (const void* out : {(const void*)dx, (const void*)d_initial_state, (const void*)dw_db})
+    for (const void* t : {x, dy, initial_state, d_final_state, (const void*)weight, (const void*)bias})
+      if (out && out == t) return VIG_EINVAL;
+  if (dx == d_initial_state || dx == (void*)dw_db || (dw_db && d_initial_state == (void*)dw_db)) return VIG_EINVAL;
+  if (dw_db && (!workspace || workspace_bytes < vig::causal_conv_bwd_workspace(B, L, D, W))) return VIG_ENOSPC;
+  p.dy = dy, p.d_final = d_final_state, p.dx = dx, p.d_initial = d_initial_state, p.dparams = dw_db;
+  return vig::launch_causal_conv_bwd(p, workspace, io_dtype, (hipStream_t)stream);
+}
+
+int vig_causal_conv1d_step(const void* x, const float* weight, const float* bias, void* state, void* y, int B, int D, int W, long long x_stride, int silu, int io_dtype, void* stream) {
+  const long long strides[2] = {x_stride ? x_stride : D, x_stride && x_stride <= vig::kScanRow ? x_stride : D};
+  vig::CausalConv p;
+  const int rc = conv_arguments(p, x, weight, bias, nullptr, B, 1, D, W, strides, silu, 0, io_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!state || !y || !on_element(state, element_size(io_dtype)) || !on_element(y, element_size(io_dtype)) || strides[0] < D) return VIG_EINVAL;
+  if (y == x || y == state || state == x || state == (void*)weight || state == (void*)bias) return VIG_EINVAL;
+  p.y = y, p.final = state;
+  return vig::launch_causal_conv_step(p, io_dtype, (hipStream_t)stream);
+}
+
+static int norm_arguments(vig::AddNorm& p, long long rows, int C, float eps, int io_dtype, int sum_dtype) {
+  if (rows <= 0 || C <= 0 || !(eps >= 0.f)) return VIG_EINVAL;
+  if (!dtype_ok(io_dtype) || !dtype_ok(sum_dtype) || (io_dtype == VIG_F32 && sum_dtype != VIG_F32) || C > vig::kNormWidth || rows > (1LL << 24)) return VIG_ENOTSUP;
+  p = {};
+  p.rows = rows, p.C = C, p.eps = eps, p.io_dtype = io_dtype, p.sum_dtype = sum_dtype;
+  return VIG_OK;
+}
+
+int vig_add_layernorm_fwd(const void* x, const void* residual, const float* weight, const float* bias, void* sum, void* y, float* stats, long long rows, int C, float eps,
+                          int io_dtype, int sum_dtype, void* stream) {
+  vig::AddNorm p;
+  const int rc = norm_arguments(p, rows, C, eps, io_dtype, sum_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!x || !weight || !y || !residual != !sum || (!residual && sum_dtype != io_dtype)) return VIG_EINVAL;
+  if (!on_element(x, element_size(io_dtype)) || !on_element(y, element_size(io_dtype)) || !on_element(residual, element_size(sum_dtype)) || !on_element(sum, element_size(sum_dtype)) ||
+      !on_element(weight, 4) || !on_element(bias, 4) || !on_element(stats, 4))
+    return VIG_EINVAL;
+  for (const void* out : {(const void*)sum, (const void*)y, (const void*)stats})
+    for (const void* t : {x, residual, (const void*)weight, (const void*)bias})
+      if (out && out == t) return VIG_EINVAL;
+  if (sum == y || (stats && (stats == y || stats == sum))) return VIG_EINVAL;
+  p.x = x, p.residual = residual, p.weight = weight, p.bias = bias, p.sum = sum, p.y = y, p.stats = stats;
+  return vig::launch_add_norm(p, (hipStream_t)stream);
+}
+
+size_t vig_add_layernorm_bwd_workspace(long long rows, int C) { return rows > 0 && rows <= (1LL << 24) && C > 0 && C <= vig::kNormWidth ? vig::add_norm_bwd_workspace(rows, C) : 0; }
+
+int vig_add_layernorm_bwd(const void* sum, const float* stats, const float* weight, const void* dy, const void* d_sum, void* d_residual, void* dx, float* dw_db, void* workspace,
+                          size_t workspace_bytes, long long rows, int C, int io_dtype, int sum_dtype, void* stream) {
+  vig::AddNorm p;
+  const int rc = norm_arguments(p, rows, C, 0.f, io_dtype, sum_dtype);
+  if (rc != VIG_OK) return rc;
+  if (!sum || !stats || !weight || !dy || (!d_residual && !dx && !dw_db)) return VIG_EINVAL;
+  const int held = element_size(sum_dtype), io = element_size(io_dtype);
+  if (!on_element(sum, held) || !on_element(d_sum, held) || !on_element(d_residual, held) || !on_element(dy, io) || !on_element(dx, io) || !on_element(weight, 4) ||
+      !on_element(stats, 4) || !on_element(dw_db, 4) || !aligned16(workspace))
+    return VIG_EINVAL;
+  for (const void* out : {(const void*)d_residual, (const void*)dx, (const void*)dw_db})
+    for (const void* t : {sum, dy, d_sum, (const void*)stats, (const void*)weight})
+      if (out && out == t) return VIG_EINVAL;
+  if ((dx && (dx == d_residual || dx == (void*)dw_db)) || (d_residual && d_residual == (void*)dw_db)) return VIG_EINVAL;
+  if (dw_db && (!workspace || workspace_bytes < vig::add_norm_bwd_workspace(rows, C))) return VIG_ENOSPC;
+  p.held = sum, p.stats = const_cast<float*>(stats), p.weight = weight, p.dy = dy, p.d_sum = d_sum, p.d_residual = d_residual, p.dx = dx, p.dparams = dw_db;
+  return vig::launch_add_norm_bwd(p, workspace, (hipStream_t)stream);
+}
+
 int vig_adamw_many(void* const* param, const void* const* grad, void* const* exp_avg, void* const* exp_avg_sq, float* const* avg_scale,
                    float* const* sq_scale, const long long* n, const long long* first, const int* param_dtype, const int* grad_dtype, int count, int state_bits, double lr,
                    double beta1, double beta2, double eps, double weight_decay, long long step, const float* lr_on_device,

@@ -148,6 +148,74 @@ struct GatedScanStep {
 };
 int launch_gated_scan_step(const GatedScanStep& s, hipStream_t stream);
 
+// The selective state space scan (selective_scan.hip, selective_scan_bwd.hip; CN: a quarter of N states, as a power of two), its workspaces and what the forward keeps for the backward.
+struct Rows {  // a tensor whose rows of channels (or states) lie `l` elements apart, batch elements `b`, groups `g`
+  const void* at;
+  long long b, l, g;
+};
+
+struct SelScanArgs {
+  Rows x, delta, z, B, C, d_o;  // z.at may be null; d_o: backward
+  const float *A, *skip, *bias, *h0, *dhT;  // but for A they may be null
+  void *o, *dx, *ddelta, *dz, *dB, *dC;
+  float *hT, *dh0, *dparams;  // dparams: gradients of A [D, N], the skip's factors [D] and the bias [D]
+  float* kept;    // states that enter each tile of tokens, [B, tiles, D, 4 CN]
+  float* ends;    // chunks: what each leaves from nothing, later what enters it, [B, chunks, D, 4 CN]
+  float* sums;    // ... and the sum of its steps, [B, chunks, D]
+  float* shared;  // backward: gradients of B and C over a workgroup's channels, [B, G, blocks, L, 2, 4 CN]
+  float* params;  // ... those of dparams over a chunk's tokens, [B, chunks, D N + 2 D]
+  int batch, L, D, N, G, of_group, blocks, chunks, chunk;  // of_group: channels of a group, blocks: workgroups for them; chunk: tokens, whole tiles
+  bool softplus, reverse;
+};
+constexpr int kScanStates = 64;  // most of a channel
+size_t selective_scan_workspace(int batch, int L, int D, int N, int G);
+size_t selective_scan_kept(int batch, int L, int D, int N);
+size_t selective_scan_bwd_workspace(int batch, int L, int D, int N, int G);
+int launch_selective_scan(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream);
+int launch_selective_scan_bwd(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream);
+struct SelScanStep {
+  const void *x, *delta, *z, *B, *C;  // z may be null
+  const float *A, *skip, *bias;       // the last two may be null
+  float* state;
+  void* o;
+  int batch, D, N, G;
+  long long x_stride, delta_stride, z_stride, B_strides[2], C_strides[2];  // between batch elements; B, C: and between groups
+  int softplus, io_dtype;
+};
+int launch_selective_scan_step(const SelScanStep& s, hipStream_t stream);
+
+// The short causal convolution (causal_conv.hip)
+struct CausalConv {
+  const void *x, *initial, *dy, *d_final;  // states [B, W - 1, D]; all but x may be null
+  const float *weight, *bias;              // [D, W]; bias may be null
+  void *y, *final, *dx, *d_initial;        // dense; the step: final is the state
+  float *dparams, *parts;                  // gradients of the weight [D, W] and the bias [D]; may be null
+  long long xb, xl;                        // strides of x
+  int B, L, D, W;
+  bool silu, reverse;
+  int blocks, groups, run;                 // workgroups along a row, groups of runs along the tokens, tokens of a run
+};
+int launch_causal_conv(CausalConv& p, int io_dtype, hipStream_t stream);
+int launch_causal_conv_step(CausalConv& p, int io_dtype, hipStream_t stream);
+size_t causal_conv_bwd_workspace(int B, int L, int D, int W);
+int launch_causal_conv_bwd(CausalConv& p, void* workspace, int io_dtype, hipStream_t stream);
+
+// Residual add and layer norm (add_norm.hip)
+struct AddNorm {
+  const void *x, *residual, *held, *dy, *d_sum;  // held: the sum (or x), in the backward
+  const float *weight, *bias;
+  void *sum, *y, *dx, *d_residual;
+  float *stats, *dparams, *parts;                // stats: mean and rstd of each row; dparams: gradients of weight and bias [2, C]
+  long long rows, each;                          // each: rows of a workgroup
+  int C;
+  float eps;
+  int io_dtype, sum_dtype;
+};
+constexpr int kNormWidth = 16384;
+int launch_add_norm(const AddNorm& p, hipStream_t stream);
+size_t add_norm_bwd_workspace(long long rows, int C);
+int launch_add_norm_bwd(AddNorm& p, void* workspace, hipStream_t stream);
+
 // Norm of many gradients and AdamW over many tensors (update.hip).
 struct AdamW {
   void* const* param;

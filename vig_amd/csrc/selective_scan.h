@@ -1,0 +1,250 @@
+// The selective scan's pieces that its forward and its backward share (selective_scan.hip, selective_scan_bwd.hip).
+//
+// A wave takes sixteen channels: lane = 16 q + j holds the states n = q CN .. q CN + CN - 1 of channel j, so that a row of sixteen lanes reads a row of a
+// tensor.  Tokens come in tiles of T = 4 R: the lane loads, prepares (step, step times x, gate) and stores the tokens 4 m + q of its channel, m < R, each value once in the wave,
+// and passes them on to the other three lanes of the channel through LDS that no other wave touches.  What a lane sums over its own states of the
+// tokens 4 m .. 4 m + 3 is added up over q by swaps of lane rows that leave token 4 m + q with q (of_rows).
+#pragma once
+#include "common.h"
+#include "launch.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace vig {
+
+int launch_selective_join(const SelScanArgs& p, int np, bool back, hipStream_t stream);
+
+namespace {
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr unsigned kNowhere = 0x40000000u;  // byte offset behind every descriptor here: loads give 0, stores nothing
+constexpr int kScanWaves = 4;               // of a workgroup, on channels side by side
+constexpr int kScanBlock = 16 * kScanWaves; // channels of a workgroup
+constexpr int kScanGroups = 1024;           // workgroups that sequences are cut for
+
+// tokens of a tile (the backward keeps two numbers a state and token in registers: 128 of them at most)
+constexpr int scan_tile(int CN) { return CN <= 4 ? 16 : 64 / CN; }
+template <int CN> constexpr int kTileTokens = scan_tile(CN);
+// states of a lane: a quarter of N, as a power of two
+inline int scan_states(int N) {
+  int CN = 1;
+  while (4 * CN < N) CN *= 2;
+  return CN;
+}
+template <typename F> int by_states(int CN, F f) {
+  switch (CN) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 4: return f(std::integral_constant<int, 4>{});
+    case 8: return f(std::integral_constant<int, 8>{});
+    default: return f(std::integral_constant<int, 16>{});
+  }
+}
+// Chunks of tokens: none where the sequences and channels alone fill the chip.
+inline void cut_chunks(SelScanArgs& p) {
+  const int T = scan_tile(scan_states(p.N));
+  p.of_group = p.D / p.G, p.blocks = (p.of_group + kScanBlock - 1) / kScanBlock;
+  const long long groups = (long long)p.batch * p.G * p.blocks;
+  const long long want = std::max(1LL, std::min<long long>(kScanGroups / std::min<long long>(groups, kScanGroups), (p.L + T - 1) / T));
+  p.chunk = (int)(((p.L + want - 1) / want + T - 1) / T * T);
+  p.chunks = (p.L + p.chunk - 1) / p.chunk;
+}
+// whether every launch stays below 2^32 threads
+inline bool scan_fits(const SelScanArgs& p) {
+  const long long NP = 4 * scan_states(p.N), most = 0xffffffLL;
+  return (long long)p.batch * p.G * p.blocks * p.chunks <= most && (long long)p.batch * p.D * NP / 256 < most && (long long)p.batch * p.G * p.L / 128 * NP < most;
+}
+inline unsigned scan_grid(const SelScanArgs& p) { return (unsigned)((long long)p.batch * p.G * p.blocks * p.chunks); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float load1(rsrc_t r, unsigned off, float) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0)); }
+__device__ __forceinline__ float load1(rsrc_t r, unsigned off, uint16_t) { return bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0)); }
+__device__ __forceinline__ void store1(rsrc_t r, unsigned off, float v, float) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, off, 0, 0); }
+__device__ __forceinline__ void store1(rsrc_t r, unsigned off, float v, uint16_t) { __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(v), r, off, 0, 0); }
+
+// Where a wave stands.
+struct Stand {
+  int b, g, block, chunk;
+  int wave, q, j, c;  // c: channel
+  bool has;
+  int first, end;     // tokens of the chunk
+  __device__ __forceinline__ Stand(const SelScanArgs& p) {
+    // (workgroups go round the eight XCDs: each takes a stretch of neighbours, which share lines and the rows of B and C)
+    const unsigned each = gridDim.x / 8;
+    unsigned id = blockIdx.x;
+    if (id < 8 * each) id = id % 8 * each + id / 8;
+    block = (int)(id % (unsigned)p.blocks), id /= (unsigned)p.blocks;
+    g = (int)(id % (unsigned)p.G), id /= (unsigned)p.G;
+    chunk = (int)(id % (unsigned)p.chunks), b = (int)(id / (unsigned)p.chunks);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = (threadIdx.x >> 4) & 3, j = threadIdx.x & 15;
+    const int in = block * kScanBlock + wave * 16 + j;
+    has = in < p.of_group;
+    c = g * p.of_group + in;
+    first = chunk * p.chunk, end = min(first + p.chunk, p.L);
+  }
+};
+
+// Rows of a tile of T tokens from token `first` of the walk on: a descriptor and the lane's offsets in it.
+template <int T> struct Tile {
+  int first, end;
+  bool reverse;
+  long long row;  // of memory, where the tile begins
+  __device__ __forceinline__ Tile(const SelScanArgs& p, int first, int end) : first(first), end(end), reverse(p.reverse), row(p.reverse ? (long long)p.L - first - T : first) {}
+  // (may begin in front of the tensor, in rows that no lane reads)
+  template <typename S> __device__ __forceinline__ rsrc_t at(const void* base, long long before, long long pitch) const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(static_cast<const S*>(base)) + before + row * pitch, 0, (int)kNowhere, 0x00020000);
+  }
+  __device__ __forceinline__ unsigned in(int k) const { return (unsigned)(reverse ? T - 1 - k : k); }
+  __device__ __forceinline__ bool is(int k) const { return first + k < end; }
+};
+
+// log(1 + e), e in [0, 1], by the series of 2 atanh(e / (2 + e)): to 2 units of 2^-24 of itself, also where 1 + e would round e away
+__device__ __forceinline__ float log1p_01(float e) {
+  const float s = e * __builtin_amdgcn_rcpf(2.f + e), w = s * s;
+  float t = fmaf(w, 1.f / 13, 1.f / 11);
+  t = fmaf(w, t, 1.f / 9), t = fmaf(w, t, 1.f / 7), t = fmaf(w, t, 0.2f), t = fmaf(w, t, 1.f / 3);
+  return 2.f * fmaf(s * w, t, s);
+}
+// the step of a token from what its projection gives, and its derivative
+__device__ __forceinline__ float step_of(float raw, bool softplus) {
+  return softplus ? fmaxf(raw, 0.f) + log1p_01(exp_fast(-fabsf(raw))) : raw;
+}
+__device__ __forceinline__ float dstep_of(float raw, bool softplus) {
+  if (!softplus) return 1.f;
+  const float e = exp_fast(-fabsf(raw));
+  return (raw >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+}
+
+// sums over the four lane rows of four tokens' values: the row q is left with token q's
+__device__ __forceinline__ float of_rows(float s0, float s1, float s2, float s3) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(s0), __float_as_uint(s2), false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s1), __float_as_uint(s3), false, false);
+  const float even = __uint_as_float(a[0]) + __uint_as_float(a[1]), odd = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+  const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(even), __float_as_uint(odd), false, false);
+  return __uint_as_float(c[0]) + __uint_as_float(c[1]);
+}
+// the sum over the four lane rows, in all of them
+__device__ __forceinline__ float of_all_rows(float s) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+  s = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A wave's LDS: of a tile each channel's values along the tokens (K of them), each token's B and C.
+template <int CN, int K> struct Pass {
+  static constexpr int T = kTileTokens<CN>, kPitch = T + 4, NP = 4 * CN;
+  float of_channel[K][16][kPitch];
+  float of_token[2][T][NP];
+};
+// what other lanes of the wave wrote is read behind this
+__device__ __forceinline__ void passed() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+template <int N> __device__ __forceinline__ void read_lds(float (&v)[N], const float* from) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(from + i);
+      v[i] = w[0], v[i + 1] = w[1], v[i + 2] = w[2], v[i + 3] = w[3];
+    }
+  } else if constexpr (N == 2) {
+    const f32x2_t w = *reinterpret_cast<const f32x2_t*>(from);
+    v[0] = w[0], v[1] = w[1];
+  } else {
+    v[0] = *from;
+  }
+}
+
+// A lane's states in memory, [.., D, stride] with `stride` numbers a channel of which `n` are there
+template <int CN> __device__ __forceinline__ void load_states(float (&h)[CN], const float* base, size_t row, int D, int stride, int n, const Stand& at) {
+#pragma unroll
+  for (int i = 0; i < CN; ++i) h[i] = base && at.has && at.q * CN + i < n ? base[(row * D + at.c) * stride + at.q * CN + i] : 0.f;
+}
+template <int CN> __device__ __forceinline__ void store_states(float* base, const float (&h)[CN], size_t row, int D, int stride, int n, const Stand& at) {
+  if (!at.has) return;
+#pragma unroll
+  for (int i = 0; i < CN; ++i)
+    if (at.q * CN + i < n) base[(row * D + at.c) * stride + at.q * CN + i] = h[i];
+}
+// ... of rows of 4 CN numbers, all of them there, on 16-byte boundaries
+template <int CN> __device__ __forceinline__ void keep_states(float* base, const float (&h)[CN], size_t row, int D, const Stand& at) {
+  if (!at.has) return;
+  float* to = base + (row * D + at.c) * (4 * CN) + at.q * CN;
+  if constexpr (CN >= 4) {
+#pragma unroll
+    for (int i = 0; i < CN; i += 4) *reinterpret_cast<f32x4_t*>(to + i) = f32x4_t{h[i], h[i + 1], h[i + 2], h[i + 3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < CN; ++i) to[i] = h[i];
+  }
+}
+template <int CN> __device__ __forceinline__ void kept_states(float (&h)[CN], const float* base, size_t row, int D, const Stand& at) {
+  const float* from = base + (row * D + at.c) * (4 * CN) + at.q * CN;
+  if (!at.has) {
+#pragma unroll
+    for (int i = 0; i < CN; ++i) h[i] = 0.f;
+    return;
+  }
+  if constexpr (CN >= 4) {
+#pragma unroll
+    for (int i = 0; i < CN; i += 4) {
+      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(from + i);
+      h[i] = w[0], h[i + 1] = w[1], h[i + 2] = w[2], h[i + 3] = w[3];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CN; ++i) h[i] = from[i];
+  }
+}
+
+// Numbers of B or C of a tile as loaded: token 4 m + q, states j, j + 16, ...
+template <typename S, int CN> struct Shared {
+  static constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN, E = NP > 16 ? NP / 16 : 1;
+  float v[R][E];
+  __device__ __forceinline__ void load(const Rows& t, const SelScanArgs& p, const Tile<T>& tile, const Stand& at) {
+    const rsrc_t r = tile.template at<S>(t.at, at.b * t.b + at.g * t.g, t.l);
+    const unsigned pitch = (unsigned)t.l * sizeof(S);
+#pragma unroll
+    for (int m = 0; m < R; ++m)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int k = 4 * m + at.q, n = at.j + 16 * e;
+        v[m][e] = load1(r, tile.is(k) && n < p.N ? tile.in(k) * pitch + n * sizeof(S) : kNowhere, S{});
+      }
+  }
+  __device__ __forceinline__ void pass(float (&to)[T][NP], const Stand& at) const {
+#pragma unroll
+    for (int m = 0; m < R; ++m)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (NP >= 16 || at.j < NP) to[4 * m + at.q][at.j + 16 * e] = v[m][e];
+  }
+};
+// Values of a tile's rows of channels as loaded: token 4 m + q of channel j
+template <typename S, int T> struct Channels {
+  float v[T / 4];
+  __device__ __forceinline__ void load(const Rows& t, const Tile<T>& tile, const Stand& at) {
+    const rsrc_t r = tile.template at<S>(t.at, at.b * t.b, t.l);
+    const unsigned pitch = (unsigned)t.l * sizeof(S);
+#pragma unroll
+    for (int m = 0; m < T / 4; ++m) {
+      const int k = 4 * m + at.q;
+      v[m] = load1(r, tile.is(k) && at.has ? tile.in(k) * pitch + at.c * sizeof(S) : kNowhere, S{});
+    }
+  }
+};
+template <typename S, int T> __device__ __forceinline__ void store_rows(void* base, const float (&v)[T / 4], const SelScanArgs& p, const Tile<T>& tile, const Stand& at) {
+  const rsrc_t r = tile.template at<S>(base, (long long)at.b * p.L * p.D, p.D);
+  const unsigned pitch = (unsigned)p.D * sizeof(S);
+#pragma unroll
+  for (int m = 0; m < T / 4; ++m) {
+    const int k = 4 * m + at.q;
+    store1(r, tile.is(k) && at.has ? tile.in(k) * pitch + at.c * sizeof(S) : kNowhere, v[m], S{});
+  }
+}
+
+}  // namespace
+}  // namespace vig
