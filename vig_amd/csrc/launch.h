@@ -165,7 +165,7 @@ struct SelScanArgs {
   float* shared;  // backward: gradients of B and C over a workgroup's channels, [B, G, blocks, L, 2, 4 CN]
   float* params;  // ... those of dparams over a chunk's tokens, [B, chunks, D N + 2 D]
   int batch, L, D, N, G, of_group, blocks, chunks, chunk;  // of_group: channels of a group, blocks: workgroups for them; chunk: tokens, whole tiles
-  bool softplus, reverse;
+  int softplus, reverse;  // (not bool: a flag of one byte is compared into a lane mask, and what it selects ends up in vector registers)
 };
 constexpr int kScanStates = 64;  // most of a channel
 size_t selective_scan_workspace(int batch, int L, int D, int N, int G);
@@ -192,7 +192,7 @@ struct CausalConv {
   float *dparams, *parts;                  // gradients of the weight [D, W] and the bias [D]; may be null
   long long xb, xl;                        // strides of x
   int B, L, D, W;
-  bool silu, reverse;
+  int silu, reverse;
   int blocks, groups, run;                 // workgroups along a row, groups of runs along the tokens, tokens of a run
 };
 int launch_causal_conv(CausalConv& p, int io_dtype, hipStream_t stream);

@@ -18,7 +18,7 @@ int launch_selective_join(const SelScanArgs& p, int np, bool back, hipStream_t s
 namespace {
 
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
-constexpr unsigned kNowhere = 0x40000000u;  // byte offset behind every descriptor here: loads give 0, stores nothing
+constexpr unsigned kNowhere = 0x40000000u;  // byte offset behind every descriptor here (sixteen rows of kScanRow elements at most)
 constexpr int kScanWaves = 4;               // of a workgroup, on channels side by side
 constexpr int kScanBlock = 16 * kScanWaves; // channels of a workgroup
 constexpr int kScanGroups = 1024;           // workgroups that sequences are cut for
@@ -85,18 +85,34 @@ struct Stand {
   }
 };
 
-// Rows of a tile of T tokens from token `first` of the walk on: a descriptor and the lane's offsets in it.
+// A tile of tokens from token `first` of the walk on, as many of them as lie in front of `end` (one at least).  A tensor's descriptor begins at the lowest of their rows in memory and ends
+// behind the highest, so that lanes without a token, whose offsets lie outside, read zeros and store nothing.
 template <int T> struct Tile {
-  int first, end;
-  bool reverse;
-  long long row;  // of memory, where the tile begins
-  __device__ __forceinline__ Tile(const SelScanArgs& p, int first, int end) : first(first), end(end), reverse(p.reverse), row(p.reverse ? (long long)p.L - first - T : first) {}
-  // (may begin in front of the tensor, in rows that no lane reads)
-  template <typename S> __device__ __forceinline__ rsrc_t at(const void* base, long long before, long long pitch) const {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<S*>(static_cast<const S*>(base)) + before + row * pitch, 0, (int)kNowhere, 0x00020000);
+  int rows, from, step;  // the row of memory of token k lies from + step k rows behind the lowest
+  long long lowest;
+  __device__ __forceinline__ Tile(const SelScanArgs& p, int first, int end) {
+    rows = min(end - first, T);
+    lowest = p.reverse ? (long long)p.L - first - rows : first;
+    from = p.reverse ? rows - 1 : 0, step = p.reverse ? -1 : 1;
   }
-  __device__ __forceinline__ unsigned in(int k) const { return (unsigned)(reverse ? T - 1 - k : k); }
-  __device__ __forceinline__ bool is(int k) const { return first + k < end; }
+};
+// A tensor's rows as a lane reads or writes them, one element each
+template <typename S> struct Line {
+  const char* at;
+  unsigned pitch, offset;  // bytes; offset: the lane's, from its row of lanes' first token
+  // column: the lane's element of a row, or none
+  __device__ __forceinline__ void stand(const SelScanArgs& p, const void* base, long long before, long long l, int q, int column, bool has) {
+    at = static_cast<const char*>(base) + before * (long long)sizeof(S);
+    pitch = (unsigned)l * sizeof(S);
+    offset = has ? column * sizeof(S) + (p.reverse ? 0u - q * pitch : q * pitch) : kNowhere;
+  }
+  template <int T> __device__ __forceinline__ rsrc_t of(const Tile<T>& t) const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at) + t.lowest * pitch, 0, (int)(t.rows * pitch), 0x00020000);
+  }
+  // token 4 m + q of the tile
+  template <int T> __device__ __forceinline__ unsigned place(const Tile<T>& t, int m) const { return offset + (unsigned)(t.from + t.step * 4 * m) * pitch; }
+  template <int T> __device__ __forceinline__ float load(rsrc_t r, const Tile<T>& t, int m) const { return load1(r, place(t, m), S{}); }
+  template <int T> __device__ __forceinline__ void store(const Tile<T>& t, int m, float v) const { store1(of(t), place(t, m), v, S{}); }
 };
 
 // log(1 + e), e in [0, 1], by the series of 2 atanh(e / (2 + e)): to 2 units of 2^-24 of itself, also where 1 + e would round e away
@@ -107,13 +123,15 @@ __device__ __forceinline__ float log1p_01(float e) {
   return 2.f * fmaf(s * w, t, s);
 }
 // the step of a token from what its projection gives, and its derivative
-__device__ __forceinline__ float step_of(float raw, bool softplus) {
-  return softplus ? fmaxf(raw, 0.f) + log1p_01(exp_fast(-fabsf(raw))) : raw;
+__device__ __forceinline__ float step_of(float raw, int softplus) {
+  const float soft = fmaxf(raw, 0.f) + log1p_01(exp_fast(-fabsf(raw)));
+  return softplus ? soft : raw;
 }
-__device__ __forceinline__ float dstep_of(float raw, bool softplus) {
+__device__ __forceinline__ float dstep_of(float raw, int softplus) {
   if (!softplus) return 1.f;
   const float e = exp_fast(-fabsf(raw));
-  return (raw >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+  const float soft = (raw >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+  return softplus ? soft : 1.f;
 }
 
 // sums over the four lane rows of four tokens' values: the row q is left with token q's
@@ -203,17 +221,18 @@ template <int CN> __device__ __forceinline__ void kept_states(float (&h)[CN], co
 // Numbers of B or C of a tile as loaded: token 4 m + q, states j, j + 16, ...
 template <typename S, int CN> struct Shared {
   static constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN, E = NP > 16 ? NP / 16 : 1;
+  Line<S> line[E];
   float v[R][E];
-  __device__ __forceinline__ void load(const Rows& t, const SelScanArgs& p, const Tile<T>& tile, const Stand& at) {
-    const rsrc_t r = tile.template at<S>(t.at, at.b * t.b + at.g * t.g, t.l);
-    const unsigned pitch = (unsigned)t.l * sizeof(S);
+  __device__ __forceinline__ void stand(const SelScanArgs& p, const Rows& t, const Stand& at) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) line[e].stand(p, t.at, at.b * t.b + at.g * t.g, t.l, at.q, at.j + 16 * e, at.j + 16 * e < p.N);
+  }
+  __device__ __forceinline__ void load(const Tile<T>& t) {
+    const rsrc_t r = line[0].of(t);
 #pragma unroll
     for (int m = 0; m < R; ++m)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int k = 4 * m + at.q, n = at.j + 16 * e;
-        v[m][e] = load1(r, tile.is(k) && n < p.N ? tile.in(k) * pitch + n * sizeof(S) : kNowhere, S{});
-      }
+      for (int e = 0; e < E; ++e) v[m][e] = line[e].load(r, t, m);
   }
   __device__ __forceinline__ void pass(float (&to)[T][NP], const Stand& at) const {
 #pragma unroll
@@ -225,25 +244,20 @@ template <typename S, int CN> struct Shared {
 };
 // Values of a tile's rows of channels as loaded: token 4 m + q of channel j
 template <typename S, int T> struct Channels {
+  Line<S> line;
   float v[T / 4];
-  __device__ __forceinline__ void load(const Rows& t, const Tile<T>& tile, const Stand& at) {
-    const rsrc_t r = tile.template at<S>(t.at, at.b * t.b, t.l);
-    const unsigned pitch = (unsigned)t.l * sizeof(S);
+  __device__ __forceinline__ void stand(const SelScanArgs& p, const Rows& t, const Stand& at) { line.stand(p, t.at, at.b * t.b, t.l, at.q, at.c, at.has); }
+  __device__ __forceinline__ void load(const Tile<T>& t) {
+    const rsrc_t r = line.of(t);
 #pragma unroll
-    for (int m = 0; m < T / 4; ++m) {
-      const int k = 4 * m + at.q;
-      v[m] = load1(r, tile.is(k) && at.has ? tile.in(k) * pitch + at.c * sizeof(S) : kNowhere, S{});
-    }
+    for (int m = 0; m < T / 4; ++m) v[m] = line.load(r, t, m);
   }
 };
-template <typename S, int T> __device__ __forceinline__ void store_rows(void* base, const float (&v)[T / 4], const SelScanArgs& p, const Tile<T>& tile, const Stand& at) {
-  const rsrc_t r = tile.template at<S>(base, (long long)at.b * p.L * p.D, p.D);
-  const unsigned pitch = (unsigned)p.D * sizeof(S);
-#pragma unroll
-  for (int m = 0; m < T / 4; ++m) {
-    const int k = 4 * m + at.q;
-    store1(r, tile.is(k) && at.has ? tile.in(k) * pitch + at.c * sizeof(S) : kNowhere, v[m], S{});
-  }
+// a dense tensor's
+template <typename S> __device__ __forceinline__ Line<S> dense_line(const SelScanArgs& p, void* base, const Stand& at) {
+  Line<S> line;
+  line.stand(p, base, (long long)at.b * p.L * p.D, p.D, at.q, at.c, at.has);
+  return line;
 }
 
 }  // namespace

@@ -36,12 +36,14 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
   float sum = 0.f;
   Channels<S, T> x, delta, z;
   Shared<S, CN> B, C;
+  x.stand(p, p.x, at), delta.stand(p, p.delta, at), B.stand(p, p.B, at);
+  if constexpr (!FOLD) C.stand(p, p.C, at), z.stand(p, p.z, at);
+  const Line<S> out = dense_line<S>(p, p.o, at);
   auto load = [&](int first) {
     const Tile<T> tile(p, first, at.end);
-    x.load(p.x, tile, at), delta.load(p.delta, tile, at);
-    B.load(p.B, p, tile, at);
-    if constexpr (!FOLD) C.load(p.C, p, tile, at);
-    if (gated) z.load(p.z, tile, at);
+    x.load(tile), delta.load(tile), B.load(tile);
+    if constexpr (!FOLD) C.load(tile);
+    if (gated) z.load(tile);
   };
   load(at.first);
   for (int first = at.first; first < at.end; first += T) {
@@ -49,7 +51,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     float xs[R], zs[R];
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const float step = tile.is(4 * m + at.q) ? step_of(delta.v[m] + bias, p.softplus) : 0.f;
+      const float step = first + 4 * m + at.q < at.end ? step_of(delta.v[m] + bias, p.softplus) : 0.f;
       xs[m] = x.v[m], zs[m] = z.v[m];
       pass.of_channel[0][at.j][4 * m + at.q] = step;
       pass.of_channel[1][at.j][4 * m + at.q] = step * x.v[m];
@@ -61,7 +63,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     if (first + T < at.end) load(first + T);
     if constexpr (!FOLD)
       if (p.kept) keep_states(p.kept, h, (size_t)at.b * ((p.L + T - 1) / T) + first / T, p.D, at);
-    float y[R];
 #pragma unroll
     for (int m = 0; m < R; ++m) {
       float step[4], u[4], s[4];
@@ -80,12 +81,12 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
         }
       }
       if constexpr (!FOLD) {
-        y[m] = fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3]));
-        if (gated) y[m] *= zs[m] * sigmoidf_(zs[m]);
+        float y = fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3]));
+        if (gated) y *= zs[m] * sigmoidf_(zs[m]);
+        out.store(tile, m, y);
       }
     }
     passed();
-    if constexpr (!FOLD) store_rows<S>(p.o, y, p, tile, at);
   }
   if constexpr (FOLD) {
     keep_states(p.ends, h, row, p.D, at);

@@ -60,34 +60,36 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   float sum = 0.f, dskip = 0.f, dbias = 0.f, dA[CN];
 #pragma unroll
   for (int i = 0; i < CN; ++i) dA[i] = 0.f;
+  [[maybe_unused]] const Line<S> dx = dense_line<S>(p, p.dx, at), ddelta = dense_line<S>(p, p.ddelta, at), dz = dense_line<S>(p, p.dz, at);
   const int tiles = (p.L + T - 1) / T, last = at.first + (at.end - 1 - at.first) / T * T;
   Channels<S, T> x, delta, z, d_o;
   Shared<S, CN> B, C;
+  delta.stand(p, p.delta, at), d_o.stand(p, p.d_o, at), C.stand(p, p.C, at), z.stand(p, p.z, at);
+  if constexpr (!FOLD) x.stand(p, p.x, at), B.stand(p, p.B, at);
   auto load = [&](int first) {
     const Tile<T> tile(p, first, at.end);
-    delta.load(p.delta, tile, at), d_o.load(p.d_o, tile, at), C.load(p.C, p, tile, at);
-    if (gated) z.load(p.z, tile, at);
-    if constexpr (!FOLD) x.load(p.x, tile, at), B.load(p.B, p, tile, at);
+    delta.load(tile), d_o.load(tile), C.load(tile);
+    if (gated) z.load(tile);
+    if constexpr (!FOLD) x.load(tile), B.load(tile);
   };
   load(last);
   for (int first = last, turn = 0; first >= at.first; first -= T, turn ^= 1) {
-    const Tile<T> tile(p, first, at.end);
-    float raw[R], xs[R], steps[R], dy[R], by_y[R];  // by_y: what makes dz of y
+    [[maybe_unused]] const Tile<T> tile(p, first, at.end);
+    float raw[R], xs[R], by_y[R];  // by_y: what makes dz of y
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const bool is = tile.is(4 * m + at.q);
       raw[m] = delta.v[m] + bias, xs[m] = x.v[m];
-      steps[m] = is ? step_of(raw[m], p.softplus) : 0.f;
-      dy[m] = d_o.v[m];
+      const float step = first + 4 * m + at.q < at.end ? step_of(raw[m], p.softplus) : 0.f;
+      float dy = d_o.v[m];
       if (gated) {
         const float s = sigmoidf_(z.v[m]), g = z.v[m] * s;
-        by_y[m] = dy[m] * fmaf(g, 1.f - s, s);
-        dy[m] *= g;
+        by_y[m] = dy * fmaf(g, 1.f - s, s);
+        dy *= g;
       }
-      pass.of_channel[0][at.j][4 * m + at.q] = steps[m];
-      pass.of_channel[1][at.j][4 * m + at.q] = dy[m];
-      if constexpr (FOLD) sum += steps[m];
-      else pass.of_channel[2][at.j][4 * m + at.q] = steps[m] * xs[m];
+      pass.of_channel[0][at.j][4 * m + at.q] = step;
+      pass.of_channel[1][at.j][4 * m + at.q] = dy;
+      if constexpr (FOLD) sum += step;
+      else pass.of_channel[2][at.j][4 * m + at.q] = step * xs[m];
     }
     if constexpr (!FOLD) B.pass(pass.of_token[0], at);
     C.pass(pass.of_token[1], at);
@@ -120,11 +122,11 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
       };
       float h[CN], a[T][CN], ph[T][CN];
       kept_states(h, p.kept, (size_t)at.b * tiles + first / T, p.D, at);
-      if (first > at.first) load(first - T);
       // forward again
       float few[8];
 #pragma unroll
       for (int m = 0; m < R; ++m) {
+        __builtin_amdgcn_sched_barrier(0);
         float step[4], d[4], u[4], s[4];
         read_lds(step, &pass.of_channel[0][at.j][4 * m]);
         read_lds(d, &pass.of_channel[1][at.j][4 * m]);
@@ -132,6 +134,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int t = 4 * m + k;
+          if constexpr (CN >= 8) __builtin_amdgcn_sched_barrier(0);
           float b[CN], c[CN];
           read_lds(b, &pass.of_token[0][t][at.q * CN]);
           read_lds(c, &pass.of_token[1][t][at.q * CN]);
@@ -146,12 +149,12 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
             if (t % TT == TT - 1 && i % 8 == NN - 1) shared(few, 1, t - (TT - 1), i - (NN - 1));
           }
         }
-        if (gated) by_y[m] *= fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3]));
+        if (gated) dz.store(tile, m, by_y[m] * fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3])));
       }
       // and back
-      float ds[R], dx[R];
 #pragma unroll
       for (int m = R - 1; m >= 0; --m) {
+        __builtin_amdgcn_sched_barrier(0);
         float step[4], d[4], u[4], du[4], dd[4];
         read_lds(step, &pass.of_channel[0][at.j][4 * m]);
         read_lds(d, &pass.of_channel[1][at.j][4 * m]);
@@ -159,6 +162,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
 #pragma unroll
         for (int k = 3; k >= 0; --k) {
           const int t = 4 * m + k;
+          if constexpr (CN >= 8) __builtin_amdgcn_sched_barrier(0);
           float b[CN], c[CN];
           read_lds(b, &pass.of_token[0][t][at.q * CN]);
           read_lds(c, &pass.of_token[1][t][at.q * CN]);
@@ -175,23 +179,24 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
           }
         }
         const float du_m = of_rows(du[0], du[1], du[2], du[3]), dd_m = of_rows(dd[0], dd[1], dd[2], dd[3]);
-        dx[m] = fmaf(steps[m], du_m, skip * dy[m]);
-        ds[m] = fmaf(xs[m], du_m, dd_m * kLn2) * dstep_of(raw[m], p.softplus);
-        if (tile.is(4 * m + at.q)) dbias += ds[m], dskip = fmaf(dy[m], xs[m], dskip);
+        const float dy = pass.of_channel[1][at.j][4 * m + at.q];
+        const float ds = fmaf(xs[m], du_m, dd_m * kLn2) * dstep_of(raw[m], p.softplus);
+        dx.store(tile, m, fmaf(pass.of_channel[0][at.j][4 * m + at.q], du_m, skip * dy));
+        ddelta.store(tile, m, ds);
+        if (first + 4 * m + at.q < at.end) dbias += ds, dskip = fmaf(dy, xs[m], dskip);
+        // (the next tile's rows, into registers that the last tokens' factors have left)
+        if (m == R - 1 && first > at.first) load(first - T);
       }
-      store_rows<S>(p.dx, dx, p, tile, at);
-      store_rows<S>(p.ddelta, ds, p, tile, at);
-      if (gated) store_rows<S>(p.dz, by_y, p, tile, at);
       // the workgroup's sums (the other turn's are read until the next barrier)
       __syncthreads();
       const size_t rows = (((size_t)at.b * p.G + at.g) * p.blocks + at.block) * p.L;
       for (int e = threadIdx.x; e < 2 * T * NP; e += 64 * kScanWaves) {
-        const int n = e % NP, which = e / NP % 2, t = e / (2 * NP);
-        if (!tile.is(t)) break;
+        const int n = e % NP, which = e / NP % 2, t = first + e / (2 * NP);
+        if (t >= at.end) break;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kScanWaves; ++w) s += boards[turn][w].v[which][t][n];
-        p.shared[((rows + tile.row + tile.in(t)) * 2 + which) * NP + n] = s;
+        for (int w = 0; w < kScanWaves; ++w) s += boards[turn][w].v[which][t - first][n];
+        p.shared[((rows + (p.reverse ? p.L - 1 - t : t)) * 2 + which) * NP + n] = s;
       }
     }
   }
