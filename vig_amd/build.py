@@ -79,10 +79,10 @@ def _host_library(srcs: list[str], out: str, extra_libs: list[str], verbose: boo
 def build_torch_extension(verbose: bool = True) -> str:
     """Builds vig_amd/lib/libvig_torch_ext.so, the PyTorch-ROCm operator library over the C ABI (csrc/torch_ext.cpp), and
     vig_amd/lib/vig_host.so, the op-level calls and the recorded block as a CPython module
-    (csrc/py_calls.cpp, csrc/train_block.cpp)."""
+    (csrc/py_calls.cpp and the sources beside it)."""
     with ThreadPoolExecutor(max_workers=2) as ex:
         jobs = [ex.submit(_host_library, ["torch_ext.cpp"], EXT, [], verbose),
-                ex.submit(_host_library, ["py_calls.cpp", "train_block.cpp", "model_forward.cpp", "scan_calls.cpp"], CALLS, ["-ltorch_python"], verbose)]
+                ex.submit(_host_library, ["py_calls.cpp", "train_block.cpp", "model_forward.cpp", "scan_calls.cpp", "selective_calls.cpp"], CALLS, ["-ltorch_python"], verbose)]
         for j in jobs:
             j.result()
     return EXT

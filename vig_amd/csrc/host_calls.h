@@ -5,6 +5,7 @@
 #include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -88,6 +89,39 @@ inline int run_forward(const Tensor& q, const Tensor& k, const Tensor& v, const 
             c.B, c.H, c.L, c.Dk, c.Dv, c.scale, c.out_scale, c.io, c.gd, stream_of(q));
 }
 
+// [B, L, D] (or [B, D]) whose channels lie side by side in rows that do not overlap; anything else is copied.
+inline Tensor rows(const Tensor& t) {
+  const int64_t d = t.dim(), pitch = t.stride(d - 2);
+  const bool side = t.size(d - 1) == 1 || t.stride(d - 1) == 1;
+  return side && (t.size(d - 2) == 1 || (pitch >= t.size(d - 1) && pitch <= (1 << 18))) ? t : t.contiguous();
+}
+// (batch, token) strides; a row alone is as far from the next as it is wide
+struct Strides {
+  long long v[2];
+  explicit Strides(const Tensor& t) : v{t.size(0) == 1 ? 0 : (long long)t.stride(0), t.size(1) == 1 ? (long long)t.size(2) : (long long)t.stride(1)} {}
+};
+inline bool simple(const Tensor& t) { return t.defined() && t.is_cuda() && !t.unsafeGetTensorImpl()->is_python_dispatch() && t.layout() == at::kStrided; }
+
+
+// a tensor of forward-mode differentiation, whose tangent a launch would drop
+inline bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline bool records(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// A leaf's gradient is added up on the stream of the graph that first used it, as long as one lives.  Where that is the default stream a captured backward pass would
+// wait there, which breaks the capture in a destructor and ends the process: refused before anything is recorded.
+inline void refuse_held_leaf(const Tensor& t) {
+  if (!records(t) || !t.is_leaf()) return;
+  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!held || !held->stream()) return;
+  TORCH_CHECK(held->stream()->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
+              "a graph recorded on the default stream still holds a leaf that is captured here; drop that graph (its outputs) or detach the leaf first");
+}
+
+// What was written behind autograd's back: tensors saved for a backward pass notice.
+inline void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 inline Tensor tensor_arg(PyObject* o) {
   if (o == Py_None) return Tensor();
   return THPVariable_Check(o) ? THPVariable_Unpack(o) : Tensor();
@@ -106,6 +140,13 @@ PyObject* refuse_held_leaves(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* gated_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* adamw(PyObject*, PyObject* const* a, Py_ssize_t n);
 PyObject* grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n);
+
+// the methods of selective_calls.cpp
+PyObject* selective_scan(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* selective_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* causal_conv1d(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* causal_conv1d_step(PyObject*, PyObject* const* a, Py_ssize_t n);
+PyObject* add_layernorm(PyObject*, PyObject* const* a, Py_ssize_t n);
 
 // the methods of model_forward.cpp
 PyObject* make_plan(PyObject*, PyObject* const* a, Py_ssize_t n);

@@ -170,6 +170,11 @@ PyMethodDef kMethods[] = {
     {"gated_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_scan_step)), METH_FASTCALL, nullptr},
     {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adamw)), METH_FASTCALL, nullptr},
     {"grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(grad_norm)), METH_FASTCALL, nullptr},
+    {"selective_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(selective_scan)), METH_FASTCALL, nullptr},
+    {"selective_scan_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(selective_scan_step)), METH_FASTCALL, nullptr},
+    {"causal_conv1d", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(causal_conv1d)), METH_FASTCALL, nullptr},
+    {"causal_conv1d_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(causal_conv1d_step)), METH_FASTCALL, nullptr},
+    {"add_layernorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_layernorm)), METH_FASTCALL, nullptr},
     {"make_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(make_plan)), METH_FASTCALL, nullptr},
     {"plan_describes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(plan_describes)), METH_FASTCALL, nullptr},
     {"run_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(run_plan)), METH_FASTCALL, nullptr},

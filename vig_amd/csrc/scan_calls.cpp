@@ -4,7 +4,6 @@
 // are 720 addresses, sizes and types, which Python reads in 0.4 ms, twice what the kernels take.
 #include "host_calls.h"
 
-#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <deque>
@@ -13,22 +12,9 @@
 namespace vig_host {
 namespace {
 
-// [B, L, D] (or [B, D]) whose channels lie side by side in rows that do not overlap; anything else is copied.
-Tensor rows(const Tensor& t) {
-  const int64_t d = t.dim(), pitch = t.stride(d - 2);
-  const bool side = t.size(d - 1) == 1 || t.stride(d - 1) == 1;
-  return side && (t.size(d - 2) == 1 || (pitch >= t.size(d - 1) && pitch <= (1 << 18))) ? t : t.contiguous();
-}
-// (batch, token) strides; a row alone is as far from the next as it is wide
-struct Strides {
-  long long v[2];
-  explicit Strides(const Tensor& t) : v{t.size(0) == 1 ? 0 : (long long)t.stride(0), t.size(1) == 1 ? (long long)t.size(2) : (long long)t.stride(1)} {}
-};
 const void* second(const Tensor& g, bool both) {
   return both ? static_cast<const char*>(g.data_ptr()) + g.size(0) / 2 * g.stride(0) * g.element_size() : nullptr;
 }
-
-bool simple(const Tensor& t) { return t.defined() && t.is_cuda() && !t.unsafeGetTensorImpl()->is_python_dispatch() && t.layout() == at::kStrided; }
 
 // What vig_gated_scan_fwd and _bwd take; everything else is ops.py's to word.
 bool scan_call(const Tensor& x, const Tensor& g, const Tensor& h0, bool both) {
@@ -104,25 +90,6 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     return {dx, dg, dh0, Tensor(), Tensor(), Tensor()};
   }
 };
-
-// a tensor of forward-mode differentiation, whose tangent a launch would drop
-bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
-bool records(const Tensor& t) { return t.defined() && t.requires_grad(); }
-
-// A leaf's gradient is added up on the stream of the graph that first used it, as long as one lives.  Where that is the default stream a captured backward pass would
-// wait there, which breaks the capture in a destructor and ends the process: refused before anything is recorded.
-void refuse_held_leaf(const Tensor& t) {
-  if (!records(t) || !t.is_leaf()) return;
-  const auto held = torch::autograd::impl::try_get_grad_accumulator(t);
-  if (!held || !held->stream()) return;
-  TORCH_CHECK(held->stream()->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
-              "gated_scan: a graph recorded on the default stream still holds a leaf that is captured here; drop that graph (its outputs) or detach the leaf first");
-}
-
-// What was written behind autograd's back: tensors saved for a backward pass notice.
-void written(const Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
 
 }  // namespace
 

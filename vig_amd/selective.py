@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib, ops
+from . import _ext, _lib, ops
 from .ops import _dt, _operator, _refuse_held_leaves, _refuse_tangents, _scan_rows, _scan_strides
 
 MOST_STATES = 64  # of a channel
@@ -62,6 +62,11 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     finite stays in its sequence's channel, where every later output is not finite then, and in gradients of the rows that channels share.
     x, delta, z, B, C may be columns of wider rows (read in place).  Up to 2^24 tokens of 2^18 channels.  States and sums are held in fp32, in an order fixed by the sizes.
     Differentiable in every tensor; the forward then keeps the state in front of every 16th token (8th above 16, 4th above 32 states), 4 bytes a channel and token at 16 states."""
+    calls = _ext.calls()
+    if calls is not None:  # one native call for what the kernels take; None: not of that kind
+        r = calls.selective_scan(x, delta, A, B, C, D, z, delta_bias, initial_state, delta_softplus, reverse, output_final_state)
+        if r is not None:
+            return r if output_final_state else (r, None)
     ops._check_cuda(x, delta, A, B, C, D, z, delta_bias, initial_state)
     if x.dim() != 3 or delta.shape != x.shape or (z is not None and z.shape != x.shape):
         raise ValueError("x, delta and z must be [B,L,D] of the same sizes")
@@ -202,6 +207,11 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
                         z: Optional[torch.Tensor] = None, delta_bias: Optional[torch.Tensor] = None, delta_softplus: bool = False) -> torch.Tensor:
     """selective_scan for one token of every sequence: x, delta, z [B,D], B and C [B,N] or [B,G,N]; state (fp32 [B,D,N], contiguous, apart from the others' memory) is moved on
     in place, the output returned in x's dtype.  Inference only."""
+    calls = _ext.calls()
+    if calls is not None:
+        o = calls.selective_scan_step(x, delta, A, B, C, D, z, delta_bias, state, delta_softplus)
+        if o is not None:
+            return o
     ops._check_cuda(x, delta, A, B, C, state, D, z, delta_bias)
     given = (x, delta, A, B, C, state, D, z, delta_bias)
     if _needs_graph(*given):
@@ -255,6 +265,11 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     x: [B,L,D] in fp32 or bf16, or columns of wider rows (read in place); weight [D,W] (or [D,1,W], as torch.nn.Conv1d has it), W 2, 3 or 4; bias [D].  initial_state: the W - 1 rows in
     front of the first token, [B,W-1,D] of x's dtype (zeros without it); final_state: the last W - 1 rows, for what follows.  reverse: the walk goes from the last token to the first, and the
     states' rows with it.  Sums are held in fp32, in an order fixed by the sizes and by how the rows lie.  Differentiable in every tensor."""
+    calls = _ext.calls()
+    if calls is not None:
+        r = calls.causal_conv1d(x, weight, bias, initial_state, silu, reverse, output_final_state)
+        if r is not None:
+            return r if output_final_state else (r, None)
     ops._check_cuda(x, weight, bias, initial_state)
     if x.dim() != 3:
         raise ValueError("x must be [B,L,D]")
@@ -350,6 +365,11 @@ def _conv_backward(x, w, b, h0, dy, d_final, silu, reverse, want_state, want_par
 def causal_conv1d_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, bias: Optional[torch.Tensor] = None, silu: bool = False) -> torch.Tensor:
     """causal_conv1d for one token of every sequence: x [B,D]; state, the W - 1 rows in front ([B,W-1,D] of x's dtype, contiguous, apart from x's memory), takes x in and lets its
     oldest row go, in place.  Inference only."""
+    calls = _ext.calls()
+    if calls is not None:
+        y = calls.causal_conv1d_step(x, weight, state, bias, silu)
+        if y is not None:
+            return y
     ops._check_cuda(x, weight, state, bias)
     if _needs_graph(x, weight, state, bias):
         raise ValueError("causal_conv1d_step updates its state in place and records no gradient; use causal_conv1d")
@@ -391,6 +411,12 @@ def add_layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     As rmsnorm(), with a mean and a bias, and a gradient for each.  x [..., C] in fp32 or bf16, C up to 16384; residual of its dtype or in fp32 (a residual stream in fp32 beside bf16
     branches), which is the dtype of the sum.  The sum as it is stored is what is normalised.  weight, bias [C].  Up to 2^24 rows.  Differentiable in every tensor, the weight's and
     the bias's gradient added up in an order fixed by the sizes and by how the rows lie."""
+    calls = _ext.calls()
+    if calls is not None:
+        r = calls.add_layernorm(x, weight, bias, residual, eps)
+        if r is not None:
+            y, total = (r, x) if residual is None else r
+            return (y, total) if prenorm else y
     ops._check_cuda(x, weight, bias, residual)
     given = (x, weight, bias, residual)
     _refuse_tangents("add_layernorm", *given)
