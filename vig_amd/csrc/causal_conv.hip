@@ -30,36 +30,76 @@ template <int V, typename T> __device__ __forceinline__ void store_vec(T* to, co
   *reinterpret_cast<Whole*>(to) = w;
 }
 
-// A thread's place: channels from c on, tokens of the walk from `first` to `end`
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr unsigned kNowhere = 0x80000000u;  // byte offset behind every descriptor here
+
+// V channels of a row as stored
+template <typename T, int V> struct Piece {
+  static constexpr int kBytes = V * sizeof(T);
+  u32x4_t v;
+  __device__ __forceinline__ void load(rsrc_t r, unsigned off) {
+    if constexpr (kBytes == 16) v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+    else if constexpr (kBytes == 8) { const u32x2_t w = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); v[0] = w[0], v[1] = w[1]; }
+    else if constexpr (kBytes == 4) v[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else v[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+  }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(v[i]);
+      else x[i] = i & 1 ? bf16hi_to_f32(v[i / 2]) : bf16lo_to_f32(v[i / 2]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(x[i]);
+      else if constexpr (V == 1) v[0] = f32_to_bf16(x[0]);
+      else if (i & 1) v[i / 2] = pack_bf16x2(x[i - 1], x[i]);
+    }
+  }
+  __device__ __forceinline__ void store(rsrc_t r, unsigned off) const {
+    if constexpr (kBytes == 16) __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
+    else if constexpr (kBytes == 8) __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{v[0], v[1]}, r, off, 0, 0);
+    else if constexpr (kBytes == 4) __builtin_amdgcn_raw_buffer_store_b32(v[0], r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16((uint16_t)v[0], r, off, 0, 0);
+  }
+};
+
+// A thread's place: channels from c on, tokens of the walk from `first` to `end`; and the tokens that its workgroup reads, from `low` to `high`
 template <int V> struct Run {
-  int b, c, first, end;
+  int b, c, first, end, low, high;
   bool has;
   __device__ __forceinline__ Run(const CausalConv& p) {
     unsigned id = blockIdx.x;
     const int block = (int)(id % (unsigned)p.blocks);
     id /= (unsigned)p.blocks;
-    const int runs = (int)(id % (unsigned)p.groups) * kConvRuns + threadIdx.x / kConvLanes;
+    const long long group = (long long)(id % (unsigned)p.groups) * kConvRuns * p.run;
     b = (int)(id / (unsigned)p.groups);
     c = (block * kConvLanes + threadIdx.x % kConvLanes) * V;
-    first = (int)min((long long)runs * p.run, (long long)p.L), end = min(first + p.run, p.L);
+    first = (int)min(group + threadIdx.x / kConvLanes * p.run, (long long)p.L), end = min(first + p.run, p.L);
+    low = (int)max(group - (p.W - 1), 0LL), high = (int)min(group + kConvRuns * p.run + p.W - 1, (long long)p.L);
     has = c < p.D && first < end;
   }
 };
-
-// x of the walk's token t, in front of the first from the state
-template <typename T, int V>
-__device__ __forceinline__ void load_row(float (&x)[V], const CausalConv& p, int b, int c, int t) {
-  const T* from = nullptr;
-  if (t >= 0) from = static_cast<const T*>(p.x) + b * p.xb + (p.reverse ? p.L - 1 - t : t) * p.xl + c;
-  else if (p.initial) from = static_cast<const T*>(p.initial) + ((long long)b * (p.W - 1) + t + p.W - 1) * p.D + c;
-  if (from) {
-    load_vec<V>(x, from);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = 0.f;
+// The workgroup's rows of a tensor: the descriptor begins at the lowest in memory and ends behind the highest, so that rows in front of the first token and behind the last
+// read as zeros and are not stored
+template <typename T> struct RowsOf {
+  rsrc_t r;
+  unsigned pitch, offset;  // offset: of token 0 of the walk, for this thread
+  bool reverse;
+  template <int V> __device__ __forceinline__ RowsOf(const CausalConv& p, const Run<V>& at, const void* base, long long sb, long long sl) {
+    reverse = p.reverse != 0;
+    const long long lowest = p.reverse ? (long long)p.L - at.high : at.low;
+    r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(base)) + at.b * sb + lowest * sl, 0, (int)((at.high - at.low) * (unsigned)(sl * sizeof(T))), 0x00020000);
+    pitch = (unsigned)sl * sizeof(T);
+    offset = at.has ? at.c * (unsigned)sizeof(T) : kNowhere;
+    low = at.low, high = at.high;
   }
-}
-__device__ __forceinline__ long long dense_row(const CausalConv& p, int b, int t) { return ((long long)b * p.L + (p.reverse ? p.L - 1 - t : t)) * p.D; }
+  int low, high;
+  // (rows that are not there wrap round to offsets behind the descriptor)
+  __device__ __forceinline__ unsigned of(int t) const { return offset + (unsigned)(reverse ? high - 1 - t : t - low) * pitch; }
+};
 
 template <int V, int W> struct Taps {
   float w[V][W], bias[V];
@@ -72,40 +112,84 @@ template <int V, int W> struct Taps {
     }
   }
 };
+// the state's row of token t < 0, or zeros
+template <typename T, int V>
+__device__ __forceinline__ void state_row(float (&x)[V], const CausalConv& p, int b, int c, int t) {
+  if (p.initial) {
+    load_vec<V>(x, static_cast<const T*>(p.initial) + ((long long)b * (p.W - 1) + t + p.W - 1) * p.D + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = 0.f;
+  }
+}
+
+// Tokens whose rows are on their way together: the next ones' while a thread works on these
+constexpr int kConvTokens = 8;
 
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void causal_conv_kernel(CausalConv p) {
   const Run<V> at(p);
+  const RowsOf<T> in(p, at, p.x, p.xb, p.xl), out(p, at, p.y, (long long)p.L * p.D, p.D);
+  Piece<T, V> raw[2][kConvTokens];
+  auto load = [&](Piece<T, V> (&to)[kConvTokens], int t) {
+#pragma unroll
+    for (int k = 0; k < kConvTokens; ++k) to[k].load(in.r, in.of(t + k));
+  };
+  Piece<T, V> edge[W - 1];
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) edge[k].load(in.r, in.of(at.first - (W - 1) + k));
+  load(raw[0], at.first);
   if (!at.has) return;
   Taps<V, W> taps;
   taps.load(p, at.c);
   float rows[W][V];  // the last one is the newest
 #pragma unroll
-  for (int k = 1; k < W; ++k) load_row<T, V>(rows[k], p, at.b, at.c, at.first - W + k);
-  T* const final = static_cast<T*>(p.final);
-  const long long held = (long long)at.b * (W - 1);
-  if (final && at.first == 0) {  // states of the state, where there are fewer tokens than it has rows
-#pragma unroll
-    for (int k = 1; k < W; ++k)
-      if (k - 1 - p.L >= 0) store_vec<V>(final + (held + k - 1 - p.L) * p.D + at.c, rows[k]);
+  for (int k = 0; k + 1 < W; ++k) {
+    if (at.first - (W - 1) + k < 0) state_row<T, V>(rows[k + 1], p, at.b, at.c, at.first - (W - 1) + k);
+    else edge[k].get(rows[k + 1]);
   }
-#pragma unroll 4
-  for (int t = at.first; t < at.end; ++t) {
+  auto work = [&](const Piece<T, V> (&from)[kConvTokens], int t) {
 #pragma unroll
-    for (int k = 0; k + 1 < W; ++k)
+    for (int k = 0; k < kConvTokens; ++k) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) rows[k][i] = rows[k + 1][i];
-    load_row<T, V>(rows[W - 1], p, at.b, at.c, t);
-    float y[V];
+      for (int j = 0; j + 1 < W; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float s = taps.bias[i];
+        for (int i = 0; i < V; ++i) rows[j][i] = rows[j + 1][i];
+      from[k].get(rows[W - 1]);
+      float y[V];
 #pragma unroll
-      for (int k = 0; k < W; ++k) s = fmaf(taps.w[i][k], rows[k][i], s);
-      y[i] = p.silu ? s * sigmoidf_(s) : s;
+      for (int i = 0; i < V; ++i) {
+        float s = taps.bias[i];
+#pragma unroll
+        for (int j = 0; j < W; ++j) s = fmaf(taps.w[i][j], rows[j][i], s);
+        y[i] = p.silu ? s * sigmoidf_(s) : s;
+      }
+      Piece<T, V> o;
+      o.set(y);
+      o.store(out.r, t + k < at.end ? out.of(t + k) : kNowhere);
     }
-    store_vec<V>(static_cast<T*>(p.y) + dense_row(p, at.b, t) + at.c, y);
-    if (final && t >= p.L - (W - 1)) store_vec<V>(final + (held + t - (p.L - (W - 1))) * p.D + at.c, rows[W - 1]);
+  };
+  for (int t = at.first; t < at.end; t += 2 * kConvTokens) {
+    load(raw[1], t + kConvTokens);
+    work(raw[0], t);
+    if (t + kConvTokens >= at.end) break;
+    load(raw[0], t + 2 * kConvTokens);
+    work(raw[1], t + kConvTokens);
+  }
+  if (!p.final || at.end != p.L) return;
+  // the last rows, those of the state among them where there are few tokens
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) {
+    const int t = p.L - (W - 1) + k;
+    float x[V];
+    if (t < 0) {
+      state_row<T, V>(x, p, at.b, at.c, t);
+    } else {
+      Piece<T, V> last;
+      last.load(in.r, in.of(t));
+      last.get(x);
+    }
+    store_vec<V>(static_cast<T*>(p.final) + ((long long)at.b * (W - 1) + k) * p.D + at.c, x);
   }
 }
 
@@ -114,56 +198,67 @@ template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CausalConv p) {
   __shared__ float sums[kConvRuns][kConvLanes * V + 1];
   const Run<V> at(p);
-  Taps<V, W> taps;
-  float dw[V][W], db[V], x[W][V], dpre[W][V];  // the last rows are the newest
+  const RowsOf<T> in(p, at, p.x, p.xb, p.xl), grad(p, at, p.dy, (long long)p.L * p.D, p.D), out(p, at, p.dx, (long long)p.L * p.D, p.D);
+  float dw[V][W], db[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     db[i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) dw[i][k] = 0.f, dpre[k][i] = 0.f;
+    for (int k = 0; k < W; ++k) dw[i][k] = 0.f;
   }
-  if (at.has) {
-    taps.load(p, at.c);
+  Piece<T, V> raw_x[kConvTokens], raw_dy[kConvTokens], edge[W - 1];
+  auto load = [&](int t) {
 #pragma unroll
-    for (int k = 1; k < W; ++k) load_row<T, V>(x[k], p, at.b, at.c, at.first - W + k);
+    for (int k = 0; k < kConvTokens; ++k) raw_x[k].load(in.r, in.of(t + k)), raw_dy[k].load(grad.r, grad.of(t + k));
+  };
+#pragma unroll
+  for (int k = 0; k + 1 < W; ++k) edge[k].load(in.r, in.of(at.first - (W - 1) + k));
+  load(at.first);
+  if (at.has) {
+    Taps<V, W> taps;
+    taps.load(p, at.c);
+    float x[W][V], dpre[W][V];  // the last rows are the newest
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k) {
+      if (at.first - (W - 1) + k < 0) state_row<T, V>(x[k + 1], p, at.b, at.c, at.first - (W - 1) + k);
+      else edge[k].get(x[k + 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) dpre[k][i] = 0.f;
     const T* const final = static_cast<const T*>(p.d_final);
     const long long held = (long long)at.b * (W - 1);
-    // the gradient of token t is whole once dpre of t + W - 1 is there
-    const int stop = at.end + W - 1;
-#pragma unroll 2
-    for (int t = at.first; t < stop; ++t) {
+    // the gradient of a token is whole once dpre of the token W - 1 behind it is there
+    for (int t0 = at.first; t0 < at.end + W - 1; t0 += kConvTokens) {
+      Piece<T, V> now_x[kConvTokens], now_dy[kConvTokens];
 #pragma unroll
-      for (int k = 0; k + 1 < W; ++k)
+      for (int k = 0; k < kConvTokens; ++k) now_x[k] = raw_x[k], now_dy[k] = raw_dy[k];
+      if (t0 + kConvTokens < at.end + W - 1) load(t0 + kConvTokens);
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] = x[k + 1][i], dpre[k][i] = dpre[k + 1][i];
-      if (t < p.L) {
-        load_row<T, V>(x[W - 1], p, at.b, at.c, t);
-        load_vec<V>(dpre[W - 1], static_cast<const T*>(p.dy) + dense_row(p, at.b, t) + at.c);
-        if (p.silu) {
+      for (int u = 0; u < kConvTokens; ++u) {
+        const int t = t0 + u;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
+        for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[k][i] = x[k + 1][i], dpre[k][i] = dpre[k + 1][i];
+        now_x[u].get(x[W - 1]);
+        now_dy[u].get(dpre[W - 1]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (p.silu) {
             float s = taps.bias[i];
 #pragma unroll
             for (int k = 0; k < W; ++k) s = fmaf(taps.w[i][k], x[k][i], s);
-            const float g = sigmoidf_(s);
-            dpre[W - 1][i] *= fmaf(s * g, 1.f - g, g);
+            const float g = sigmoidf_(s), d = dpre[W - 1][i] * fmaf(s * g, 1.f - g, g);
+            dpre[W - 1][i] = t < p.L ? d : 0.f;
           }
+          const float own = t < at.end ? dpre[W - 1][i] : 0.f;
+          db[i] += own;
+#pragma unroll
+          for (int k = 0; k < W; ++k) dw[i][k] = fmaf(own, x[k][i], dw[i][k]);
         }
-        if (t < at.end) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            db[i] += dpre[W - 1][i];
-#pragma unroll
-            for (int k = 0; k < W; ++k) dw[i][k] = fmaf(dpre[W - 1][i], x[k][i], dw[i][k]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) dpre[W - 1][i] = 0.f;
-      }
-      const int to = t - (W - 1);  // (dpre[k] is of token to + k)
-      if (to >= at.first || at.first == 0) {
-        if (to < 0 && !p.d_initial) continue;
+        const int to = t - (W - 1);  // (dpre[k] is of token to + k)
         float g[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -171,14 +266,16 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CausalConv p) {
 #pragma unroll
           for (int k = 0; k < W; ++k) g[i] = fmaf(taps.w[i][W - 1 - k], dpre[k][i], g[i]);
         }
-        if (final && to >= p.L - (W - 1)) {
+        if (final && to >= p.L - (W - 1) && to < at.end) {
           float f[V];
           load_vec<V>(f, final + (held + to - (p.L - (W - 1))) * p.D + at.c);
 #pragma unroll
           for (int i = 0; i < V; ++i) g[i] += f[i];
         }
-        if (to >= 0) store_vec<V>(static_cast<T*>(p.dx) + dense_row(p, at.b, to) + at.c, g);
-        else store_vec<V>(static_cast<T*>(p.d_initial) + (held + to + W - 1) * p.D + at.c, g);
+        Piece<T, V> o;
+        o.set(g);
+        o.store(out.r, to >= at.first && to < at.end ? out.of(to) : kNowhere);
+        if (to < 0 && at.first == 0 && p.d_initial) store_vec<V>(static_cast<T*>(p.d_initial) + (held + to + W - 1) * p.D + at.c, g);
       }
     }
   }

@@ -181,8 +181,9 @@ struct SelScanStep {
   int batch, D, N, G;
   long long x_stride, delta_stride, z_stride, B_strides[2], C_strides[2];  // between batch elements; B, C: and between groups
   int softplus, io_dtype;
+  int blocks;  // workgroups along the channels
 };
-int launch_selective_scan_step(const SelScanStep& s, hipStream_t stream);
+int launch_selective_scan_step(SelScanStep& s, hipStream_t stream);
 
 // The short causal convolution (causal_conv.hip)
 struct CausalConv {

@@ -55,6 +55,8 @@ inline bool scan_fits(const SelScanArgs& p) {
   const long long NP = 4 * scan_states(p.N), most = 0xffffffLL;
   return (long long)p.batch * p.G * p.blocks * p.chunks <= most && (long long)p.batch * p.D * NP / 256 < most && (long long)p.batch * p.G * p.L / 128 * NP < most;
 }
+// Few chunks are joined by those who come behind them (entering), many by a launch of their own: each reads all in front of it, 68 bytes a channel of 16 states.
+constexpr int kFewChunks = 32;
 inline unsigned scan_grid(const SelScanArgs& p) { return (unsigned)((long long)p.batch * p.G * p.blocks * p.chunks); }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -215,6 +217,29 @@ template <int CN> __device__ __forceinline__ void kept_states(float (&h)[CN], co
   } else {
 #pragma unroll
     for (int i = 0; i < CN; ++i) h[i] = from[i];
+  }
+}
+
+// What enters a chunk from the chunks in front of it (BACK: behind it), whose ends and sums of steps a launch before has left: h, what enters the first of them, moved on
+template <bool BACK, int CN> __device__ __forceinline__ void entering(float (&h)[CN], const float (&A)[CN], const SelScanArgs& p, const Stand& at) {
+  constexpr int K = CN <= 4 ? 8 : 4;  // on their way together
+  if (!at.has) return;
+  const int count = BACK ? p.chunks - 1 - at.chunk : at.chunk;
+  for (int k0 = 0; k0 < count; k0 += K) {
+    float leaves[K][CN], sum[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = min(k0 + k, count - 1);
+      const size_t row = (size_t)at.b * p.chunks + (BACK ? p.chunks - 1 - i : i);
+      kept_states(leaves[k], p.ends, row, p.D, at);
+      sum[k] = p.sums[row * p.D + at.c];
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k0 + k >= count) break;
+#pragma unroll
+      for (int i = 0; i < CN; ++i) h[i] = fmaf(__builtin_amdgcn_exp2f(A[i] * sum[k]), h[i], leaves[k][i]);
+    }
   }
 }
 

@@ -27,10 +27,11 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) h[i] = 0.f;
-  } else if (p.chunks > 1) {
+  } else if (p.chunks > kFewChunks) {
     kept_states(h, p.ends, row, p.D, at);
   } else {
     load_states(h, p.h0, at.b, p.D, p.N, p.N, at);
+    entering<false>(h, A, p, at);
   }
   const bool gated = !FOLD && p.z.at;
   float sum = 0.f;
@@ -98,9 +99,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
 }
 
 // What chunks leave -> what enters them, in place: along the walk (forward), or against it (backward, whose last chunk is entered by the end's gradient).
-// A thread for each state of a channel.
+// A thread for each state of a channel, eight chunks on their way together.
 template <bool BACK>
 __global__ __launch_bounds__(256) void selective_join_kernel(SelScanArgs p, int np) {
+  constexpr int K = 8;
   const long long n = (long long)p.D * np, id = (long long)blockIdx.x * 256 + threadIdx.x;
   if (id >= p.batch * n) return;
   const long long b = id / n, in = id - b * n;
@@ -108,68 +110,105 @@ __global__ __launch_bounds__(256) void selective_join_kernel(SelScanArgs p, int 
   const float* from = BACK ? p.dhT : p.h0;
   float h = from && s < p.N ? from[(b * p.D + c) * p.N + s] : 0.f;
   const float A = s < p.N ? p.A[(long long)c * p.N + s] * kLog2e : 0.f;
-  for (int k = 0; k < p.chunks; ++k) {
-    const size_t row = (size_t)b * p.chunks + (BACK ? p.chunks - 1 - k : k);
-    float* at = p.ends + row * n + in;
-    const float leaves = *at, a = __builtin_amdgcn_exp2f(A * p.sums[row * p.D + c]);
-    *at = h;
-    h = fmaf(a, h, leaves);
+  auto row = [&](int k) { return (size_t)b * p.chunks + (BACK ? p.chunks - 1 - k : k); };
+  for (int k0 = 0; k0 < p.chunks; k0 += K) {
+    float leaves[K], sum[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const size_t r = row(min(k0 + k, p.chunks - 1));
+      leaves[k] = p.ends[r * n + in], sum[k] = p.sums[r * p.D + c];
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (k0 + k >= p.chunks) break;
+      p.ends[row(k0 + k) * n + in] = h;
+      h = fmaf(__builtin_amdgcn_exp2f(A * sum[k]), h, leaves[k]);
+    }
   }
 }
 
-// ---- one token of every sequence.  NL lanes take a channel, four states each: side by side in pieces of 16 bytes (WHOLE), or NL apart.
+// ---- one token of every sequence.  NL lanes take a channel, four states each: side by side in pieces of 16 bytes (WHOLE; B and C in whole fours then too), or NL apart.  A thread goes through
+// ROWS sequences' states of the channel, all of them on their way together.
 
-template <typename S, int NL, bool WHOLE>
+template <typename S> __device__ __forceinline__ void four(float (&v)[4], const S* from);
+template <> __device__ __forceinline__ void four<uint16_t>(float (&v)[4], const uint16_t* from) {
+  const u32x2_t w = *reinterpret_cast<const u32x2_t*>(from);
+  v[0] = bf16lo_to_f32(w[0]), v[1] = bf16hi_to_f32(w[0]), v[2] = bf16lo_to_f32(w[1]), v[3] = bf16hi_to_f32(w[1]);
+}
+template <> __device__ __forceinline__ void four<float>(float (&v)[4], const float* from) {
+  const f32x4_t w = *reinterpret_cast<const f32x4_t*>(from);
+  v[0] = w[0], v[1] = w[1], v[2] = w[2], v[3] = w[3];
+}
+
+template <typename S, int NL, bool WHOLE, int ROWS>
 __global__ __launch_bounds__(256) void selective_step_kernel(SelScanStep p) {
-  const long long id = ((long long)blockIdx.x * 256 + threadIdx.x) / NL;
-  const int l = threadIdx.x % NL;
-  const bool is = id < (long long)p.batch * p.D;  // (the others still take part in the sums)
-  const long long at = is ? id : 0;
-  const int b = (int)(at / p.D), c = (int)(at - (long long)b * p.D), g = c / (p.D / p.G);
-  const float raw = Elem<S>::load(static_cast<const S*>(p.delta) + b * p.delta_stride + c) + (p.bias ? p.bias[c] : 0.f);
-  const float x = Elem<S>::load(static_cast<const S*>(p.x) + b * p.x_stride + c);
-  const S* const B = static_cast<const S*>(p.B) + b * p.B_strides[0] + g * p.B_strides[1];
-  const S* const C = static_cast<const S*>(p.C) + b * p.C_strides[0] + g * p.C_strides[1];
-  float* const state = p.state + at * p.N;
-  const float* const decay = p.A + (long long)c * p.N;
+  constexpr int kChannels = 256 / NL;
+  const int l = threadIdx.x % NL, c = (int)(blockIdx.x % (unsigned)p.blocks) * kChannels + threadIdx.x / NL, first = (int)(blockIdx.x / (unsigned)p.blocks) * ROWS;
+  const bool is = c < p.D && (!WHOLE || 4 * l < p.N);
   auto n = [&](int i) { return WHOLE ? 4 * l + i : l + NL * i; };
-  float h[4], a[4];
-  if constexpr (WHOLE) {
-    if (4 * l < p.N) {
-      const f32x4_t hv = *reinterpret_cast<const f32x4_t*>(state + 4 * l), av = *reinterpret_cast<const f32x4_t*>(decay + 4 * l);
+  float a[4] = {0.f, 0.f, 0.f, 0.f}, h[ROWS][4], b[ROWS][4], g[ROWS][4], x[ROWS], raw[ROWS], z[ROWS];
+  const int group = is ? c / (p.D / p.G) : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = hv[i], a[i] = av[i];
+  for (int r = 0; r < ROWS; ++r) {
+    const long long row = first + r;
+    x[r] = raw[r] = z[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[r][i] = b[r][i] = g[r][i] = 0.f;
+    if (!is || row >= p.batch) continue;
+    const float* const state = p.state + (row * p.D + c) * p.N;
+    const S* const B = static_cast<const S*>(p.B) + row * p.B_strides[0] + group * p.B_strides[1];
+    const S* const C = static_cast<const S*>(p.C) + row * p.C_strides[0] + group * p.C_strides[1];
+    if constexpr (WHOLE) {
+      four<float>(h[r], state + 4 * l), four<S>(b[r], B + 4 * l), four<S>(g[r], C + 4 * l);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n(i) < p.N) h[r][i] = state[n(i)], b[r][i] = Elem<S>::load(B + n(i)), g[r][i] = Elem<S>::load(C + n(i));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n(i) < p.N) h[i] = state[n(i)], a[i] = decay[n(i)];
+    x[r] = Elem<S>::load(static_cast<const S*>(p.x) + row * p.x_stride + c), raw[r] = Elem<S>::load(static_cast<const S*>(p.delta) + row * p.delta_stride + c);
+    if (p.z) z[r] = Elem<S>::load(static_cast<const S*>(p.z) + row * p.z_stride + c);
   }
-  const float step = step_of(raw, p.softplus), u = step * x;
-  float y = 0.f;
+  float bias = 0.f, skip = 0.f;
+  if (is) {
+    const float* const decay = p.A + (long long)c * p.N;
+    if constexpr (WHOLE) {
+      four<float>(a, decay + 4 * l);
+    } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (n(i) < p.N) {
-      h[i] = fmaf(u, Elem<S>::load(B + n(i)), exp_fast(step * a[i]) * h[i]);
-      y = fmaf(Elem<S>::load(C + n(i)), h[i], y);
+      for (int i = 0; i < 4; ++i)
+        if (n(i) < p.N) a[i] = decay[n(i)];
     }
-#pragma unroll
-  for (int k = 1; k < NL; k *= 2) y += __shfl_xor(y, k);
-  if (!is) return;
-  if constexpr (WHOLE) {
-    if (4 * l < p.N) *reinterpret_cast<f32x4_t*>(state + 4 * l) = f32x4_t{h[0], h[1], h[2], h[3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n(i) < p.N) state[n(i)] = h[i];
+    if (p.bias) bias = p.bias[c];
+    if (p.skip) skip = p.skip[c];
   }
-  if (l) return;
-  if (p.skip) y = fmaf(p.skip[c], x, y);
-  if (p.z) {
-    const float z = Elem<S>::load(static_cast<const S*>(p.z) + b * p.z_stride + c);
-    y *= z * sigmoidf_(z);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const float step = step_of(raw[r] + bias, p.softplus), u = step * x[r];
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[r][i] = fmaf(u, b[r][i], exp_fast(step * a[i]) * h[r][i]);
+      // (a state that is not there may have become NaN of an infinite step)
+      if (WHOLE || n(i) < p.N) y = fmaf(g[r][i], h[r][i], y);
+    }
+    if (!is) y = 0.f;
+#pragma unroll
+    for (int k = 1; k < NL; k *= 2) y += __shfl_xor(y, k);
+    const long long row = first + r;
+    if (!is || row >= p.batch) continue;
+    float* const state = p.state + (row * p.D + c) * p.N;
+    if constexpr (WHOLE) {
+      *reinterpret_cast<f32x4_t*>(state + 4 * l) = f32x4_t{h[r][0], h[r][1], h[r][2], h[r][3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n(i) < p.N) state[n(i)] = h[r][i];
+    }
+    if (l) continue;
+    y = fmaf(skip, x[r], y);
+    if (p.z) y *= z[r] * sigmoidf_(z[r]);
+    Elem<S>::store(static_cast<S*>(p.o) + row * p.D + c, y);
   }
-  Elem<S>::store(static_cast<S*>(p.o) + at, y);
 }
 
 }  // namespace
@@ -185,24 +224,34 @@ static int run_forward(const SelScanArgs& p, hipStream_t stream) {
   const dim3 grid(scan_grid(p)), block(64 * kScanWaves);
   if (p.chunks > 1) {
     hipLaunchKernelGGL((selective_scan_kernel<S, CN, true>), grid, block, 0, stream, p);
-    const int rc = launch_selective_join(p, 4 * CN, false, stream);
+    const int rc = p.chunks > kFewChunks ? launch_selective_join(p, 4 * CN, false, stream) : 0;
     if (rc) return rc;
   }
   hipLaunchKernelGGL((selective_scan_kernel<S, CN, false>), grid, block, 0, stream, p);
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }
 
-template <typename S, int NL>
-static int run_step(const SelScanStep& p, hipStream_t stream) {
-  const long long groups = ((long long)p.batch * p.D * NL + 255) / 256;
+template <typename S, int NL, bool WHOLE, int ROWS>
+static int run_step(SelScanStep& p, hipStream_t stream) {
+  p.blocks = (p.D + 256 / NL - 1) / (256 / NL);
+  const long long groups = (long long)p.blocks * ((p.batch + ROWS - 1) / ROWS);
   if (groups > 0xffffff) return -95;
-  const bool whole = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % 16 == 0 && reinterpret_cast<uintptr_t>(p.A) % 16 == 0;
-  hipLaunchKernelGGL((whole ? selective_step_kernel<S, NL, true> : selective_step_kernel<S, NL, false>), dim3((unsigned)groups), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((selective_step_kernel<S, NL, WHOLE, ROWS>), dim3((unsigned)groups), dim3(256), 0, stream, p);
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }
+// Four sequences a thread once that leaves four workgroups a compute unit
+template <typename S, int NL>
+static int step_rows(SelScanStep& p, hipStream_t stream) {
+  auto on = [](const void* t, size_t bytes) { return reinterpret_cast<uintptr_t>(t) % bytes == 0; };
+  bool whole = p.N % 4 == 0 && on(p.state, 16) && on(p.A, 16) && on(p.B, 4 * sizeof(S)) && on(p.C, 4 * sizeof(S));
+  for (int k = 0; k < 2; ++k) whole = whole && p.B_strides[k] % 4 == 0 && p.C_strides[k] % 4 == 0;
+  const bool many = (long long)p.batch * p.D * NL / (4 * 256) >= 1024;
+  if (whole) return many ? run_step<S, NL, true, 4>(p, stream) : run_step<S, NL, true, 1>(p, stream);
+  return many ? run_step<S, NL, false, 4>(p, stream) : run_step<S, NL, false, 1>(p, stream);
+}
 
-int launch_selective_scan_step(const SelScanStep& p, hipStream_t stream) {
-  return by_states(scan_states(p.N), [&](auto nl) { return p.io_dtype == VIG_BF16 ? run_step<uint16_t, nl>(p, stream) : run_step<float, nl>(p, stream); });
+int launch_selective_scan_step(SelScanStep& p, hipStream_t stream) {
+  return by_states(scan_states(p.N), [&](auto nl) { return p.io_dtype == VIG_BF16 ? step_rows<uint16_t, nl>(p, stream) : step_rows<float, nl>(p, stream); });
 }
 
 int launch_selective_scan(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream) {

@@ -51,10 +51,11 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) back[i] = 0.f;
-  } else if (p.chunks > 1) {
+  } else if (p.chunks > kFewChunks) {
     kept_states(back, p.ends, row, p.D, at);
   } else {
     load_states(back, p.dhT, at.b, p.D, p.N, p.N, at);
+    entering<true>(back, A, p, at);
   }
   const bool gated = p.z.at;
   float sum = 0.f, dskip = 0.f, dbias = 0.f, dA[CN];
@@ -239,7 +240,7 @@ static int run_backward(const SelScanArgs& p, hipStream_t stream) {
   const dim3 grid(scan_grid(p)), block(64 * kScanWaves);
   if (p.chunks > 1) {
     hipLaunchKernelGGL((selective_scan_bwd_kernel<S, CN, true>), grid, block, 0, stream, p);
-    const int rc = launch_selective_join(p, 4 * CN, true, stream);
+    const int rc = p.chunks > kFewChunks ? launch_selective_join(p, 4 * CN, true, stream) : 0;
     if (rc) return rc;
   }
   hipLaunchKernelGGL((selective_scan_bwd_kernel<S, CN, false>), grid, block, 0, stream, p);
