@@ -101,14 +101,28 @@ template <typename T> struct RowsOf {
   __device__ __forceinline__ unsigned of(int t) const { return offset + (unsigned)(reverse ? high - 1 - t : t - low) * pitch; }
 };
 
+// Weights of V channels: in pieces of 16 bytes where they begin on one
+template <int N> __device__ __forceinline__ void load_floats(float (&x)[N], const float* from) {
+  if (N % 4 == 0 && reinterpret_cast<uintptr_t>(from) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i + 3 < N; i += 4) {
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + i);
+      x[i] = v[0], x[i + 1] = v[1], x[i + 2] = v[2], x[i + 3] = v[3];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = from[i];
+  }
+}
 template <int V, int W> struct Taps {
-  float w[V][W], bias[V];
+  float w[V * W], bias[V];
   __device__ __forceinline__ void load(const CausalConv& p, int c) {
+    load_floats(w, p.weight + (long long)c * W);
+    if (p.bias) {
+      load_floats(bias, p.bias + c);
+    } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-#pragma unroll
-      for (int k = 0; k < W; ++k) w[i][k] = p.weight[(long long)(c + i) * W + k];
-      bias[i] = p.bias ? p.bias[c + i] : 0.f;
+      for (int i = 0; i < V; ++i) bias[i] = 0.f;
     }
   }
 };
@@ -124,7 +138,7 @@ __device__ __forceinline__ void state_row(float (&x)[V], const CausalConv& p, in
 }
 
 // Tokens whose rows are on their way together: the next ones' while a thread works on these
-constexpr int kConvTokens = 8;
+constexpr int kConvTokens = 2;
 
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void causal_conv_kernel(CausalConv p) {
@@ -161,7 +175,7 @@ __global__ __launch_bounds__(256) void causal_conv_kernel(CausalConv p) {
       for (int i = 0; i < V; ++i) {
         float s = taps.bias[i];
 #pragma unroll
-        for (int j = 0; j < W; ++j) s = fmaf(taps.w[i][j], rows[j][i], s);
+        for (int j = 0; j < W; ++j) s = fmaf(taps.w[i * W + j], rows[j][i], s);
         y[i] = p.silu ? s * sigmoidf_(s) : s;
       }
       Piece<T, V> o;
@@ -249,7 +263,7 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CausalConv p) {
           if (p.silu) {
             float s = taps.bias[i];
 #pragma unroll
-            for (int k = 0; k < W; ++k) s = fmaf(taps.w[i][k], x[k][i], s);
+            for (int k = 0; k < W; ++k) s = fmaf(taps.w[i * W + k], x[k][i], s);
             const float g = sigmoidf_(s), d = dpre[W - 1][i] * fmaf(s * g, 1.f - g, g);
             dpre[W - 1][i] = t < p.L ? d : 0.f;
           }
@@ -264,7 +278,7 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(CausalConv p) {
         for (int i = 0; i < V; ++i) {
           g[i] = 0.f;
 #pragma unroll
-          for (int k = 0; k < W; ++k) g[i] = fmaf(taps.w[i][W - 1 - k], dpre[k][i], g[i]);
+          for (int k = 0; k < W; ++k) g[i] = fmaf(taps.w[i * W + W - 1 - k], dpre[k][i], g[i]);
         }
         if (final && to >= p.L - (W - 1) && to < at.end) {
           float f[V];
@@ -315,7 +329,7 @@ __global__ __launch_bounds__(256) void causal_conv_step_kernel(CausalConv p) {
   for (int i = 0; i < V; ++i) {
     float s = taps.bias[i];
 #pragma unroll
-    for (int k = 0; k < W; ++k) s = fmaf(taps.w[i][k], rows[k][i], s);
+    for (int k = 0; k < W; ++k) s = fmaf(taps.w[i * W + k], rows[k][i], s);
     y[i] = p.silu ? s * sigmoidf_(s) : s;
   }
 #pragma unroll

@@ -60,8 +60,12 @@ constexpr int kFewChunks = 32;
 inline unsigned scan_grid(const SelScanArgs& p) { return (unsigned)((long long)p.batch * p.G * p.blocks * p.chunks); }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float load1(rsrc_t r, unsigned off, float) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0)); }
-__device__ __forceinline__ float load1(rsrc_t r, unsigned off, uint16_t) { return bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0)); }
+// An element as stored, and its value: rows that are loaded ahead stay as they came, since whatever is done to them there would wait for them
+template <typename S> using Raw = std::conditional_t<sizeof(S) == 2, uint16_t, uint32_t>;
+__device__ __forceinline__ uint32_t load1(rsrc_t r, unsigned off, float) { return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); }
+__device__ __forceinline__ uint16_t load1(rsrc_t r, unsigned off, uint16_t) { return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0); }
+__device__ __forceinline__ float value(uint16_t raw) { return bf16_to_f32(raw); }
+__device__ __forceinline__ float value(uint32_t raw) { return __uint_as_float(raw); }
 __device__ __forceinline__ void store1(rsrc_t r, unsigned off, float v, float) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, off, 0, 0); }
 __device__ __forceinline__ void store1(rsrc_t r, unsigned off, float v, uint16_t) { __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(v), r, off, 0, 0); }
 
@@ -113,7 +117,7 @@ template <typename S> struct Line {
   }
   // token 4 m + q of the tile
   template <int T> __device__ __forceinline__ unsigned place(const Tile<T>& t, int m) const { return offset + (unsigned)(t.from + t.step * 4 * m) * pitch; }
-  template <int T> __device__ __forceinline__ float load(rsrc_t r, const Tile<T>& t, int m) const { return load1(r, place(t, m), S{}); }
+  template <int T> __device__ __forceinline__ Raw<S> load(rsrc_t r, const Tile<T>& t, int m) const { return load1(r, place(t, m), S{}); }
   template <int T> __device__ __forceinline__ void store(const Tile<T>& t, int m, float v) const { store1(of(t), place(t, m), v, S{}); }
 };
 
@@ -124,15 +128,13 @@ __device__ __forceinline__ float log1p_01(float e) {
   t = fmaf(w, t, 1.f / 9), t = fmaf(w, t, 1.f / 7), t = fmaf(w, t, 0.2f), t = fmaf(w, t, 1.f / 3);
   return 2.f * fmaf(s * w, t, s);
 }
-// the step of a token from what its projection gives, and its derivative
+// the step of a token from what its projection gives (with the bias), and its derivative
 __device__ __forceinline__ float step_of(float raw, int softplus) {
   const float soft = fmaxf(raw, 0.f) + log1p_01(exp_fast(-fabsf(raw)));
   return softplus ? soft : raw;
 }
 __device__ __forceinline__ float dstep_of(float raw, int softplus) {
-  if (!softplus) return 1.f;
-  const float e = exp_fast(-fabsf(raw));
-  const float soft = (raw >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
+  const float e = exp_fast(-fabsf(raw)), soft = (raw >= 0.f ? 1.f : e) * __builtin_amdgcn_rcpf(1.f + e);
   return softplus ? soft : 1.f;
 }
 
@@ -190,39 +192,43 @@ template <int CN> __device__ __forceinline__ void store_states(float* base, cons
     if (at.q * CN + i < n) base[(row * D + at.c) * stride + at.q * CN + i] = h[i];
 }
 // ... of rows of 4 CN numbers, all of them there, on 16-byte boundaries
-template <int CN> __device__ __forceinline__ void keep_states(float* base, const float (&h)[CN], size_t row, int D, const Stand& at) {
-  if (!at.has) return;
-  float* to = base + (row * D + at.c) * (4 * CN) + at.q * CN;
-  if constexpr (CN >= 4) {
-#pragma unroll
-    for (int i = 0; i < CN; i += 4) *reinterpret_cast<f32x4_t*>(to + i) = f32x4_t{h[i], h[i + 1], h[i + 2], h[i + 3]};
-  } else {
-#pragma unroll
-    for (int i = 0; i < CN; ++i) to[i] = h[i];
+template <int CN> struct Kept {
+  unsigned offset;
+  __device__ __forceinline__ explicit Kept(const Stand& at) : offset(at.has ? (at.c * 4 + at.q) * CN * (unsigned)sizeof(float) : kNowhere) {}
+  static __device__ __forceinline__ rsrc_t of(const float* base, size_t row, int D) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base) + row * (unsigned)(D * 4 * CN), 0, D * 4 * CN * (int)sizeof(float), 0x00020000);
   }
-}
-template <int CN> __device__ __forceinline__ void kept_states(float (&h)[CN], const float* base, size_t row, int D, const Stand& at) {
-  const float* from = base + (row * D + at.c) * (4 * CN) + at.q * CN;
-  if (!at.has) {
+  __device__ __forceinline__ void store(float* base, size_t row, int D, const float (&h)[CN]) const {
+    const rsrc_t r = of(base, row, D);
+    if constexpr (CN >= 4) {
 #pragma unroll
-    for (int i = 0; i < CN; ++i) h[i] = 0.f;
-    return;
-  }
-  if constexpr (CN >= 4) {
+      for (int i = 0; i < CN; i += 4)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{__float_as_uint(h[i]), __float_as_uint(h[i + 1]), __float_as_uint(h[i + 2]), __float_as_uint(h[i + 3])}, r, offset + 4 * i, 0, 0);
+    } else {
 #pragma unroll
-    for (int i = 0; i < CN; i += 4) {
-      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(from + i);
-      h[i] = w[0], h[i + 1] = w[1], h[i + 2] = w[2], h[i + 3] = w[3];
+      for (int i = 0; i < CN; ++i) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(h[i]), r, offset + 4 * i, 0, 0);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < CN; ++i) h[i] = from[i];
   }
-}
+  __device__ __forceinline__ void load(float (&h)[CN], const float* base, size_t row, int D) const {
+    const rsrc_t r = of(base, row, D);
+    if constexpr (CN >= 4) {
+#pragma unroll
+      for (int i = 0; i < CN; i += 4) {
+        const u32x4_t w = __builtin_amdgcn_raw_buffer_load_b128(r, offset + 4 * i, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[i + k] = __uint_as_float(w[k]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CN; ++i) h[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, offset + 4 * i, 0, 0));
+    }
+  }
+};
 
 // What enters a chunk from the chunks in front of it (BACK: behind it), whose ends and sums of steps a launch before has left: h, what enters the first of them, moved on
 template <bool BACK, int CN> __device__ __forceinline__ void entering(float (&h)[CN], const float (&A)[CN], const SelScanArgs& p, const Stand& at) {
   constexpr int K = CN <= 4 ? 8 : 4;  // on their way together
+  const Kept<CN> kept(at);
   if (!at.has) return;
   const int count = BACK ? p.chunks - 1 - at.chunk : at.chunk;
   for (int k0 = 0; k0 < count; k0 += K) {
@@ -231,7 +237,7 @@ template <bool BACK, int CN> __device__ __forceinline__ void entering(float (&h)
     for (int k = 0; k < K; ++k) {
       const int i = min(k0 + k, count - 1);
       const size_t row = (size_t)at.b * p.chunks + (BACK ? p.chunks - 1 - i : i);
-      kept_states(leaves[k], p.ends, row, p.D, at);
+      kept.load(leaves[k], p.ends, row, p.D);
       sum[k] = p.sums[row * p.D + at.c];
     }
 #pragma unroll
@@ -247,7 +253,7 @@ template <bool BACK, int CN> __device__ __forceinline__ void entering(float (&h)
 template <typename S, int CN> struct Shared {
   static constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN, E = NP > 16 ? NP / 16 : 1;
   Line<S> line[E];
-  float v[R][E];
+  Raw<S> v[R][E];
   __device__ __forceinline__ void stand(const SelScanArgs& p, const Rows& t, const Stand& at) {
 #pragma unroll
     for (int e = 0; e < E; ++e) line[e].stand(p, t.at, at.b * t.b + at.g * t.g, t.l, at.q, at.j + 16 * e, at.j + 16 * e < p.N);
@@ -264,13 +270,14 @@ template <typename S, int CN> struct Shared {
     for (int m = 0; m < R; ++m)
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (NP >= 16 || at.j < NP) to[4 * m + at.q][at.j + 16 * e] = v[m][e];
+        if (NP >= 16 || at.j < NP) to[4 * m + at.q][at.j + 16 * e] = value(v[m][e]);
   }
 };
 // Values of a tile's rows of channels as loaded: token 4 m + q of channel j
 template <typename S, int T> struct Channels {
   Line<S> line;
-  float v[T / 4];
+  Raw<S> v[T / 4];
+  __device__ __forceinline__ float operator[](int m) const { return value(v[m]); }
   __device__ __forceinline__ void stand(const SelScanArgs& p, const Rows& t, const Stand& at) { line.stand(p, t.at, at.b * t.b, t.l, at.q, at.c, at.has); }
   __device__ __forceinline__ void load(const Tile<T>& t) {
     const rsrc_t r = line.of(t);

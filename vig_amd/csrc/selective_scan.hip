@@ -24,11 +24,13 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
 #pragma unroll
   for (int i = 0; i < CN; ++i) A[i] *= kLog2e;
   const size_t row = (size_t)at.b * p.chunks + at.chunk;
+  const Kept<CN> kept(at);
+  [[maybe_unused]] const int tiles = (p.L + T - 1) / T;
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) h[i] = 0.f;
   } else if (p.chunks > kFewChunks) {
-    kept_states(h, p.ends, row, p.D, at);
+    kept.load(h, p.ends, row, p.D);
   } else {
     load_states(h, p.h0, at.b, p.D, p.N, p.N, at);
     entering<false>(h, A, p, at);
@@ -52,10 +54,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     float xs[R], zs[R];
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const float step = first + 4 * m + at.q < at.end ? step_of(delta.v[m] + bias, p.softplus) : 0.f;
-      xs[m] = x.v[m], zs[m] = z.v[m];
+      const float step = first + 4 * m + at.q < at.end ? step_of(delta[m] + bias, p.softplus) : 0.f;
+      xs[m] = x[m], zs[m] = z[m];
       pass.of_channel[0][at.j][4 * m + at.q] = step;
-      pass.of_channel[1][at.j][4 * m + at.q] = step * x.v[m];
+      pass.of_channel[1][at.j][4 * m + at.q] = step * x[m];
       if constexpr (FOLD) sum += step;
     }
     B.pass(pass.of_token[0], at);
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     passed();
     if (first + T < at.end) load(first + T);
     if constexpr (!FOLD)
-      if (p.kept) keep_states(p.kept, h, (size_t)at.b * ((p.L + T - 1) / T) + first / T, p.D, at);
+      if (p.kept) kept.store(p.kept, (size_t)at.b * tiles + first / T, p.D, h);
 #pragma unroll
     for (int m = 0; m < R; ++m) {
       float step[4], u[4], s[4];
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     passed();
   }
   if constexpr (FOLD) {
-    keep_states(p.ends, h, row, p.D, at);
+    kept.store(p.ends, row, p.D, h);
     sum = of_all_rows(sum);
     if (at.q == 0 && at.has) p.sums[row * p.D + at.c] = sum;
   } else if (p.hT && at.chunk == p.chunks - 1) {

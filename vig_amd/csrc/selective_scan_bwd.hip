@@ -12,21 +12,33 @@
 namespace vig {
 namespace {
 
-template <int CTRL> __device__ __forceinline__ float from_lane(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-// Sums of eight values over the sixteen channels of a lane row: lane j holds in out[i] those of value i + 2 (j >> 2 & 1) + 4 (j >> 3).
-__device__ __forceinline__ void of_channels(const float (&v)[8], float (&out)[2], int j) {
-  float w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = (j & 8 ? v[i + 4] : v[i]) + from_lane<0x128>(j & 8 ? v[i] : v[i + 4]);  // (row_ror:8)
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    // (row_half_mirror: the other four of eight, in some order)
-    float s = (j & 4 ? w[i + 2] : w[i]) + from_lane<0x141>(j & 4 ? w[i] : w[i + 2]);
-    s += from_lane<0xb1>(s);  // (quad_perm 1 0 3 2)
-    out[i] = s + from_lane<0x4e>(s);  // (quad_perm 2 3 0 1)
-  }
+// Sums of eight values over the sixteen channels of a lane row: lane j is left in out[i] with that of value i + 2 (j >> 2 & 1) + 4 (j >> 3).
+// Half the values stay with each half of the row, half of these with each half of it, and a sum over four lanes closes: 16 additions, each of them with its exchange of lanes, and the ones
+// that only some lanes take behind the ones that all do.  In assembly, because the compiler makes a selection of each addition that only some lanes take (22 instructions).  An instruction
+// that reads another lane's register stands two behind the one that wrote it: the compiler does not look in here.
+__device__ __forceinline__ void of_channels(const float (&v)[8], float (&out)[2]) {
+  float w0, w1, w2, w3;
+  asm("s_nop 1\n\t"
+      "v_add_f32_dpp %0, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %1, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %2, %8, %8 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %3, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %0, %10, %10 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+      "v_add_f32_dpp %1, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+      "v_add_f32_dpp %2, %12, %12 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+      "v_add_f32_dpp %3, %13, %13 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+      "v_add_f32_dpp %4, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %5, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %4, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+      "v_add_f32_dpp %5, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+      "s_nop 0\n\t"
+      "v_add_f32_dpp %0, %4, %4 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %1, %5, %5 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 0\n\t"
+      "v_add_f32_dpp %4, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "v_add_f32_dpp %5, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf"
+      : "=&v"(w0), "=&v"(w1), "=&v"(w2), "=&v"(w3), "=&v"(out[0]), "=&v"(out[1])
+      : "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]));
 }
 
 // A workgroup's sums of its waves' gradients of B (0) and C (1)
@@ -34,25 +46,43 @@ template <int CN> struct Board {
   float v[2][kTileTokens<CN>][4 * CN];
 };
 
+// A wave's LDS: of a tile each channel's step, dy, step times x and x of a token side by side, each token's B and C.
+template <int CN> struct BackPass {
+  static constexpr int T = kTileTokens<CN>;
+  f32x4_t of_channel[T][16];
+  float of_token[2][T][4 * CN];
+};
+// ... as a lane reads them of a token
+template <int CN> struct Token {
+  f32x4_t of;
+  float b[CN], c[CN];
+  __device__ __forceinline__ void read(const BackPass<CN>& pass, int t, const Stand& at, bool both) {
+    of = pass.of_channel[t][at.j];
+    if (both) read_lds(b, &pass.of_token[0][t][at.q * CN]);
+    read_lds(c, &pass.of_token[1][t][at.q * CN]);
+  }
+};
+
 // FOLD: only what a chunk hands back to the one in front of it
 template <typename S, int CN, bool FOLD>
 __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_bwd_kernel(SelScanArgs p) {
   constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN;
-  __shared__ __align__(16) Pass<CN, 3> lds[kScanWaves];
+  __shared__ __align__(16) BackPass<CN> lds[kScanWaves];
   __shared__ __align__(16) Board<CN> boards[FOLD ? 1 : 2][FOLD ? 1 : kScanWaves];
   const Stand at(p);
-  Pass<CN, 3>& pass = lds[at.wave];
+  BackPass<CN>& pass = lds[at.wave];
   const float bias = p.bias && at.has ? p.bias[at.c] : 0.f, skip = p.skip && at.has ? p.skip[at.c] : 0.f;
   float A[CN], back[CN];  // back: a dh of the token behind
   load_states(A, p.A, 0, p.D, p.N, p.N, at);
 #pragma unroll
   for (int i = 0; i < CN; ++i) A[i] *= kLog2e;
   const size_t row = (size_t)at.b * p.chunks + at.chunk;
+  const Kept<CN> states(at);
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) back[i] = 0.f;
   } else if (p.chunks > kFewChunks) {
-    kept_states(back, p.ends, row, p.D, at);
+    states.load(back, p.ends, row, p.D);
   } else {
     load_states(back, p.dhT, at.b, p.D, p.N, p.N, at);
     entering<true>(back, A, p, at);
@@ -64,6 +94,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   [[maybe_unused]] const Line<S> dx = dense_line<S>(p, p.dx, at), ddelta = dense_line<S>(p, p.ddelta, at), dz = dense_line<S>(p, p.dz, at);
   const int tiles = (p.L + T - 1) / T, last = at.first + (at.end - 1 - at.first) / T * T;
   Channels<S, T> x, delta, z, d_o;
+  [[maybe_unused]] float kept[CN];
   Shared<S, CN> B, C;
   delta.stand(p, p.delta, at), d_o.stand(p, p.d_o, at), C.stand(p, p.C, at), z.stand(p, p.z, at);
   if constexpr (!FOLD) x.stand(p, p.x, at), B.stand(p, p.B, at);
@@ -72,43 +103,42 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
     delta.load(tile), d_o.load(tile), C.load(tile);
     if (gated) z.load(tile);
     if constexpr (!FOLD) x.load(tile), B.load(tile);
+    if constexpr (!FOLD && CN <= 4) states.load(kept, p.kept, (size_t)at.b * tiles + first / T, p.D);  // (more of them have no room)
   };
   load(last);
   for (int first = last, turn = 0; first >= at.first; first -= T, turn ^= 1) {
     [[maybe_unused]] const Tile<T> tile(p, first, at.end);
-    float raw[R], xs[R], by_y[R];  // by_y: what makes dz of y
+    float by_raw[R], by_y[R];  // what makes gradients of raw steps of those of steps, and dz of y
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      raw[m] = delta.v[m] + bias, xs[m] = x.v[m];
-      const float step = first + 4 * m + at.q < at.end ? step_of(raw[m], p.softplus) : 0.f;
-      float dy = d_o.v[m];
+      const float raw = delta[m] + bias, step = first + 4 * m + at.q < at.end ? step_of(raw, p.softplus) : 0.f;
+      float dy = d_o[m], xs = 0.f;
+      if constexpr (!FOLD) xs = x[m];
+      by_raw[m] = dstep_of(raw, p.softplus);
       if (gated) {
-        const float s = sigmoidf_(z.v[m]), g = z.v[m] * s;
+        const float zs = z[m], s = sigmoidf_(zs), g = zs * s;
         by_y[m] = dy * fmaf(g, 1.f - s, s);
         dy *= g;
       }
-      pass.of_channel[0][at.j][4 * m + at.q] = step;
-      pass.of_channel[1][at.j][4 * m + at.q] = dy;
+      pass.of_channel[4 * m + at.q][at.j] = f32x4_t{step, dy, step * xs, xs};
       if constexpr (FOLD) sum += step;
-      else pass.of_channel[2][at.j][4 * m + at.q] = step * xs[m];
     }
     if constexpr (!FOLD) B.pass(pass.of_token[0], at);
     C.pass(pass.of_token[1], at);
     passed();
+    // a token's numbers are on their way while the one in front is worked on; the fences keep the compiler from reading further ahead, for which there are no registers
+    constexpr int kAhead = CN <= 4 ? 2 : 1;
+    Token<CN> ahead[kAhead];
     if constexpr (FOLD) {
       if (first > at.first) load(first - T);
+      if (kAhead > 1) ahead[(T - 1) % kAhead].read(pass, T - 1, at, false);
 #pragma unroll
-      for (int m = R - 1; m >= 0; --m) {
-        float step[4], d[4];
-        read_lds(step, &pass.of_channel[0][at.j][4 * m]);
-        read_lds(d, &pass.of_channel[1][at.j][4 * m]);
+      for (int t = T - 1; t >= 0; --t) {
+        if (kAhead == 1) ahead[0].read(pass, t, at, false);
+        else if (t > 0) ahead[(t - 1) % kAhead].read(pass, t - 1, at, false);
+        const Token<CN>& now = ahead[t % kAhead];
 #pragma unroll
-        for (int k = 3; k >= 0; --k) {
-          float c[CN];
-          read_lds(c, &pass.of_token[1][4 * m + k][at.q * CN]);
-#pragma unroll
-          for (int i = 0; i < CN; ++i) back[i] = __builtin_amdgcn_exp2f(step[k] * A[i]) * fmaf(c[i], d[k], back[i]);
-        }
+        for (int i = 0; i < CN; ++i) back[i] = __builtin_amdgcn_exp2f(now.of[0] * A[i]) * fmaf(now.c[i], now.of[1], back[i]);
       }
       passed();
     } else {
@@ -117,92 +147,90 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
       constexpr int TT = CN >= 8 ? 1 : 8 / CN, NN = CN >= 8 ? 8 : CN;
       auto shared = [&](const float (&v)[8], int which, int token, int state) {
         float s[2];
-        of_channels(v, s, at.j);
+        of_channels(v, s);
         const int i = at.j & 1, e = i + 2 * (at.j >> 2 & 1) + 4 * (at.j >> 3);
         board.v[which][token + e / NN][at.q * CN + state + e % NN] = i ? s[1] : s[0];
       };
-      float h[CN], a[T][CN], ph[T][CN];
-      kept_states(h, p.kept, (size_t)at.b * tiles + first / T, p.D, at);
+      float h[CN], a[T][CN], ph[T][CN], few[8], of_four[4];
+      if constexpr (CN > 4) states.load(kept, p.kept, (size_t)at.b * tiles + first / T, p.D);
+#pragma unroll
+      for (int i = 0; i < CN; ++i) h[i] = kept[i];
       // forward again
-      float few[8];
+      if (kAhead > 1) ahead[0].read(pass, 0, at, true);
 #pragma unroll
-      for (int m = 0; m < R; ++m) {
+      for (int t = 0; t < T; ++t) {
         __builtin_amdgcn_sched_barrier(0);
-        float step[4], d[4], u[4], s[4];
-        read_lds(step, &pass.of_channel[0][at.j][4 * m]);
-        read_lds(d, &pass.of_channel[1][at.j][4 * m]);
-        read_lds(u, &pass.of_channel[2][at.j][4 * m]);
+        if (kAhead == 1) ahead[0].read(pass, t, at, true);
+        else if (t + 1 < T) ahead[(t + 1) % kAhead].read(pass, t + 1, at, true);
+        const Token<CN>& now = ahead[t % kAhead];
+        of_four[t % 4] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = 4 * m + k;
-          if constexpr (CN >= 8) __builtin_amdgcn_sched_barrier(0);
-          float b[CN], c[CN];
-          read_lds(b, &pass.of_token[0][t][at.q * CN]);
-          read_lds(c, &pass.of_token[1][t][at.q * CN]);
-          s[k] = 0.f;
-#pragma unroll
-          for (int i = 0; i < CN; ++i) {
-            a[t][i] = __builtin_amdgcn_exp2f(step[k] * A[i]);
-            ph[t][i] = a[t][i] * h[i];
-            h[i] = fmaf(u[k], b[i], ph[t][i]);
-            s[k] = fmaf(c[i], h[i], s[k]);
-            few[t % TT * NN + i % 8] = d[k] * h[i];
-            if (t % TT == TT - 1 && i % 8 == NN - 1) shared(few, 1, t - (TT - 1), i - (NN - 1));
-          }
+        for (int i = 0; i < CN; ++i) {
+          a[t][i] = __builtin_amdgcn_exp2f(now.of[0] * A[i]);
+          ph[t][i] = a[t][i] * h[i];
+          h[i] = fmaf(now.of[2], now.b[i], ph[t][i]);
+          of_four[t % 4] = fmaf(now.c[i], h[i], of_four[t % 4]);
+          few[t % TT * NN + i % 8] = now.of[1] * h[i];
+          if (t % TT == TT - 1 && i % 8 == NN - 1) shared(few, 1, t - (TT - 1), i - (NN - 1));
         }
-        if (gated) dz.store(tile, m, by_y[m] * fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3])));
+        if (t % 4 == 3 && gated) {
+          const int m = t / 4;
+          dz.store(tile, m, by_y[m] * fmaf(skip, pass.of_channel[4 * m + at.q][at.j][3], of_rows(of_four[0], of_four[1], of_four[2], of_four[3])));
+        }
       }
       // and back
+      float of_du[4];
+      if (kAhead > 1) ahead[(T - 1) % kAhead].read(pass, T - 1, at, true);
 #pragma unroll
-      for (int m = R - 1; m >= 0; --m) {
+      for (int t = T - 1; t >= 0; --t) {
         __builtin_amdgcn_sched_barrier(0);
-        float step[4], d[4], u[4], du[4], dd[4];
-        read_lds(step, &pass.of_channel[0][at.j][4 * m]);
-        read_lds(d, &pass.of_channel[1][at.j][4 * m]);
-        read_lds(u, &pass.of_channel[2][at.j][4 * m]);
+        if (kAhead == 1) ahead[0].read(pass, t, at, true);
+        else if (t > 0) ahead[(t - 1) % kAhead].read(pass, t - 1, at, true);
+        const Token<CN>& now = ahead[t % kAhead];
+        of_du[t % 4] = of_four[t % 4] = 0.f;
 #pragma unroll
-        for (int k = 3; k >= 0; --k) {
-          const int t = 4 * m + k;
-          if constexpr (CN >= 8) __builtin_amdgcn_sched_barrier(0);
-          float b[CN], c[CN];
-          read_lds(b, &pass.of_token[0][t][at.q * CN]);
-          read_lds(c, &pass.of_token[1][t][at.q * CN]);
-          du[k] = dd[k] = 0.f;
-#pragma unroll
-          for (int i = 0; i < CN; ++i) {
-            const float dh = fmaf(c[i], d[k], back[i]), e = dh * ph[t][i];
-            du[k] = fmaf(b[i], dh, du[k]);
-            dd[k] = fmaf(A[i], e, dd[k]);
-            dA[i] = fmaf(step[k], e, dA[i]);
-            back[i] = a[t][i] * dh;
-            few[t % TT * NN + i % 8] = dh * u[k];
-            if (t % TT == 0 && i % 8 == NN - 1) shared(few, 0, t, i - (NN - 1));
-          }
+        for (int i = 0; i < CN; ++i) {
+          const float dh = fmaf(now.c[i], now.of[1], back[i]), e = dh * ph[t][i];
+          of_du[t % 4] = fmaf(now.b[i], dh, of_du[t % 4]);
+          of_four[t % 4] = fmaf(A[i], e, of_four[t % 4]);
+          dA[i] = fmaf(now.of[0], e, dA[i]);
+          back[i] = a[t][i] * dh;
+          few[t % TT * NN + i % 8] = dh * now.of[2];
+          if (t % TT == 0 && i % 8 == NN - 1) shared(few, 0, t, i - (NN - 1));
         }
-        const float du_m = of_rows(du[0], du[1], du[2], du[3]), dd_m = of_rows(dd[0], dd[1], dd[2], dd[3]);
-        const float dy = pass.of_channel[1][at.j][4 * m + at.q];
-        const float ds = fmaf(xs[m], du_m, dd_m * kLn2) * dstep_of(raw[m], p.softplus);
-        dx.store(tile, m, fmaf(pass.of_channel[0][at.j][4 * m + at.q], du_m, skip * dy));
-        ddelta.store(tile, m, ds);
-        if (first + 4 * m + at.q < at.end) dbias += ds, dskip = fmaf(dy, xs[m], dskip);
-        // (the next tile's rows, into registers that the last tokens' factors have left)
-        if (m == R - 1 && first > at.first) load(first - T);
+        if (t % 4 == 0) {
+          const int m = t / 4;
+          const float du = of_rows(of_du[0], of_du[1], of_du[2], of_du[3]), dd = of_rows(of_four[0], of_four[1], of_four[2], of_four[3]);
+          const f32x4_t own = pass.of_channel[4 * m + at.q][at.j];
+          const float ds = fmaf(own[3], du, dd * kLn2) * by_raw[m];
+          dx.store(tile, m, fmaf(own[0], du, skip * own[1]));
+          ddelta.store(tile, m, ds);
+          if (first + 4 * m + at.q < at.end) dbias += ds, dskip = fmaf(own[1], own[3], dskip);
+          // (the next tile's rows, into registers that the last tokens' factors have left)
+          if (m == R - 1 && first > at.first) load(first - T);
+        }
       }
       // the workgroup's sums (the other turn's are read until the next barrier)
       __syncthreads();
-      const size_t rows = (((size_t)at.b * p.G + at.g) * p.blocks + at.block) * p.L;
-      for (int e = threadIdx.x; e < 2 * T * NP; e += 64 * kScanWaves) {
-        const int n = e % NP, which = e / NP % 2, t = first + e / (2 * NP);
-        if (t >= at.end) break;
-        float s = 0.f;
+      constexpr int kSums = 2 * T * NP, kThreads = 64 * kScanWaves;
+      const size_t rows = (((size_t)at.b * p.G + at.g) * p.blocks + at.block) * p.L + tile.lowest;
+      const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(p.shared + rows * 2 * NP, 0, tile.rows * 2 * NP * (int)sizeof(float), 0x00020000);
 #pragma unroll
-        for (int w = 0; w < kScanWaves; ++w) s += boards[turn][w].v[which][t - first][n];
-        p.shared[((rows + (p.reverse ? p.L - 1 - t : t)) * 2 + which) * NP + n] = s;
+      for (int k = 0; k < (kSums + kThreads - 1) / kThreads; ++k) {
+        const int e = threadIdx.x + k * kThreads, n = e % NP, which = e / NP % 2, t = e / (2 * NP);
+        float s = 0.f;
+        if (kSums % kThreads == 0 || e < kSums) {
+#pragma unroll
+          for (int w = 0; w < kScanWaves; ++w) s += boards[turn][w].v[which][t][n];
+        }
+        // (tokens behind the end lie outside the descriptor; so do numbers behind the tile's)
+        const unsigned to = (unsigned)(((tile.from + tile.step * t) * 2 + which) * NP + n) * sizeof(float);
+        store1(r, kSums % kThreads == 0 || e < kSums ? to : kNowhere, s, 0.f);
       }
     }
   }
   if constexpr (FOLD) {
-    keep_states(p.ends, back, row, p.D, at);
+    states.store(p.ends, row, p.D, back);
     sum = of_all_rows(sum);
     if (at.q == 0 && at.has) p.sums[row * p.D + at.c] = sum;
   } else {
