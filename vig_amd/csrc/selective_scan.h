@@ -154,11 +154,11 @@ __device__ __forceinline__ float of_all_rows(float s) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A wave's LDS: of a tile each channel's values along the tokens (K of them), each token's B and C.
-template <int CN, int K> struct Pass {
-  static constexpr int T = kTileTokens<CN>, kPitch = T + 4, NP = 4 * CN;
-  float of_channel[K][16][kPitch];
-  float of_token[2][T][NP];
+// A wave's LDS: of a tile four numbers of each token and channel side by side, each token's B and C.
+template <int CN> struct Pass {
+  static constexpr int T = kTileTokens<CN>;
+  f32x4_t of_channel[T][16];
+  float of_token[2][T][4 * CN];
 };
 // what other lanes of the wave wrote is read behind this
 __device__ __forceinline__ void passed() {

@@ -13,11 +13,11 @@ namespace {
 // ---- forward.  FOLD: only what a chunk of tokens leaves from nothing, and the sum of its steps
 
 template <typename S, int CN, bool FOLD>
-__global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScanArgs p) {
+__global__ __launch_bounds__(64 * kScanWaves, CN > 4 ? 4 : FOLD ? 8 : 7) void selective_scan_kernel(SelScanArgs p) {
   constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN;
-  __shared__ __align__(16) Pass<CN, 2> lds[kScanWaves];
+  __shared__ __align__(16) Pass<CN> lds[kScanWaves];
   const Stand at(p);
-  Pass<CN, 2>& pass = lds[at.wave];
+  Pass<CN>& pass = lds[at.wave];
   const float bias = p.bias && at.has ? p.bias[at.c] : 0.f, skip = p.skip && at.has ? p.skip[at.c] : 0.f;
   float A[CN], h[CN];
   load_states(A, p.A, 0, p.D, p.N, p.N, at);
@@ -29,11 +29,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) h[i] = 0.f;
-  } else if (p.chunks > kFewChunks) {
-    kept.load(h, p.ends, row, p.D);
-  } else {
-    load_states(h, p.h0, at.b, p.D, p.N, p.N, at);
-    entering<false>(h, A, p, at);
   }
   const bool gated = !FOLD && p.z.at;
   float sum = 0.f;
@@ -49,15 +44,26 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     if (gated) z.load(tile);
   };
   load(at.first);
+  if constexpr (!FOLD) {  // (behind the first rows' loads, which are on their way meanwhile)
+    if (p.chunks > kFewChunks) {
+      kept.load(h, p.ends, row, p.D);
+    } else {
+      load_states(h, p.h0, at.b, p.D, p.N, p.N, at);
+      entering<false>(h, A, p, at);
+    }
+  }
   for (int first = at.first; first < at.end; first += T) {
     const Tile<T> tile(p, first, at.end);
-    float xs[R], zs[R];
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const float step = first + 4 * m + at.q < at.end ? step_of(delta[m] + bias, p.softplus) : 0.f;
-      xs[m] = x[m], zs[m] = z[m];
-      pass.of_channel[0][at.j][4 * m + at.q] = step;
-      pass.of_channel[1][at.j][4 * m + at.q] = step * x[m];
+      const float step = first + 4 * m + at.q < at.end ? step_of(delta[m] + bias, p.softplus) : 0.f, xs = x[m];
+      f32x4_t of = {step, step * xs, skip * xs, 1.f};
+      if constexpr (!FOLD)
+        if (gated) {
+          const float zs = z[m];
+          of[3] = zs * sigmoidf_(zs);
+        }
+      pass.of_channel[4 * m + at.q][at.j] = of;
       if constexpr (FOLD) sum += step;
     }
     B.pass(pass.of_token[0], at);
@@ -66,28 +72,35 @@ __global__ __launch_bounds__(64 * kScanWaves) void selective_scan_kernel(SelScan
     if (first + T < at.end) load(first + T);
     if constexpr (!FOLD)
       if (p.kept) kept.store(p.kept, (size_t)at.b * tiles + first / T, p.D, h);
+    // a token's numbers are on their way while the one in front is worked on; the fences keep the compiler from reading further ahead, which would cost a wave a SIMD
+    struct Token {
+      f32x2_t of;
+      float b[CN], c[CN];
+    } ahead[2];
+    auto read = [&](int t) {
+      Token& to = ahead[t % 2];
+      to.of = *reinterpret_cast<const f32x2_t*>(&pass.of_channel[t][at.j]);
+      read_lds(to.b, &pass.of_token[0][t][at.q * CN]);
+      if constexpr (!FOLD) read_lds(to.c, &pass.of_token[1][t][at.q * CN]);
+    };
+    float s[4];
+    read(0);
 #pragma unroll
-    for (int m = 0; m < R; ++m) {
-      float step[4], u[4], s[4];
-      read_lds(step, &pass.of_channel[0][at.j][4 * m]);
-      read_lds(u, &pass.of_channel[1][at.j][4 * m]);
+    for (int t = 0; t < T; ++t) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 1 < T) read(t + 1);
+      const Token& now = ahead[t % 2];
+      s[t % 4] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float b[CN], c[CN];
-        read_lds(b, &pass.of_token[0][4 * m + k][at.q * CN]);
-        if constexpr (!FOLD) read_lds(c, &pass.of_token[1][4 * m + k][at.q * CN]);
-        s[k] = 0.f;
-#pragma unroll
-        for (int i = 0; i < CN; ++i) {
-          h[i] = fmaf(u[k], b[i], __builtin_amdgcn_exp2f(step[k] * A[i]) * h[i]);
-          if constexpr (!FOLD) s[k] = fmaf(c[i], h[i], s[k]);
+      for (int i = 0; i < CN; ++i) {
+        h[i] = fmaf(now.of[1], now.b[i], __builtin_amdgcn_exp2f(now.of[0] * A[i]) * h[i]);
+        if constexpr (!FOLD) s[t % 4] = fmaf(now.c[i], h[i], s[t % 4]);
+      }
+      if constexpr (!FOLD)
+        if (t % 4 == 3) {
+          const f32x4_t own = pass.of_channel[t - 3 + at.q][at.j];
+          out.store(tile, t / 4, (of_rows(s[0], s[1], s[2], s[3]) + own[2]) * own[3]);
         }
-      }
-      if constexpr (!FOLD) {
-        float y = fmaf(skip, xs[m], of_rows(s[0], s[1], s[2], s[3]));
-        if (gated) y *= zs[m] * sigmoidf_(zs[m]);
-        out.store(tile, m, y);
-      }
     }
     passed();
   }
@@ -241,15 +254,15 @@ static int run_step(SelScanStep& p, hipStream_t stream) {
   hipLaunchKernelGGL((selective_step_kernel<S, NL, WHOLE, ROWS>), dim3((unsigned)groups), dim3(256), 0, stream, p);
   return hipGetLastError() == hipSuccess ? 0 : -5;
 }
-// Four sequences a thread once that leaves four workgroups a compute unit
+// Two sequences a thread once that leaves four workgroups a compute unit
 template <typename S, int NL>
 static int step_rows(SelScanStep& p, hipStream_t stream) {
   auto on = [](const void* t, size_t bytes) { return reinterpret_cast<uintptr_t>(t) % bytes == 0; };
   bool whole = p.N % 4 == 0 && on(p.state, 16) && on(p.A, 16) && on(p.B, 4 * sizeof(S)) && on(p.C, 4 * sizeof(S));
   for (int k = 0; k < 2; ++k) whole = whole && p.B_strides[k] % 4 == 0 && p.C_strides[k] % 4 == 0;
-  const bool many = (long long)p.batch * p.D * NL / (4 * 256) >= 1024;
-  if (whole) return many ? run_step<S, NL, true, 4>(p, stream) : run_step<S, NL, true, 1>(p, stream);
-  return many ? run_step<S, NL, false, 4>(p, stream) : run_step<S, NL, false, 1>(p, stream);
+  const bool many = (long long)p.batch * p.D * NL / (2 * 256) >= 1024;
+  if (whole) return many ? run_step<S, NL, true, 2>(p, stream) : run_step<S, NL, true, 1>(p, stream);
+  return many ? run_step<S, NL, false, 2>(p, stream) : run_step<S, NL, false, 1>(p, stream);
 }
 
 int launch_selective_scan_step(SelScanStep& p, hipStream_t stream) {

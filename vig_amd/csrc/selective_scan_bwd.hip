@@ -46,17 +46,11 @@ template <int CN> struct Board {
   float v[2][kTileTokens<CN>][4 * CN];
 };
 
-// A wave's LDS: of a tile each channel's step, dy, step times x and x of a token side by side, each token's B and C.
-template <int CN> struct BackPass {
-  static constexpr int T = kTileTokens<CN>;
-  f32x4_t of_channel[T][16];
-  float of_token[2][T][4 * CN];
-};
-// ... as a lane reads them of a token
+// What a lane reads of a token: its channel's step, dy, step times x and x, B and C
 template <int CN> struct Token {
   f32x4_t of;
   float b[CN], c[CN];
-  __device__ __forceinline__ void read(const BackPass<CN>& pass, int t, const Stand& at, bool both) {
+  __device__ __forceinline__ void read(const Pass<CN>& pass, int t, const Stand& at, bool both) {
     of = pass.of_channel[t][at.j];
     if (both) read_lds(b, &pass.of_token[0][t][at.q * CN]);
     read_lds(c, &pass.of_token[1][t][at.q * CN]);
@@ -67,10 +61,10 @@ template <int CN> struct Token {
 template <typename S, int CN, bool FOLD>
 __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_bwd_kernel(SelScanArgs p) {
   constexpr int T = kTileTokens<CN>, R = T / 4, NP = 4 * CN;
-  __shared__ __align__(16) BackPass<CN> lds[kScanWaves];
+  __shared__ __align__(16) Pass<CN> lds[kScanWaves];
   __shared__ __align__(16) Board<CN> boards[FOLD ? 1 : 2][FOLD ? 1 : kScanWaves];
   const Stand at(p);
-  BackPass<CN>& pass = lds[at.wave];
+  Pass<CN>& pass = lds[at.wave];
   const float bias = p.bias && at.has ? p.bias[at.c] : 0.f, skip = p.skip && at.has ? p.skip[at.c] : 0.f;
   float A[CN], back[CN];  // back: a dh of the token behind
   load_states(A, p.A, 0, p.D, p.N, p.N, at);
@@ -81,11 +75,6 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   if constexpr (FOLD) {
 #pragma unroll
     for (int i = 0; i < CN; ++i) back[i] = 0.f;
-  } else if (p.chunks > kFewChunks) {
-    states.load(back, p.ends, row, p.D);
-  } else {
-    load_states(back, p.dhT, at.b, p.D, p.N, p.N, at);
-    entering<true>(back, A, p, at);
   }
   const bool gated = p.z.at;
   float sum = 0.f, dskip = 0.f, dbias = 0.f, dA[CN];
@@ -106,6 +95,14 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
     if constexpr (!FOLD && CN <= 4) states.load(kept, p.kept, (size_t)at.b * tiles + first / T, p.D);  // (more of them have no room)
   };
   load(last);
+  if constexpr (!FOLD) {  // (behind the first rows' loads, which are on their way meanwhile)
+    if (p.chunks > kFewChunks) {
+      states.load(back, p.ends, row, p.D);
+    } else {
+      load_states(back, p.dhT, at.b, p.D, p.N, p.N, at);
+      entering<true>(back, A, p, at);
+    }
+  }
   for (int first = last, turn = 0; first >= at.first; first -= T, turn ^= 1) {
     [[maybe_unused]] const Tile<T> tile(p, first, at.end);
     float by_raw[R], by_y[R];  // what makes gradients of raw steps of those of steps, and dz of y
@@ -245,20 +242,30 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   }
 }
 
-// dB, dC [B, L, G, N]: the sums over a group's workgroups
+// dB, dC [B, L, G, N]: the sums over a group's workgroups.  A thread takes four states of a token's dB or dC, four workgroups' on their way together.
 template <typename S>
 __global__ __launch_bounds__(256) void selective_shared_kernel(SelScanArgs p, int np) {
-  const long long each = (long long)p.L * 2 * np, id = (long long)blockIdx.x * 256 + threadIdx.x;  // a thread: group, token, which, state
+  constexpr int K = 4;
+  const long long each = (long long)p.L * 2 * np, id = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;  // of a group: token, which, state
   if (id >= each * p.batch * p.G) return;
   const long long bg = id / each, in = id - bg * each;
   const int n = (int)(in % np), which = (int)(in / np % 2);
   const long long t = in / (2 * np);
   if (n >= p.N) return;
   const float* from = p.shared + bg * p.blocks * each + in;
-  float s = 0.f;
-  for (int k = 0; k < p.blocks; ++k) s += from[k * each];
+  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < p.blocks; k0 += K) {
+    f32x4_t v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = k0 + k < p.blocks ? *reinterpret_cast<const f32x4_t*>(from + (k0 + k) * each) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) s += v[k];
+  }
   const long long b = bg / p.G;
-  Elem<S>::store(static_cast<S*>(which ? p.dC : p.dB) + ((b * p.L + t) * p.G + (bg - b * p.G)) * p.N + n, s);
+  S* const to = static_cast<S*>(which ? p.dC : p.dB) + ((b * p.L + t) * p.G + (bg - b * p.G)) * p.N + n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.N) Elem<S>::store(to + i, s[i]);
 }
 
 }  // namespace
@@ -273,7 +280,7 @@ static int run_backward(const SelScanArgs& p, hipStream_t stream) {
   }
   hipLaunchKernelGGL((selective_scan_bwd_kernel<S, CN, false>), grid, block, 0, stream, p);
   const long long n = (long long)p.batch * p.G * p.L * 8 * CN;
-  hipLaunchKernelGGL((selective_shared_kernel<S>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, p, 4 * CN);
+  hipLaunchKernelGGL((selective_shared_kernel<S>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, p, 4 * CN);
   if (hipGetLastError() != hipSuccess) return -5;
   vig_sum_jobs sums{};
   if (!put_off(sums, p.params, p.dparams, p.batch * p.chunks, (long long)p.D * (p.N + 2), false)) return -22;
