@@ -41,12 +41,12 @@ template <typename F> int by_states(int CN, F f) {
     default: return f(std::integral_constant<int, 16>{});
   }
 }
-// Chunks of tokens: none where the sequences and channels alone fill the chip.
+// Chunks of tokens, 16 at least: none where the sequences and channels alone fill the chip.
 inline void cut_chunks(SelScanArgs& p) {
   const int T = scan_tile(scan_states(p.N));
   p.of_group = p.D / p.G, p.blocks = (p.of_group + kScanBlock - 1) / kScanBlock;
   const long long groups = (long long)p.batch * p.G * p.blocks;
-  const long long want = std::max(1LL, std::min<long long>(kScanGroups / std::min<long long>(groups, kScanGroups), (p.L + T - 1) / T));
+  const long long want = std::max(1LL, std::min<long long>(kScanGroups / std::min<long long>(groups, kScanGroups), (p.L + 15) / 16));
   p.chunk = (int)(((p.L + want - 1) / want + T - 1) / T * T);
   p.chunks = (p.L + p.chunk - 1) / p.chunk;
 }

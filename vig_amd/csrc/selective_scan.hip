@@ -87,6 +87,7 @@ __global__ __launch_bounds__(64 * kScanWaves, CN > 4 ? 4 : FOLD ? 8 : 7) void se
     read(0);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
+      if (t % 4 == 0 && t >= tile.rows) break;  // (a last tile's tokens that are not there, by fours)
       __builtin_amdgcn_sched_barrier(0);
       if (t + 1 < T) read(t + 1);
       const Token& now = ahead[t % 2];

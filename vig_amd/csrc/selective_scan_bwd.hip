@@ -133,6 +133,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
       for (int t = T - 1; t >= 0; --t) {
         if (kAhead == 1) ahead[0].read(pass, t, at, false);
         else if (t > 0) ahead[(t - 1) % kAhead].read(pass, t - 1, at, false);
+        if (t / 4 * 4 >= tile.rows) continue;  // (a last tile's tokens that are not there, by fours)
         const Token<CN>& now = ahead[t % kAhead];
 #pragma unroll
         for (int i = 0; i < CN; ++i) back[i] = __builtin_amdgcn_exp2f(now.of[0] * A[i]) * fmaf(now.c[i], now.of[1], back[i]);
@@ -148,6 +149,9 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
         const int i = at.j & 1, e = i + 2 * (at.j >> 2 & 1) + 4 * (at.j >> 3);
         board.v[which][token + e / NN][at.q * CN + state + e % NN] = i ? s[1] : s[0];
       };
+      // A last tile's tokens that are not there are left out by fours where a lane has eight states and more: the blocks that this makes need no spilled registers then (45 and 137 without).
+      // Up to four they are gone through with steps of 0: blocks cost 303 us for 278 there (128 x 196 x 768, 16 states, 13 tiles of which the last is a quarter).
+      constexpr bool kSkip = CN >= 8;
       float h[CN], a[T][CN], ph[T][CN], few[8], of_four[4];
       if constexpr (CN > 4) states.load(kept, p.kept, (size_t)at.b * tiles + first / T, p.D);
 #pragma unroll
@@ -156,6 +160,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
       if (kAhead > 1) ahead[0].read(pass, 0, at, true);
 #pragma unroll
       for (int t = 0; t < T; ++t) {
+        if (kSkip && t % 4 == 0 && t >= tile.rows) break;
         __builtin_amdgcn_sched_barrier(0);
         if (kAhead == 1) ahead[0].read(pass, t, at, true);
         else if (t + 1 < T) ahead[(t + 1) % kAhead].read(pass, t + 1, at, true);
@@ -183,6 +188,10 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
         __builtin_amdgcn_sched_barrier(0);
         if (kAhead == 1) ahead[0].read(pass, t, at, true);
         else if (t > 0) ahead[(t - 1) % kAhead].read(pass, t - 1, at, true);
+        if (kSkip && t / 4 * 4 >= tile.rows) {
+          if (t == T - 4 && first > at.first) load(first - T);
+          continue;
+        }
         const Token<CN>& now = ahead[t % kAhead];
         of_du[t % 4] = of_four[t % 4] = 0.f;
 #pragma unroll
