@@ -4,7 +4,10 @@
 //   dpre_t = dy_t (silu'(pre_t)),   dx_t = sum_k w[k] dpre_{t + W - 1 - k} (+ the final state's gradient),   dw[k] = sum_t dpre_t x_{t - W + 1 + k},   dbias = sum_t dpre_t
 //
 // Memory bounds it: a thread slides over a run of tokens of a few channels, so that a row is read once but for the W - 1 rows on a run's edges, which come out of a
-// cache.  Sixteen threads side by side take 128 bytes of a row.
+// cache.  Sixteen threads side by side take 256 bytes of a row (128 in the backward, which has twice the registers to hold).
+//
+// Measured, bf16, 4 taps, silu: 65536 x 1024 53 us, 5.1 TB/s (a large copy: 5.4); 128 x 196 x 768 forward 22, backward 34 (116 MB, part of it in the 256 MB cache; 35 operations an
+// element beside it), sums of the weights' gradient 4.
 #include "common.h"
 #include "launch.h"
 
@@ -137,7 +140,8 @@ __device__ __forceinline__ void state_row(float (&x)[V], const CausalConv& p, in
   }
 }
 
-// Tokens whose rows are on their way together: the next ones' while a thread works on these
+// Tokens whose rows are on their way together: the next ones' while a thread works on these.  us, 65536 x 1024 forward / 128 x 196 x 768 backward: two 53 / 34, four 55 / 34, eight 59 / 42 (170
+// registers, two waves a SIMD).
 constexpr int kConvTokens = 2;
 
 template <typename T, int V, int W>
@@ -360,7 +364,7 @@ template <int BYTES, typename F> int by_case(const CausalConv& p, int io_dtype, 
     return whole(p, BYTES, 4) ? f(float{}, std::integral_constant<int, BYTES / 4>{}, w) : f(float{}, std::integral_constant<int, 1>{}, w);
   });
 }
-// Runs of tokens: as long as leaves four workgroups a compute unit, so that few rows on their edges are read twice.
+// Runs of tokens: as long as leaves four workgroups a compute unit (and `most`), so that few rows on their edges are read twice.
 void cut_runs(CausalConv& p, int V, int most) {
   p.blocks = (p.D + kConvLanes * V - 1) / (kConvLanes * V);
   const long long tokens = (long long)p.B * p.blocks * p.L / (kConvRuns * 1024);

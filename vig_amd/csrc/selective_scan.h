@@ -21,7 +21,7 @@ typedef __amdgpu_buffer_rsrc_t rsrc_t;
 constexpr unsigned kNowhere = 0x40000000u;  // byte offset behind every descriptor here (sixteen rows of kScanRow elements at most)
 constexpr int kScanWaves = 4;               // of a workgroup, on channels side by side
 constexpr int kScanBlock = 16 * kScanWaves; // channels of a workgroup
-constexpr int kScanGroups = 1024;           // workgroups that sequences are cut for
+constexpr int kScanUnits = 256;             // compute units that they fill
 
 // tokens of a tile (the backward keeps two numbers a state and token in registers: 128 of them at most)
 constexpr int scan_tile(int CN) { return CN <= 4 ? 16 : 64 / CN; }
@@ -41,12 +41,14 @@ template <typename F> int by_states(int CN, F f) {
     default: return f(std::integral_constant<int, 16>{});
   }
 }
-// Chunks of tokens, 16 at least: none where the sequences and channels alone fill the chip.
+// Chunks of tokens, 16 at least: none where sequences and channels leave no compute unit without a workgroup.  Chunks cost a second walk without the outputs, two thirds of the first; what they
+// give is four workgroups a unit, whose waves hide one another's waits.  65536 x 1024, fold and walk: four a unit 229 + 305 us, two 248 + 367, one 331 + 536.  So with 256 groups of channels
+// already four chunks cost as much as one; 32 x 12 groups of 196 tokens, 64 states: one chunk 103 us, two 140.
 inline void cut_chunks(SelScanArgs& p) {
-  const int T = scan_tile(scan_states(p.N));
   p.of_group = p.D / p.G, p.blocks = (p.of_group + kScanBlock - 1) / kScanBlock;
   const long long groups = (long long)p.batch * p.G * p.blocks;
-  const long long want = std::max(1LL, std::min<long long>(kScanGroups / std::min<long long>(groups, kScanGroups), (p.L + 15) / 16));
+  const long long want = groups >= kScanUnits ? 1 : std::min<long long>(4 * kScanUnits / groups, (p.L + 15) / 16);
+  const int T = scan_tile(scan_states(p.N));
   p.chunk = (int)(((p.L + want - 1) / want + T - 1) / T * T);
   p.chunks = (p.L + p.chunk - 1) / p.chunk;
 }

@@ -4,7 +4,16 @@
 //   h_t[n] = e^{s_t A[n]} h_{t-1}[n] + s_t x_t B_t[n]                  N numbers a channel; B, C of a token shared by the channels of a group
 //   o_t = (sum_n C_t[n] h_t[n] + skip x_t) silu(z_t)
 //
-// Decays go by channel and state, so that no product of matrices is in it: for each number of state and token one exponential, four multiply-adds and a product.
+// Decays go by channel and state, so that no product of matrices is in it: for each number of state and token an exponential (two issue slots), a product for its exponent, one for
+// the decay and two multiply-adds.  The vector pipe bounds it: 500 instructions a wave, tile of 16 tokens, 16 channels and 16 states, 320 of them these (64 of them double), the others
+// the steps' softplus (80), gates, addresses and sums over the lane rows.  Sums over n stay in a lane for its four states, and h never leaves its registers.
+//
+// Sequences go through uncut where they give every compute unit a workgroup; else in chunks of tokens: a launch folds each (the state that it leaves from nothing, and the sum of its
+// steps, which is all that a decay over it takes), and the chunks are joined by the walk itself or, many of them, by a launch in between.
+//
+// Measured, bf16, 16 states, gate: 128 x 196 x 768 86 us (4.6 M numbers of state a us; the rows alone, 156 MB, 29 at the rate of a copy; vector pipe 83 % busy, 6 waves a SIMD), 65536 x 1024
+// fold 229, join 10, walk 305.  Tried: the products s x B as outer products of the matrix cores (16 blocks of 4 x 4): 88 cycles for 84 beside the arithmetic of a token,
+// which they do not run beside.  A softplus of fewer instructions for bf16 rows: no gain, and states of less precision.
 #include "selective_scan.h"
 
 namespace vig {
@@ -73,24 +82,26 @@ __global__ __launch_bounds__(64 * kScanWaves, CN > 4 ? 4 : FOLD ? 8 : 7) void se
     if constexpr (!FOLD)
       if (p.kept) kept.store(p.kept, (size_t)at.b * tiles + first / T, p.D, h);
     // a token's numbers are on their way while the one in front is worked on; the fences keep the compiler from reading further ahead, which would cost a wave a SIMD
+    constexpr int kAhead = CN <= 8 ? 2 : 1;
     struct Token {
       f32x2_t of;
       float b[CN], c[CN];
-    } ahead[2];
+    } ahead[kAhead];
     auto read = [&](int t) {
-      Token& to = ahead[t % 2];
+      Token& to = ahead[t % kAhead];
       to.of = *reinterpret_cast<const f32x2_t*>(&pass.of_channel[t][at.j]);
       read_lds(to.b, &pass.of_token[0][t][at.q * CN]);
       if constexpr (!FOLD) read_lds(to.c, &pass.of_token[1][t][at.q * CN]);
     };
     float s[4];
-    read(0);
+    if (kAhead > 1) read(0);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       if (t % 4 == 0 && t >= tile.rows) break;  // (a last tile's tokens that are not there, by fours)
       __builtin_amdgcn_sched_barrier(0);
-      if (t + 1 < T) read(t + 1);
-      const Token& now = ahead[t % 2];
+      if (kAhead == 1) read(t);
+      else if (t + 1 < T) read(t + 1);
+      const Token& now = ahead[t % kAhead];
       s[t % 4] = 0.f;
 #pragma unroll
       for (int i = 0; i < CN; ++i) {
