@@ -63,9 +63,13 @@ __global__ __launch_bounds__(64 * kScanWaves, CN > 4 ? 4 : FOLD ? 8 : 7) void se
   }
   for (int first = at.first; first < at.end; first += T) {
     const Tile<T> tile(p, first, at.end);
+    float steps[R];
+#pragma unroll
+    for (int m = 0; m < R; ++m) steps[m] = step_of(delta[m] + bias, p.softplus);
+    if (tile.rows < T) leave_out<R>(steps, tile.rows, at);
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const float step = first + 4 * m + at.q < at.end ? step_of(delta[m] + bias, p.softplus) : 0.f, xs = x[m];
+      const float step = steps[m], xs = x[m];
       f32x4_t of = {step, step * xs, skip * xs, 1.f};
       if constexpr (!FOLD)
         if (gated) {

@@ -111,13 +111,19 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
   }
   for (int first = last, turn = 0; first >= at.first; first -= T, turn ^= 1) {
     [[maybe_unused]] const Tile<T> tile(p, first, at.end);
-    float by_raw[R], by_y[R];  // what makes gradients of raw steps of those of steps, and dz of y
+    float by_raw[R], by_y[R], steps[R];  // what makes gradients of raw steps of those of steps, and dz of y
 #pragma unroll
     for (int m = 0; m < R; ++m) {
-      const float raw = delta[m] + bias, step = first + 4 * m + at.q < at.end ? step_of(raw, p.softplus) : 0.f;
+      const float raw = delta[m] + bias;
+      steps[m] = step_of(raw, p.softplus), by_raw[m] = dstep_of(raw, p.softplus);
+    }
+    // (a token that is not there has no share in the bias's gradient either)
+    if (tile.rows < T) leave_out<R>(steps, tile.rows, at), leave_out<R>(by_raw, tile.rows, at);
+#pragma unroll
+    for (int m = 0; m < R; ++m) {
+      const float step = steps[m];
       float dy = d_o[m], xs = 0.f;
       if constexpr (!FOLD) xs = x[m];
-      by_raw[m] = dstep_of(raw, p.softplus);
       if (gated) {
         const float zs = z[m], s = sigmoidf_(zs), g = zs * s;
         by_y[m] = dy * fmaf(g, 1.f - s, s);
@@ -217,7 +223,7 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
           const float ds = fmaf(own[3], du, dd * kLn2) * by_raw[m];
           dx.store(tile, m, fmaf(own[0], du, skip * own[1]));
           ddelta.store(tile, m, ds);
-          if (first + 4 * m + at.q < at.end) dbias += ds, dskip = fmaf(own[1], own[3], dskip);
+          dbias += ds, dskip = fmaf(own[1], own[3], dskip);
           // (the next tile's rows, into registers that the last tokens' factors have left)
           if (m == R - 1 && first > at.first) load(first - T);
         }
