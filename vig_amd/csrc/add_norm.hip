@@ -6,7 +6,7 @@
 // Memory bounds it: a row lies in the registers of 32, 64 or 256 threads between its sums.  The backward's threads keep their columns' sums of the rows
 // that they come by, a workgroup adds up its threads' and leaves a row of partial sums.
 //
-// Measured, 25088 x 768, bf16 rows beside an fp32 residual stream: forward 47 us, 4.9 TB/s, backward 63, 4.9 (a large copy: 5.4), sums of the parameters' gradients 4.
+// Measured, 25088 x 768, bf16 rows beside an fp32 residual stream: forward 45 us, 5.1 TB/s, backward 63, 4.9 (a large copy: 5.4), sums of the parameters' gradients 4.
 #include "common.h"
 #include "launch.h"
 
@@ -69,8 +69,15 @@ __global__ __launch_bounds__(256) void add_norm_kernel(AddNorm p) {
   const long long row = (long long)blockIdx.x * kRows + threadIdx.x / G;
   const bool is = row < p.rows;  // (lanes of a missing row still take part in the sums)
   const long long base = (is ? row : 0) * p.C;
-  float s[NV][V];
+  float s[NV][V], w[NV][V], b[NV][V];
   float total = 0.f, none = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {  // (up to four pieces of the parameters on their way with the row; more would cost registers)
+    const int c = (lane + G * i) * V;
+    if (NV > 4 || c >= p.C) continue;
+    take<V>(w[i], p.weight + c);
+    if (p.bias) take<V>(b[i], p.bias + c);
+  }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (lane + G * i) * V;
@@ -103,11 +110,12 @@ __global__ __launch_bounds__(256) void add_norm_kernel(AddNorm p) {
   for (int i = 0; i < NV; ++i) {
     const int c = (lane + G * i) * V;
     if (c >= p.C) continue;
-    float w[V], b[V];
-    take<V>(w, p.weight + c);
-    if (p.bias) take<V>(b, p.bias + c);
+    if (NV > 4) {
+      take<V>(w[i], p.weight + c);
+      if (p.bias) take<V>(b[i], p.bias + c);
+    }
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[i][e] = fmaf(s[i][e] * rstd, w[e], p.bias ? b[e] : 0.f);
+    for (int e = 0; e < V; ++e) s[i][e] = fmaf(s[i][e] * rstd, w[i][e], p.bias ? b[i][e] : 0.f);
     give<V>(static_cast<TX*>(p.y) + base + c, s[i]);
   }
 }
@@ -202,10 +210,12 @@ __global__ __launch_bounds__(256) void add_norm_bwd_kernel(AddNorm p) {
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -5; }
 
-// Eight elements a thread at once where rows begin on 16 bytes, else one; as few threads a row as hold it.
-template <typename F> int by_width(bool wide, int C, F f) {
+// Eight elements a thread at once where rows begin on 16 bytes, else one; as few threads a row as hold it, but a workgroup for each of few rows (16 of 999: 3.8 us for 6.3).
+template <typename F> int by_width(bool wide, long long rows, int C, F f) {
 #define VIG_NORM_CASE(V, NV, G) f(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, G>{})
+  const bool few = rows <= 1024;
   if (wide) {
+    if (few && C > 256 && C <= 2048) return VIG_NORM_CASE(8, 1, 256);
     if (C <= 256) return VIG_NORM_CASE(8, 1, 32);
     if (C <= 512) return VIG_NORM_CASE(8, 1, 64);
     if (C <= 1024) return VIG_NORM_CASE(8, 2, 64);
@@ -213,6 +223,7 @@ template <typename F> int by_width(bool wide, int C, F f) {
     if (C <= 4096) return VIG_NORM_CASE(8, 2, 256);
     return VIG_NORM_CASE(8, 8, 256);
   }
+  if (few && C > 64 && C <= 1024) return VIG_NORM_CASE(1, 4, 256);
   if (C <= 256) return VIG_NORM_CASE(1, 4, 64);
   if (C <= 1024) return VIG_NORM_CASE(1, 16, 64);
   if (C <= 4096) return VIG_NORM_CASE(1, 16, 256);
@@ -233,7 +244,7 @@ bool wide(const AddNorm& p) {
 
 int launch_add_norm(const AddNorm& p, hipStream_t stream) {
   return by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {
-    return by_width(wide(p), p.C, [&](auto v, auto nv, auto g) {
+    return by_width(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
       hipLaunchKernelGGL((add_norm_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)((p.rows + 256 / g - 1) / (256 / g))), dim3(256), 0, stream, p);
       return launched();
     });
@@ -250,7 +261,7 @@ int launch_add_norm_bwd(AddNorm& p, void* workspace, hipStream_t stream) {
   p.each = (p.rows + want - 1) / want;
   const long long groups = (p.rows + p.each - 1) / p.each;
   const int rc = by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {
-    return by_width(wide(p), p.C, [&](auto v, auto nv, auto g) {
+    return by_width(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
       hipLaunchKernelGGL((add_norm_bwd_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)groups), dim3(256), 0, stream, p);
       return launched();
     });
