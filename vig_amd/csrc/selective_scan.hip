@@ -5,14 +5,14 @@
 //   o_t = (sum_n C_t[n] h_t[n] + skip x_t) silu(z_t)
 //
 // Decays go by channel and state, so that no product of matrices is in it: for each number of state and token an exponential (two issue slots), a product for its exponent, one for
-// the decay and two multiply-adds.  The vector pipe bounds it: 500 instructions a wave, tile of 16 tokens, 16 channels and 16 states, 320 of them these (64 of them double), the others
-// the steps' softplus (80), gates, addresses and sums over the lane rows.  Sums over n stay in a lane for its four states, and h never leaves its registers.
+// the decay and two multiply-adds.  The vector pipe bounds it: 466 instructions a wave, tile of 16 tokens, 16 channels and 16 states, 320 of them these (64 of them double), the others
+// the steps' softplus, gates, addresses and sums over the lane rows.  Sums over n stay in a lane for its four states, and h never leaves its registers.
 //
 // Sequences go through uncut where they give every compute unit a workgroup; else in chunks of tokens: a launch folds each (the state that it leaves from nothing, and the sum of its
 // steps, which is all that a decay over it takes), and the chunks are joined by the walk itself or, many of them, by a launch in between.
 //
-// Measured, bf16, 16 states, gate: 128 x 196 x 768 86 us (4.6 M numbers of state a us; the rows alone, 156 MB, 29 at the rate of a copy; vector pipe 83 % busy, 6 waves a SIMD), 65536 x 1024
-// fold 229, join 10, walk 305.  Tried: the products s x B as outer products of the matrix cores (16 blocks of 4 x 4): 88 cycles for 84 beside the arithmetic of a token,
+// Measured, bf16, 16 states, gate: 128 x 196 x 768 83 us (3.7 M numbers of state a us; the rows alone, 156 MB, 29 at the rate of a copy; vector pipe 84 % busy, 6 waves a SIMD), 65536 x 1024
+// fold 216, join 10, walk 295.  Tried: the products s x B as outer products of the matrix cores (16 blocks of 4 x 4): 88 to 90 cycles for 84 beside the arithmetic of a token,
 // which they do not run beside.  A softplus of fewer instructions for bf16 rows: no gain, and states of less precision.
 #include "selective_scan.h"
 

@@ -7,12 +7,12 @@
 //
 // The forward kept the states that enter each tile of tokens.  A wave goes through its tiles against the walk: from the kept state forward again, with a and p of all of the
 // tile's tokens left in registers (one exponential a number of state, as in the forward), then back.
-// The vector pipe bounds it: 1440 instructions a tile of 16 tokens, 16 channels and 16 states, 830 of them the two walks, 256 the sums of dB and dC over the channels of a lane row, which
+// The vector pipe bounds it: 1424 instructions a tile of 16 tokens, 16 channels and 16 states, 830 of them the two walks, 256 the sums of dB and dC over the channels of a lane row, which
 // go on over a workgroup's four waves through LDS and over workgroups by a launch behind (four waves: 2 bytes of partial sums a channel and token).  Two waves a SIMD have 256
 // registers, 128 of them a and p.  Gradients of A, the skip and the bias stay in registers along the tokens; a launch adds up the sequences'.
 //
-// Measured, bf16, 16 states, gate: 128 x 196 x 768 278 to 307 us (the clock goes down under it), 50 at the rate of a copy for the rows; vector pipe 81 % busy.  Tiles of 8 tokens at three waves a
-// SIMD: 345, kept states of twice the size.  Sums of the partial gradients 9, of the parameters' 6.
+// Measured, bf16, 16 states, gate: 128 x 196 x 768 266 to 302 us (the clock goes down under it), 50 at the rate of a copy for the rows; vector pipe 82 % busy.  Tiles of 8 tokens at three waves a
+// SIMD: 359 for 345, kept states of twice the size.  Sums of the partial gradients 9, of the parameters' 6.
 #include "selective_scan.h"
 
 namespace vig {
