@@ -108,3 +108,25 @@ def test_same_bits_again():
         return (y.detach(), s.detach(), *torch.autograd.grad([y, s], list(given.values()), [torch.ones_like(y), torch.ones_like(s)]))
 
     assert all(torch.equal(a, b) for a, b in zip(run(), run()))
+
+
+@pytest.mark.parametrize("rows", [511, 512, 513, 1023, 1024, 1025])
+@pytest.mark.parametrize("C", [256, 257, 513, 520, 768, 1024, 1025, 2048])
+def test_lone_rows(rows, C):
+    """Where a row goes from a workgroup of its own to a wave, for rows in whole pieces and others; the backward keeps its form on both sides."""
+    announce(f"add and layer norm {rows} rows of {C}")
+    check(make(rows + C, (rows,), C, BF16, BF16), grads=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_of_the_summands_lie_apart(dtype):
+    """x and the residual get the same gradient where their types are alike, and neither changes with the other's."""
+    announce(f"add and layer norm, gradients of both summands, {dtype}")
+    t = make(3, (4,), 64, dtype, dtype)
+    x, residual = t["x"].requires_grad_(), t["residual"].requires_grad_()
+    y, total = vig_amd.add_layernorm(x, t["weight"], t["bias"], residual=residual, prenorm=True)
+    torch.autograd.backward([y, total], [torch.randn_like(y), torch.randn_like(total)])
+    assert torch.equal(x.grad, residual.grad)
+    before = residual.grad.clone()
+    x.grad.mul_(2)
+    assert torch.equal(residual.grad, before)

@@ -210,12 +210,14 @@ __global__ __launch_bounds__(256) void add_norm_bwd_kernel(AddNorm p) {
 
 int launched() { return hipGetLastError() == hipSuccess ? 0 : -5; }
 
-// Eight elements a thread at once where rows begin on 16 bytes, else one; as few threads a row as hold it, but a workgroup for each of few rows (16 of 999: 3.8 us for 6.3).
-template <typename F> int by_width(bool wide, long long rows, int C, F f) {
+// Eight elements a thread at once where rows begin on 16 bytes, else one; as few threads a row as hold it.  LONE: a workgroup for each row, where a wave a row would leave the chip to few of
+// them, each with several pieces to go through.  us of the forward, bf16, a wave / a workgroup: wide, 16 x 768 3.64 / 3.35, 512 x 768 3.90 / 3.70, 1024 x 768 4.09 / 4.19, 16 x 2048 5.08 / 3.38,
+// 16 x 384 (one piece a lane) 3.04 / 3.30; narrow, 16 x 999 8.86 / 4.21, 1024 x 385 5.79 / 4.48, 4096 x 385 7.54 / 8.68, 16 x 100 3.22 / 3.26.  The backward's workgroups take eight rows,
+// four at a time in waves: one at a time takes 11.1 for 6.4 (16 x 384), 11.9 for 7.8 (16 x 768).
+template <bool LONE, typename F> int by_width(bool wide, long long rows, int C, F f) {
 #define VIG_NORM_CASE(V, NV, G) f(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, G>{})
-  const bool few = rows <= 1024;
   if (wide) {
-    if (few && C > 256 && C <= 2048) return VIG_NORM_CASE(8, 1, 256);
+    if (LONE && rows <= 512 && C > 512 && C <= 2048) return VIG_NORM_CASE(8, 1, 256);
     if (C <= 256) return VIG_NORM_CASE(8, 1, 32);
     if (C <= 512) return VIG_NORM_CASE(8, 1, 64);
     if (C <= 1024) return VIG_NORM_CASE(8, 2, 64);
@@ -223,7 +225,7 @@ template <typename F> int by_width(bool wide, long long rows, int C, F f) {
     if (C <= 4096) return VIG_NORM_CASE(8, 2, 256);
     return VIG_NORM_CASE(8, 8, 256);
   }
-  if (few && C > 64 && C <= 1024) return VIG_NORM_CASE(1, 4, 256);
+  if (LONE && rows <= 1024 && C > 256 && C <= 1024) return VIG_NORM_CASE(1, 4, 256);
   if (C <= 256) return VIG_NORM_CASE(1, 4, 64);
   if (C <= 1024) return VIG_NORM_CASE(1, 16, 64);
   if (C <= 4096) return VIG_NORM_CASE(1, 16, 256);
@@ -244,7 +246,7 @@ bool wide(const AddNorm& p) {
 
 int launch_add_norm(const AddNorm& p, hipStream_t stream) {
   return by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {
-    return by_width(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
+    return by_width<true>(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
       hipLaunchKernelGGL((add_norm_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)((p.rows + 256 / g - 1) / (256 / g))), dim3(256), 0, stream, p);
       return launched();
     });
@@ -261,7 +263,7 @@ int launch_add_norm_bwd(AddNorm& p, void* workspace, hipStream_t stream) {
   p.each = (p.rows + want - 1) / want;
   const long long groups = (p.rows + p.each - 1) / p.each;
   const int rc = by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {
-    return by_width(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
+    return by_width<false>(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
       hipLaunchKernelGGL((add_norm_bwd_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)groups), dim3(256), 0, stream, p);
       return launched();
     });
