@@ -111,6 +111,14 @@ def test_sequences_that_are_not_cut(N):
     check(make(4, 1100, 18, 3, N, dtype=F32, padded=True), reverse=True, grads=True)
 
 
+@pytest.mark.parametrize("batch,L,N", [(199, 200, 16), (200, 200, 16), (127, 120, 5), (128, 120, 5), (299, 259, 16), (300, 259, 16), (320, 257, 40), (351, 256, 7), (352, 256, 7), (255, 255, 33)])
+def test_where_sequences_begin_to_go_through_whole(batch, L, N):
+    """Forward and backward on either side of their borders: both cut, only the backward (300 to 351 sequences of 16 channels, 16 states), neither."""
+    announce(f"selective scan, {batch} sequences of {L} tokens, {N} states")
+    check(make(batch + N, batch, L, 16, N, state=True), final=True, grads=True)
+    check(make(batch + N + 1, batch, L, 16, N, dtype=BF16), reverse=True, grads=True)
+
+
 @pytest.mark.parametrize("L", [1000, 4097])
 def test_long(L):
     announce(f"selective scan of {L} tokens")

@@ -41,13 +41,21 @@ template <typename F> int by_states(int CN, F f) {
     default: return f(std::integral_constant<int, 16>{});
   }
 }
-// Chunks of tokens, 16 at least: none where sequences and channels leave no compute unit without a workgroup.  Chunks cost a second walk without the outputs, two thirds of the first; what they
-// give is four workgroups a unit, whose waves hide one another's waits.  65536 x 1024, fold and walk: four a unit 229 + 305 us, two 248 + 367, one 331 + 536.  So with 256 groups of channels
-// already four chunks cost as much as one; 32 x 12 groups of 196 tokens, 64 states: one chunk 103 us, two 140.
-inline void cut_chunks(SelScanArgs& p) {
+// Groups of channels from which on sequences go through whole.  Chunks cost a second walk without the outputs and whole tiles; what they give is four workgroups a compute unit, whose waves hide
+// one another's waits, the more the fewer states a lane has to work on and the fewer waves there are else (the backward's).  Time of cut to whole sequences at 168, 192, 216, 252, 288, 336, 384
+// groups:  196 tokens, 16 states, forward 1.05 1.03 1.27 1.28 1.08 1.27 1.31, with the backward .91 .90 1.08 1.15 1.00 1.13 1.21;   4 states .89 .89 1.05 1.04 .98 1.07 1.13, .83 .84 .97 1.02 .91 1.02 1.03.
+// 1024 tokens, 4 states, forward .48 .54 .64 .65 .74 .79 .96;  16: .67 .76 .91 .91 .97 1.02 1.16;  64: .74 .88 1.07 1.07 1.04 1.05 1.21;  with the backward .54 .60 .70 .70 .77 .84 .94,
+// .62 .70 .84 .86 .88 .94 1.09, .63 .72 .85 .88 .89 .91 1.14.  (320 to 4096 tokens: alike.)  64 tokens, 144 and 192 groups, 4, 16, 64 states: forward 1.10 1.10, 1.23 1.23, 1.39 1.44.
+inline int whole_from(const SelScanArgs& p, bool back) {
+  const int CN = scan_states(p.N);
+  if (p.L < 256) return p.L < 128 ? 128 : 200;
+  return back || CN <= 2 ? 352 : CN <= 4 ? 300 : 200;
+}
+// Chunks of tokens, 16 at least.  65536 x 1024, 16 states, fold and walk: four workgroups a unit 229 + 305 us, two 248 + 367, one 331 + 536.
+inline void cut_chunks(SelScanArgs& p, bool back) {
   p.of_group = p.D / p.G, p.blocks = (p.of_group + kScanBlock - 1) / kScanBlock;
   const long long groups = (long long)p.batch * p.G * p.blocks;
-  const long long want = groups >= kScanUnits ? 1 : std::min<long long>(4 * kScanUnits / groups, (p.L + 15) / 16);
+  const long long want = groups >= whole_from(p, back) ? 1 : std::min<long long>(4 * kScanUnits / groups, (p.L + 15) / 16);
   const int T = scan_tile(scan_states(p.N));
   p.chunk = (int)(((p.L + want - 1) / want + T - 1) / T * T);
   p.chunks = (p.L + p.chunk - 1) / p.chunk;

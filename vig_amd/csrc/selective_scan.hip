@@ -287,7 +287,7 @@ int launch_selective_scan_step(SelScanStep& p, hipStream_t stream) {
 
 int launch_selective_scan(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream) {
   const int CN = scan_states(p.N);
-  cut_chunks(p);
+  cut_chunks(p, false);
   if (!scan_fits(p)) return -95;
   p.ends = (float*)workspace;
   p.sums = p.ends + (size_t)p.batch * p.chunks * p.D * 4 * CN;
@@ -297,7 +297,7 @@ int launch_selective_scan(SelScanArgs& p, void* workspace, int io_dtype, hipStre
 size_t selective_scan_workspace(int batch, int L, int D, int N, int G) {
   SelScanArgs p{};
   p.batch = batch, p.L = L, p.D = D, p.N = N, p.G = G;
-  cut_chunks(p);
+  cut_chunks(p, false);
   return p.chunks > 1 ? sizeof(float) * (size_t)batch * p.chunks * D * (4 * scan_states(N) + 1) : 0;
 }
 size_t selective_scan_kept(int batch, int L, int D, int N) {

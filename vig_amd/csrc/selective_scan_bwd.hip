@@ -310,7 +310,7 @@ static int run_backward(const SelScanArgs& p, hipStream_t stream) {
 
 static size_t cut_workspace(SelScanArgs& p, void* workspace) {
   const int CN = scan_states(p.N);
-  cut_chunks(p);
+  cut_chunks(p, true);
   const size_t rows = (size_t)p.batch * p.chunks;
   float* at = (float*)workspace;
   p.ends = at, at += p.chunks > 1 ? rows * p.D * 4 * CN : 0;
