@@ -130,3 +130,10 @@ def test_gradients_of_the_summands_lie_apart(dtype):
     before = residual.grad.clone()
     x.grad.mul_(2)
     assert torch.equal(residual.grad, before)
+
+
+@pytest.mark.parametrize("rows,C", [(8192, 264), (8200, 257), (11999, 40), (12001, 40), (12001, 1032), (8193, 1501), (513, 4104)])
+def test_many_rows(rows, C):
+    """As many partial sums of the parameters' gradients as there are at most, for rows in whole pieces and others."""
+    announce(f"add and layer norm {rows} rows of {C}")
+    check(make(rows + C, (rows,), C, BF16, BF16), grads=True)

@@ -6,7 +6,7 @@
 // Memory bounds it: a row lies in the registers of 32, 64 or 256 threads between its sums.  The backward's threads keep their columns' sums of the rows
 // that they come by, a workgroup adds up its threads' and leaves a row of partial sums.
 //
-// Measured, 25088 x 768, bf16 rows beside an fp32 residual stream: forward 45 us, 5.1 TB/s, backward 63, 4.9 (a large copy: 5.4), sums of the parameters' gradients 4.
+// Measured, 25088 x 768, bf16 rows beside an fp32 residual stream: forward 45 us, 5.1 TB/s, backward 57, 5.4 (a large copy: 5.4), sums of the parameters' gradients 4.
 #include "common.h"
 #include "launch.h"
 
@@ -253,13 +253,18 @@ int launch_add_norm(const AddNorm& p, hipStream_t stream) {
   });
 }
 
-// Workgroups of the backward: enough to fill the chip, few enough that their partial sums are little beside the rows.
-static long long norm_groups(long long rows) { return std::max(1LL, std::min<long long>(512, rows / 8)); }
-size_t add_norm_bwd_workspace(long long rows, int C) { return sizeof(float) * norm_groups(rows) * 2 * (size_t)C; }
+// Workgroups of the backward: enough to fill the chip, few enough that their partial sums are little beside the rows.  us with 256 / 512 / 1024 of them, bf16:  8192 x 768 21.9 / 16.9 / 17.7,
+// 25088 x 768 51.4 / 33.7 / 29.6, 65536 x 384 77.7 / 45.9 / 34.7, 30000 x 4096 394 / 235 / 179;  four pieces a lane, which leave room for half as many: 20000 x 2048 83.8 / 65.1 / 74.2;
+// long rows: 9000 x 8192 248 / 263 / 294, 16384 x 16384 794 / 828 / 880;  one element at a time: 9000 x 999 69.8 / 45.3 / 36.1, 20000 x 1501 261 / 141 / 81.
+static long long norm_groups(long long rows, int C, bool wide) {
+  const long long most = C > 4096 ? 256 : wide && ((C > 1024 && C <= 2048) || rows < 12000) ? 512 : 1024;
+  return std::max(1LL, std::min(most, rows / 8));
+}
+size_t add_norm_bwd_workspace(long long rows, int C) { return sizeof(float) * std::max(norm_groups(rows, C, true), norm_groups(rows, C, false)) * 2 * (size_t)C; }
 
 int launch_add_norm_bwd(AddNorm& p, void* workspace, hipStream_t stream) {
   p.parts = p.dparams ? (float*)workspace : nullptr;
-  const long long want = norm_groups(p.rows);
+  const long long want = norm_groups(p.rows, p.C, wide(p));
   p.each = (p.rows + want - 1) / want;
   const long long groups = (p.rows + p.each - 1) / p.each;
   const int rc = by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {

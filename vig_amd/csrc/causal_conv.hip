@@ -6,7 +6,7 @@
 // Memory bounds it: a thread slides over a run of tokens of a few channels, so that a row is read once but for the W - 1 rows on a run's edges, which come out of a
 // cache.  Sixteen threads side by side take 256 bytes of a row (128 in the backward, which has twice the registers to hold).
 //
-// Measured, bf16, 4 taps, silu: 65536 x 1024 53 us, 5.1 TB/s (a large copy: 5.4); 128 x 196 x 768 forward 22, backward 34 (116 MB, part of it in the 256 MB cache; 35 operations an
+// Measured, bf16, 4 taps, silu: 65536 x 1024 53 us, 5.1 TB/s (a large copy: 5.4); 128 x 196 x 768 forward 19, backward 33 (116 MB, part of it in the 256 MB cache; 35 operations an
 // element beside it), sums of the weights' gradient 4.
 #include "common.h"
 #include "launch.h"
@@ -364,10 +364,12 @@ template <int BYTES, typename F> int by_case(const CausalConv& p, int io_dtype, 
     return whole(p, BYTES, 4) ? f(float{}, std::integral_constant<int, BYTES / 4>{}, w) : f(float{}, std::integral_constant<int, 1>{}, w);
   });
 }
-// Runs of tokens: as long as leaves four workgroups a compute unit (and `most`), so that few rows on their edges are read twice.
+// Runs of tokens: as long as leaves two workgroups a compute unit (and `most`), so that few rows on their edges are read twice and few partial sums are left.  us, one / two / four a unit:
+// forward of 128 x 196 x 768 17.9 / 18.0 / 19.7, of 4096 x 1024 6.6 / 7.0 / 7.0;  backward of 32 x 196 x 768 17.0 / 16.5 / 21.0, of 64 x 196 x 768 21.5 / 21.3 / 24.4, of 16384 x 1024
+// 37.4 / 29.0 / 29.0.
 void cut_runs(CausalConv& p, int V, int most) {
   p.blocks = (p.D + kConvLanes * V - 1) / (kConvLanes * V);
-  const long long tokens = (long long)p.B * p.blocks * p.L / (kConvRuns * 1024);
+  const long long tokens = (long long)p.B * p.blocks * p.L / (kConvRuns * 512);
   p.run = (int)std::max(4LL, std::min<long long>(most, tokens));
   p.groups = (int)(((p.L + p.run - 1) / p.run + kConvRuns - 1) / kConvRuns);
   p.run = std::max(1, (p.L + p.groups * kConvRuns - 1) / (p.groups * kConvRuns));  // (the runs of a group of alike length)
