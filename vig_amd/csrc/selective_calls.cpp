@@ -353,7 +353,8 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& b, const std::optional<Tensor>& residual, double eps) {
     const NormOut r = norm_forward(x.contiguous(), w, held(b), residual ? residual->contiguous() : Tensor(), eps, true);
     ctx->save_for_backward({r.sum, r.stats, w});
-    ctx->saved_data["flags"] = std::vector<int64_t>{(int64_t)x.scalar_type(), b.has_value(), residual.has_value()};
+    // (edges are counted over the tensors that are there)
+    ctx->saved_data["flags"] = std::vector<int64_t>{(int64_t)x.scalar_type(), b.has_value(), residual ? (b ? 3 : 2) : -1};
     ctx->set_materialize_grads(false);
     if (residual) return {r.y, r.sum};
     return {r.y};
@@ -371,7 +372,9 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
     TORCH_CHECK(dy.scalar_type() == type && dy.numel() == sum.numel() && (!dsum.defined() || dsum.scalar_type() == sum.scalar_type()), "gradients must match the outputs in shape and dtype");
     const bool want = ctx->needs_input_grad(1) || (flags[1] && ctx->needs_input_grad(2));
     Tensor dx = at::empty(sum.sizes(), sum.options().dtype(type)), dres, params, ws, dw, db;
-    if (type != sum.scalar_type()) dres = at::empty(sum.sizes(), sum.options());
+    // (two who want the gradient of one sum get a buffer each: behind views of leaves autograd keeps both as they are, and adds the next pass's to one memory twice)
+    const bool second = flags[2] >= 0 && ctx->needs_input_grad(flags[2]);
+    if (type != sum.scalar_type() || (second && ctx->needs_input_grad(0))) dres = at::empty(sum.sizes(), sum.options());
     size_t need = 0;
     if (want) {
       params = at::empty({2 * (int64_t)C}, sum.options().dtype(at::kFloat));
@@ -385,7 +388,7 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
       dw = params.narrow(0, 0, C);
       if (flags[1]) db = params.narrow(0, C, C);
     }
-    if (flags[2] && !dres.defined()) dres = dx.alias();
+    if (second && !dres.defined()) dres = std::move(dx);
     refuse_second({&dx, &dw, &db, &dres}, "add_layernorm has no second derivative");
     return {dx, dw, db, dres, Tensor()};
   }

@@ -487,16 +487,18 @@ class _AddLayerNorm(torch.autograd.Function):
         dtype, has_bias, has_residual = ctx.kinds
         dy = dy if dy is not None else torch.zeros(total.shape, dtype=dtype, device=total.device)
         params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        # (two who want the gradient of one sum get a buffer each: behind views of leaves autograd keeps both as they are, and adds the next pass's to one memory twice)
+        both = has_residual and ctx.needs_input_grad[0] and ctx.needs_input_grad[3]
         call = torch.ops.vig_amd.add_layernorm_bwd if ops.observed() else _norm_backward
-        dx, d_residual, dparams = call(total, stats, w, dy, d_total, params)
+        dx, d_residual, dparams = call(total, stats, w, dy, d_total, params, both)
         C = w.numel()
-        if has_residual and dtype == total.dtype:
-            d_residual = dx
+        if has_residual and dtype == total.dtype and not both:
+            dx, d_residual = (dx, None) if ctx.needs_input_grad[0] else (None, dx)
         return dx, dparams[:C] if params else None, dparams[C:] if params and has_bias else None, d_residual if has_residual else None, None
 
 
-def _norm_backward(total, stats, w, dy, d_total, want_params):
-    """(dx, the residual's gradient where its type is another, weight's and bias's gradient behind one another)"""
+def _norm_backward(total, stats, w, dy, d_total, want_params, both=False):
+    """(dx, the residual's gradient where its type is another or both are wanted, weight's and bias's gradient behind one another)"""
     lib = _lib.load()
     ops._check_cuda(total, stats, w, dy, d_total)
     total, dy = total.contiguous(), dy.contiguous()
@@ -504,7 +506,7 @@ def _norm_backward(total, stats, w, dy, d_total, want_params):
     C = total.shape[-1]
     rows = total.numel() // C
     dx = torch.empty(total.shape, dtype=dy.dtype, device=total.device)
-    d_residual = torch.empty_like(total) if total.dtype != dy.dtype else None
+    d_residual = torch.empty_like(total) if both or total.dtype != dy.dtype else None
     dparams = torch.empty(2 * C, dtype=torch.float32, device=total.device) if want_params else None
     need = lib.vig_add_layernorm_bwd_workspace(rows, C) if want_params else 0
     ws = torch.empty(need, dtype=torch.uint8, device=total.device) if need else None
@@ -593,7 +595,8 @@ def _norm_operator(x, w, b, residual, eps):
     return y, total if residual is not None else _or_empty(x, None)[0], stats
 
 
-@_operator("add_layernorm_bwd(Tensor sum, Tensor stats, Tensor weight, Tensor dy, Tensor? d_sum, bool params) -> (Tensor, Tensor, Tensor)",
-           lambda total, stats, w, dy, d_total, params: (_packed(dy), _packed(total) if total.dtype != dy.dtype else _numbers(total, 0), _numbers(total, 2 * w.numel() if params else 0)))
-def _norm_bwd_operator(total, stats, w, dy, d_total, params):
-    return _or_empty(total, *_norm_backward(total, stats, w, dy, d_total, params))
+@_operator("add_layernorm_bwd(Tensor sum, Tensor stats, Tensor weight, Tensor dy, Tensor? d_sum, bool params, bool both=False) -> (Tensor, Tensor, Tensor)",
+           lambda total, stats, w, dy, d_total, params, both=False: (_packed(dy), _packed(total) if both or total.dtype != dy.dtype else _numbers(total, 0),
+                                                                     _numbers(total, 2 * w.numel() if params else 0)))
+def _norm_bwd_operator(total, stats, w, dy, d_total, params, both=False):
+    return _or_empty(total, *_norm_backward(total, stats, w, dy, d_total, params, both))
