@@ -855,7 +855,8 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
  * *_strides: elements between batch elements and between tokens (B, C: and between groups), NULL: dense; channels, and a group's states, lie side by side.  Distances
  * between tokens up to 262144.  Tensors begin on any element; `kept` and the workspaces on 16 bytes.
  * kept: NULL, or vig_selective_scan_kept(...) bytes of states for vig_selective_scan_bwd.  Sums and states are held in fp32, in an order fixed by the sizes.
- * Outputs may not overlap inputs.  VIG_ENOTSUP past 2^24 tokens, 2^18 channels, or 2^32 threads of a launch (batch times channels times N / 4 from about 2^32 on).
+ * Outputs may not overlap inputs.  VIG_ENOTSUP past 2^24 tokens, 2^18 channels, 2^18 numbers of all groups of a token's B, or 2^24 - 1 workgroups of a launch: of the walk
+ * batch * G * ceil(D / G / 64); with `kept`, and in the backward, of the sum of dB and dC batch * L * G * N / 512, N rounded up to 4, 8, 16, 32 or 64.  (Workspaces of such sizes: 0 bytes.)
  */
 size_t vig_selective_scan_fwd_workspace(int batch, int L, int D, int N, int G);
 size_t vig_selective_scan_kept(int batch, int L, int D, int N);

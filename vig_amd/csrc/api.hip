@@ -1210,10 +1210,17 @@ static int selective_arguments(vig::SelScanArgs& p, const void* x, const void* d
   return VIG_OK;
 }
 
-size_t vig_selective_scan_fwd_workspace(int batch, int L, int D, int N, int G) { return selective_sizes_ok(batch, L, D, N, G) ? vig::selective_scan_workspace(batch, L, D, N, G) : 0; }
+// ... and the launches too: the forward's, of one that keeps states for a backward (or the backward's own) the sum of dB and dC as well
+static bool selective_launches_ok(int batch, int L, int D, int N, int G, bool back, bool training) {
+  return selective_sizes_ok(batch, L, D, N, G) && vig::selective_scan_fits(batch, L, D, N, G, back, training);
+}
+
+size_t vig_selective_scan_fwd_workspace(int batch, int L, int D, int N, int G) {
+  return selective_launches_ok(batch, L, D, N, G, false, false) ? vig::selective_scan_workspace(batch, L, D, N, G) : 0;
+}
 size_t vig_selective_scan_kept(int batch, int L, int D, int N) { return selective_sizes_ok(batch, L, D, N, 1) ? vig::selective_scan_kept(batch, L, D, N) : 0; }
 size_t vig_selective_scan_bwd_workspace(int batch, int L, int D, int N, int G) {
-  return selective_sizes_ok(batch, L, D, N, G) ? vig::selective_scan_bwd_workspace(batch, L, D, N, G) : 0;
+  return selective_launches_ok(batch, L, D, N, G, true, true) ? vig::selective_scan_bwd_workspace(batch, L, D, N, G) : 0;
 }
 
 int vig_selective_scan_fwd(const void* x, const void* delta, const float* A, const void* B, const void* C, const float* D_skip, const void* z, const float* delta_bias,
@@ -1228,6 +1235,7 @@ int vig_selective_scan_fwd(const void* x, const void* delta, const float* A, con
   for (const void* t : {x, delta, B, C, z})
     if (o == t) return VIG_EINVAL;
   if (final_state && final_state == initial_state) return VIG_EINVAL;
+  if (!selective_launches_ok(batch, L, D, N, G, false, kept != nullptr)) return VIG_ENOTSUP;
   const size_t need = vig::selective_scan_workspace(batch, L, D, N, G);
   if (need && (!workspace || workspace_bytes < need)) return VIG_ENOSPC;
   p.o = o, p.hT = final_state, p.kept = kept;
@@ -1254,6 +1262,7 @@ int vig_selective_scan_bwd(const void* x, const void* delta, const float* A, con
       if (outs[i] == outs[k]) return VIG_EINVAL;
   }
   if (!on_element(d_o, element_size(io_dtype)) || !on_element(d_final_state, 4)) return VIG_EINVAL;
+  if (!selective_launches_ok(batch, L, D, N, G, true, true)) return VIG_ENOTSUP;
   if (!workspace || workspace_bytes < vig::selective_scan_bwd_workspace(batch, L, D, N, G)) return VIG_ENOSPC;
   p.kept = const_cast<float*>(kept), p.d_o = {d_o, (long long)L * D, D, 0}, p.dhT = d_final_state;
   p.dx = dx, p.ddelta = ddelta, p.dB = dB, p.dC = dC, p.dz = dz, p.dparams = dA_dD_dbias, p.dh0 = d_initial_state;

@@ -168,6 +168,8 @@ struct SelScanArgs {
   int softplus, reverse;  // (not bool: a flag of one byte is compared into a lane mask, and what it selects ends up in vector registers)
 };
 constexpr int kScanStates = 64;  // most of a channel
+// whether its launches (back: the backward's; training: also the sum of dB and dC) stay below 2^32 threads; to be asked before one
+bool selective_scan_fits(int batch, int L, int D, int N, int G, bool back, bool training);
 size_t selective_scan_workspace(int batch, int L, int D, int N, int G);
 size_t selective_scan_kept(int batch, int L, int D, int N);
 size_t selective_scan_bwd_workspace(int batch, int L, int D, int N, int G);

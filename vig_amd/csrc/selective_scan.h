@@ -60,10 +60,13 @@ inline void cut_chunks(SelScanArgs& p, bool back) {
   p.chunk = (int)(((p.L + want - 1) / want + T - 1) / T * T);
   p.chunks = (p.L + p.chunk - 1) / p.chunk;
 }
-// whether every launch stays below 2^32 threads
-inline bool scan_fits(const SelScanArgs& p) {
-  const long long NP = 4 * scan_states(p.N), most = 0xffffffLL;
-  return (long long)p.batch * p.G * p.blocks * p.chunks <= most && (long long)p.batch * p.D * NP / 256 < most && (long long)p.batch * p.G * p.L / 128 * NP < most;
+// workgroups of the sum of dB and dC, of four numbers a thread
+inline long long shared_groups(const SelScanArgs& p) { return ((long long)p.batch * p.G * p.L * 2 * scan_states(p.N) + 255) / 256; }
+// Whether every launch stays below 2^32 threads: the walk's (and the folding's), and in training the sum of dB and dC over the workgroups.  (Chunks that take a launch to be joined, more than 32
+// of them, are those of fewer than 32 workgroups' channels: 500 workgroups.)
+inline bool scan_fits(const SelScanArgs& p, bool training) {
+  const long long most = 0xffffffLL;
+  return (long long)p.batch * p.G * p.blocks * p.chunks <= most && (!training || shared_groups(p) <= most);
 }
 // Few chunks are joined by those who come behind them (entering), many by a launch of their own: each reads all in front of it, 68 bytes a channel of 16 states.
 constexpr int kFewChunks = 32;

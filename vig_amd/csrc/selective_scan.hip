@@ -288,12 +288,17 @@ int launch_selective_scan_step(SelScanStep& p, hipStream_t stream) {
 int launch_selective_scan(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream) {
   const int CN = scan_states(p.N);
   cut_chunks(p, false);
-  if (!scan_fits(p)) return -95;
   p.ends = (float*)workspace;
   p.sums = p.ends + (size_t)p.batch * p.chunks * p.D * 4 * CN;
   return by_states(CN, [&](auto cn) { return io_dtype == VIG_BF16 ? run_forward<uint16_t, cn>(p, stream) : run_forward<float, cn>(p, stream); });
 }
 
+bool selective_scan_fits(int batch, int L, int D, int N, int G, bool back, bool training) {
+  SelScanArgs p{};
+  p.batch = batch, p.L = L, p.D = D, p.N = N, p.G = G;
+  cut_chunks(p, back);
+  return scan_fits(p, training);
+}
 size_t selective_scan_workspace(int batch, int L, int D, int N, int G) {
   SelScanArgs p{};
   p.batch = batch, p.L = L, p.D = D, p.N = N, p.G = G;

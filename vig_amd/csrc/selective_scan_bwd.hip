@@ -300,8 +300,7 @@ static int run_backward(const SelScanArgs& p, hipStream_t stream) {
     if (rc) return rc;
   }
   hipLaunchKernelGGL((selective_scan_bwd_kernel<S, CN, false>), grid, block, 0, stream, p);
-  const long long n = (long long)p.batch * p.G * p.L * 8 * CN;
-  hipLaunchKernelGGL((selective_shared_kernel<S>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, p, 4 * CN);
+  hipLaunchKernelGGL((selective_shared_kernel<S>), dim3((unsigned)shared_groups(p)), dim3(256), 0, stream, p, 4 * CN);
   if (hipGetLastError() != hipSuccess) return -5;
   vig_sum_jobs sums{};
   if (!put_off(sums, p.params, p.dparams, p.batch * p.chunks, (long long)p.D * (p.N + 2), false)) return -22;
@@ -322,7 +321,6 @@ static size_t cut_workspace(SelScanArgs& p, void* workspace) {
 
 int launch_selective_scan_bwd(SelScanArgs& p, void* workspace, int io_dtype, hipStream_t stream) {
   cut_workspace(p, workspace);
-  if (!scan_fits(p)) return -95;
   return by_states(scan_states(p.N), [&](auto cn) { return io_dtype == VIG_BF16 ? run_backward<uint16_t, cn>(p, stream) : run_backward<float, cn>(p, stream); });
 }
 size_t selective_scan_bwd_workspace(int batch, int L, int D, int N, int G) {

@@ -60,7 +60,8 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     front of the first token of the walk and behind its last.  reverse: the walk goes from the last token to the first (the other direction of a bidirectional mixer, without
     turning anything round).  A token whose step is 0 (delta of -infinity in front of the softplus) and whose x is finite leaves the state as it is: padding.  A value that is not
     finite stays in its sequence's channel, where every later output is not finite then, and in gradients of the rows that channels share.
-    x, delta, z, B, C may be columns of wider rows (read in place).  Up to 2^24 tokens of 2^18 channels.  States and sums are held in fp32, in an order fixed by the sizes.
+    x, delta, z, B, C may be columns of wider rows (read in place).  Up to 2^24 tokens of 2^18 channels, G N up to 2^18, batch G ceil(D / G / 64) below 2^24; with gradients batch L G N
+    (N rounded up to a power of two, 4 at least) below 2^33.  States and sums are held in fp32, in an order fixed by the sizes.
     Differentiable in every tensor; the forward then keeps the state in front of every 16th token (8th above 16, 4th above 32 states), 4 bytes a channel and token at 16 states."""
     calls = _ext.calls()
     if calls is not None:  # one native call for what the kernels take; None: not of that kind
