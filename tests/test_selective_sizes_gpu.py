@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import vig_amd
+from vig_amd import _ext
 
 from . import selective_ref as R
 from .test_selective_gpu import BF16, make, roundings
@@ -30,3 +31,27 @@ def test_two_to_the_31_numbers_of_b():
         R.close(t[:1], want[name], size[name], n, name)
         for at in range(0, batch, 1024):
             assert bool((t[at:at + 1024] == t[:1]).all()), name
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_groups_far_apart_in_one_token(native, monkeypatch):
+    """One token's B and C, taken out of [B, G, L, N]: groups as far apart as a sequence is long."""
+    announce(f"selective scan, groups 2^19 elements apart, native {native}")
+    if not native:
+        monkeypatch.setattr(_ext, "calls", lambda: None)
+    t = make(23, 2, 1, 6, 16, G=2, state=True)
+    room = torch.randn(2, 2, 1 << 15, 16, device="cuda")
+    want = vig_amd.selective_scan(**t, output_final_state=True)
+    for k in "BC":
+        far = room.clone()[:, :, 77:78].permute(0, 2, 1, 3)
+        far.copy_(t[k])
+        assert far.stride(2) == 1 << 19
+        t[k] = far
+    got = vig_amd.selective_scan(**t, output_final_state=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        state = t["initial_state"].clone()
+        step = {k: t[k][:, 0] for k in ("x", "delta", "B", "C", "z")}
+        o = vig_amd.selective_scan_step(**step, A=t["A"], state=state, D=t["D"], delta_bias=t["delta_bias"], delta_softplus=True)
+    want, size = (R.scan(**t, mag=m) for m in (False, True))
+    R.close(o, want["o"][:, 0], size["o"][:, 0], roundings(t, 1), "o"), R.close(state, want["final"], size["final"], roundings(t, 1), "state")

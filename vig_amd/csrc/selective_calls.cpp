@@ -57,7 +57,8 @@ Tensor shared_rows(const Tensor& given, int64_t dims) {
   const Tensor t = given.dim() == dims ? given.unsqueeze(-2) : given;
   const int64_t G = t.size(-2), N = t.size(-1), apart = G > 1 ? (G - 1) * t.stride(-2) + N : N;
   if ((N > 1 && t.stride(-1) != 1) || (G > 1 && t.stride(-2) < N)) return t.contiguous();
-  return dims == 3 && t.size(1) > 1 && (t.stride(1) < apart || t.stride(1) > (1 << 18)) ? t.contiguous() : t;
+  const int64_t next = dims == 3 && t.size(1) > 1 ? t.stride(1) : apart;  // (a token alone is as far from the next as its groups reach)
+  return dims == 3 && (next < apart || next > (1 << 18)) ? t.contiguous() : t;
 }
 struct SharedStrides {  // batch element, token (where there is one), group
   long long v[3];

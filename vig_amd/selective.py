@@ -107,7 +107,8 @@ def _shared_rows(t, dims):
     if N > 1 and t.stride(-1) != 1:
         return t.contiguous()
     apart = (G - 1) * t.stride(-2) + N if G > 1 else N
-    if (G > 1 and t.stride(-2) < N) or (dims == 3 and t.shape[1] > 1 and not apart <= t.stride(1) <= 1 << 18):
+    # (a token alone is as far from the next as its groups reach)
+    if (G > 1 and t.stride(-2) < N) or (dims == 3 and not apart <= (t.stride(1) if t.shape[1] > 1 else apart) <= 1 << 18):
         return t.contiguous()
     return t
 
