@@ -102,7 +102,6 @@ struct Strides {
 };
 inline bool simple(const Tensor& t) { return t.defined() && t.is_cuda() && !t.unsafeGetTensorImpl()->is_python_dispatch() && t.layout() == at::kStrided; }
 
-
 // a tensor of forward-mode differentiation, whose tangent a launch would drop
 inline bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 inline bool records(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -120,6 +119,13 @@ inline void refuse_held_leaf(const Tensor& t) {
 // What was written behind autograd's back: tensors saved for a backward pass notice.
 inline void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// A flag's truth; what has none (a tensor of several numbers) raises its own error here, before anything is launched.
+inline bool truth(PyObject* o) {
+  const int t = PyObject_IsTrue(o);
+  if (t < 0) throw python_error();
+  return t != 0;
 }
 
 inline Tensor tensor_arg(PyObject* o) {

@@ -182,8 +182,8 @@ PyObject* selective_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 12, "selective_scan takes 12 arguments");
   if (!tensor_args(a, 9)) Py_RETURN_NONE;
   Scan s{tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]), tensor_arg(a[3]), tensor_arg(a[4]), tensor_arg(a[5]), tensor_arg(a[6]), tensor_arg(a[7]), tensor_arg(a[8]),
-         PyObject_IsTrue(a[9]) == 1, PyObject_IsTrue(a[10]) == 1};
-  const bool want = PyObject_IsTrue(a[11]) == 1;
+         truth(a[9]), truth(a[10])};
+  const bool want = truth(a[11]);
   const Given all = {&s.x, &s.delta, &s.A, &s.B, &s.C, &s.D, &s.z, &s.bias, &s.h0};
   if (!s.x.defined() || !s.B.defined() || !s.C.defined() || !scan_ok(s, 3) || observed() || any_dual(all)) Py_RETURN_NONE;
   if (recorded(all)) {
@@ -202,7 +202,7 @@ PyObject* selective_scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 10, "selective_scan_step takes 10 arguments");
   if (!tensor_args(a, 9)) Py_RETURN_NONE;
   Scan s{tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]), tensor_arg(a[3]), tensor_arg(a[4]), tensor_arg(a[5]), tensor_arg(a[6]), tensor_arg(a[7]), tensor_arg(a[8]),
-         PyObject_IsTrue(a[9]) == 1, false};
+         truth(a[9]), false};
   const Given all = {&s.x, &s.delta, &s.A, &s.B, &s.C, &s.D, &s.z, &s.bias, &s.h0};
   if (!s.x.defined() || !s.B.defined() || !s.C.defined() || !s.h0.defined() || !s.h0.is_contiguous() || !scan_ok(s, 2) || observed() || any_dual(all)) Py_RETURN_NONE;
   if (at::GradMode::is_enabled())
@@ -292,7 +292,7 @@ PyObject* causal_conv1d(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 7, "causal_conv1d takes 7 arguments");
   if (!tensor_args(a, 4)) Py_RETURN_NONE;
   const Tensor x = tensor_arg(a[0]), w = tensor_arg(a[1]), b = tensor_arg(a[2]), h0 = tensor_arg(a[3]);
-  const bool silu = PyObject_IsTrue(a[4]) == 1, reverse = PyObject_IsTrue(a[5]) == 1, want = PyObject_IsTrue(a[6]) == 1;
+  const bool silu = truth(a[4]), reverse = truth(a[5]), want = truth(a[6]);
   if (!x.defined() || !simple(x) || x.dim() != 3 || dtype_code(x) < 0 || !sizes_ok(x) || !taps_ok(w, x) || !numbers(b, x, {x.size(2)}) ||
       !fits(h0, x, x.scalar_type(), {x.size(0), w.size(-1) - 1, x.size(2)}) || observed())
     Py_RETURN_NONE;
@@ -313,7 +313,7 @@ PyObject* causal_conv1d_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   TORCH_CHECK_TYPE(n == 5, "causal_conv1d_step takes 5 arguments");
   if (!tensor_args(a, 4)) Py_RETURN_NONE;
   const Tensor x = tensor_arg(a[0]), w = tensor_arg(a[1]), h = tensor_arg(a[2]), b = tensor_arg(a[3]);
-  const bool silu = PyObject_IsTrue(a[4]) == 1;
+  const bool silu = truth(a[4]);
   if (!x.defined() || !h.defined() || !simple(x) || x.dim() != 2 || dtype_code(x) < 0 || !sizes_ok(x) || !taps_ok(w, x) || !numbers(b, x, {x.size(1)}) ||
       !fits(h, x, x.scalar_type(), {x.size(0), w.size(-1) - 1, x.size(1)}) || !h.is_contiguous() || observed())
     Py_RETURN_NONE;
