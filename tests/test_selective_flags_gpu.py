@@ -1,4 +1,4 @@
-"""Flags of the selective mixer's calls that are neither true nor false."""
+"""What is neither true nor false, and who speaks in a refusal."""
 import pytest
 import torch
 
@@ -25,3 +25,13 @@ def test_a_flag_without_a_truth(call, flag, native, monkeypatch):
     with pytest.raises(RuntimeError, match="ambiguous"):
         getattr(vig_amd, call)(**t, **{flag: torch.tensor([True, False])})
     assert before is None or torch.equal(t["state"], before)
+
+
+@pytest.mark.parametrize("call", ["selective_scan", "causal_conv1d", "add_layernorm"])
+def test_a_refused_capture_names_its_call(call, monkeypatch):
+    announce(f"{call}, leaves in a capture without the native calls")
+    monkeypatch.setattr(_ext, "calls", lambda: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    leaves = {k: t.requires_grad_() for k, t in CALLS[call]("cuda").items()}
+    with pytest.raises(RuntimeError, match=f"^{call}: .*capture"):
+        getattr(vig_amd, call)(**leaves)

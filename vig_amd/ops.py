@@ -1169,7 +1169,7 @@ def _gated_scan(x, g, initial_state, both, want_final):
     return o, h
 
 
-def _refuse_held_leaves(*ts):
+def _refuse_held_leaves(*ts, by="gated_scan"):
     """Before leaves of the caller are taken into a captured call in another form than their own (the native call looks at what it is given by itself): a leaf whose
     gradient would be added up on the default stream ends the process there.  Which stream that is only the native module can tell."""
     leaves = [t for t in ts if t is not None and t.is_cuda and t.requires_grad and t.is_leaf]
@@ -1177,7 +1177,7 @@ def _refuse_held_leaves(*ts):
         return
     calls = _ext.calls()
     if calls is None:
-        raise RuntimeError("gated_scan: a gradient of leaves is recorded in a capture by the native calls only (vig_amd/lib/vig_host.so); detach the leaves or run without gradients")
+        raise RuntimeError(f"{by}: a gradient of leaves is recorded in a capture by the native calls only (vig_amd/lib/vig_host.so); detach the leaves or run without gradients")
     calls.refuse_held_leaves(*leaves)
 
 

@@ -75,7 +75,7 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     _same_type(x, delta=delta, B=B, C=C, z=z)
     given = (x, delta, A, B, C, D, z, delta_bias, initial_state)
     _refuse_tangents("selective_scan", *given)
-    _refuse_held_leaves(*given)
+    _refuse_held_leaves(*given, by="selective_scan")
     batch, L, width = x.shape
     N = B.shape[-1]
     A, D, delta_bias = _number("A", A, (width, N), x), _number("D", D, (width,), x), _number("delta_bias", delta_bias, (width,), x)
@@ -277,7 +277,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
         raise ValueError("x must be [B,L,D]")
     given = (x, weight, bias, initial_state)
     _refuse_tangents("causal_conv1d", *given)
-    _refuse_held_leaves(*given)
+    _refuse_held_leaves(*given, by="causal_conv1d")
     batch, L, width = x.shape
     w = _taps(weight, width)
     W = w.shape[1]
@@ -422,7 +422,7 @@ def add_layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     ops._check_cuda(x, weight, bias, residual)
     given = (x, weight, bias, residual)
     _refuse_tangents("add_layernorm", *given)
-    _refuse_held_leaves(*given)
+    _refuse_held_leaves(*given, by="add_layernorm")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MOST_WIDTH:
         raise ValueError(f"x must be [..., C] with C from 1 to {MOST_WIDTH}")
     if not eps >= 0:
