@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void add_norm_kernel(AddNorm p) {
   __shared__ float board[2][8];
   Sum<G> sum{board};
   const int lane = threadIdx.x % G;
-  const long long row = (long long)blockIdx.x * kRows + threadIdx.x / G;
+  const long long row = p.first + (long long)blockIdx.x * kRows + threadIdx.x / G;
   const bool is = row < p.rows;  // (lanes of a missing row still take part in the sums)
   const long long base = (is ? row : 0) * p.C;
   float s[NV][V], w[NV][V], b[NV][V];
@@ -244,11 +244,16 @@ bool wide(const AddNorm& p) {
 
 }  // namespace
 
-int launch_add_norm(const AddNorm& p, hipStream_t stream) {
+int launch_add_norm(AddNorm& p, hipStream_t stream) {
+  constexpr long long most = 1LL << 23;  // rows of a launch: below 2^32 threads where a row takes a workgroup
   return by_types(p.io_dtype, p.sum_dtype, [&](auto tx, auto ts) {
     return by_width<true>(wide(p), p.rows, p.C, [&](auto v, auto nv, auto g) {
-      hipLaunchKernelGGL((add_norm_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)((p.rows + 256 / g - 1) / (256 / g))), dim3(256), 0, stream, p);
-      return launched();
+      for (p.first = 0; p.first < p.rows; p.first += most) {
+        const long long groups = (std::min(most, p.rows - p.first) + 256 / g - 1) / (256 / g);
+        hipLaunchKernelGGL((add_norm_kernel<decltype(tx), decltype(ts), v, nv, g>), dim3((unsigned)groups), dim3(256), 0, stream, p);
+        if (const int rc = launched()) return rc;
+      }
+      return 0;
     });
   });
 }

@@ -209,13 +209,13 @@ struct AddNorm {
   const float *weight, *bias;
   void *sum, *y, *dx, *d_residual;
   float *stats, *dparams, *parts;                // stats: mean and rstd of each row; dparams: gradients of weight and bias [2, C]
-  long long rows, each;                          // each: rows of a workgroup
+  long long rows, first, each;                   // first: of a launch of the forward; each: rows of a workgroup of the backward
   int C;
   float eps;
   int io_dtype, sum_dtype;
 };
 constexpr int kNormWidth = 16384;
-int launch_add_norm(const AddNorm& p, hipStream_t stream);
+int launch_add_norm(AddNorm& p, hipStream_t stream);
 size_t add_norm_bwd_workspace(long long rows, int C);
 int launch_add_norm_bwd(AddNorm& p, void* workspace, hipStream_t stream);
 
