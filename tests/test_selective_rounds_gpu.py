@@ -11,14 +11,31 @@ from .test_causal_conv_gpu import check as check_conv, make as make_conv
 from .test_selective_gpu import BF16, F32, check as check_scan, make as make_scan, roundings
 from .util import announce
 
-
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def gate_terms(monkeypatch):
+    """The magnitude of dz by the terms of silu'(z) = s + z s (1 - s), s = 1 / (1 + e^-z), and not by their sum: near z = -1.278 they cancel.  At z = -1.2784892 (one of 21546 gates of 513
+    channels) s = 0.2178075, z s (1 - s) = -0.2178129 and silu' = -5.4e-6, while each term is rounded by up to U = 2^-24 of itself: 2 x 0.2178 U, 8 10^4 U of the sum, where roundings() counts
+    5604 of it.  (The kernel was 4.0e-10 off, 0.12 U of dy y (|s| + |z s (1 - s)|).)  As the other magnitudes are taken: every sum with absolute values in it."""
+    whole = R.scan
+
+    def scan(*args, mag=False, **given):
+        out = whole(*args, mag=mag, **given)
+        if mag and "dz" in out:
+            z = R.f64(given["z"])
+            s = torch.sigmoid(z)
+            out["dz"] = out["dz"] / R.dsilu(z).abs() * s * (1 + z.abs() * (1 - s))
+        return out
+
+    monkeypatch.setattr(R, "scan", scan)
 
 
 # 64 channels a workgroup, four workgroups' sums on their way together: 5, 6, 8, 9 and 12 of a group
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("width,N,G", [(257, 16, 1), (384, 16, 1), (512, 13, 1), (513, 5, 1), (768, 16, 1), (768, 40, 2), (1152, 3, 3)])
-def test_groups_of_many_channels(width, N, G, dtype):
+def test_groups_of_many_channels(width, N, G, dtype, gate_terms):
     announce(f"selective scan, {width} channels in {G} groups, N {N} {dtype}")
     check_scan(make_scan(31, 2, 21, width, N, G, dtype, state=True), final=True, grads=True)
 
