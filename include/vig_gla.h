@@ -850,11 +850,11 @@ int vig_gated_scan_step(const void* x, const void* g, float* state, void* o, int
  *
  * x, delta, z [batch, L, D], B, C [batch, L, G, N] (a group's for the D / G channels side by side), o dense, all of io_dtype; A [D, N], D_skip, delta_bias [D] fp32.
  * D_skip, z (no gate), delta_bias may be NULL.  initial_state (NULL: zeros) and final_state (NULL: not wanted): fp32 [batch, D, N], in front of the first and
- * behind the last token of the walk.  reverse: the walk goes from token L - 1 to token 0.  A token with a step of 0 (delta of -infinity in front of the softplus) and a
- * finite x leaves the state as it is (padding).  N up to 64.
+ * behind the last token of the walk.  reverse: the walk goes from token L - 1 to token 0.  A token with a step of 0 (delta of -infinity in front of the softplus), a finite x and a
+ * finite B leaves the state as it is (padding).  N up to 64.
  * *_strides: elements between batch elements and between tokens (B, C: and between groups), NULL: dense; channels, and a group's states, lie side by side.  Distances
- * between tokens up to 262144.  Tensors begin on any element; `kept` and the workspaces on 16 bytes.
- * kept: NULL, or vig_selective_scan_kept(...) bytes of states for vig_selective_scan_bwd.  Sums and states are held in fp32, in an order fixed by the sizes.
+ * between tokens (of one token alone: its groups' reach) up to 262144.  Tensors begin on any element; `kept` and the workspaces on 16 bytes.
+ * kept: NULL, or vig_selective_scan_kept(...) bytes of states for vig_selective_scan_bwd: a channel and token 1, 2 or 4 bytes up to 4, 8 or 16 states, 16 up to 32, 64 up to 64.  Sums and states are held in fp32, in an order fixed by the sizes.
  * Outputs may not overlap inputs.  VIG_ENOTSUP past 2^24 tokens, 2^18 channels, 2^18 numbers of all groups of a token's B, or 2^24 - 1 workgroups of a launch: of the walk
  * batch * G * ceil(D / G / 64); with `kept`, and in the backward, of the sum of dB and dC batch * L * G * N / 512, N rounded up to 4, 8, 16, 32 or 64.  (Workspaces of such sizes: 0 bytes.)
  */
@@ -887,12 +887,13 @@ int vig_selective_scan_step(const void* x, const void* delta, const float* A, co
  *
  * x [B, L, D] with x_strides (batch element, token; NULL: dense), weight [D, W] and bias [D] (NULL: none) fp32, y dense of io_dtype.  initial_state (NULL: zeros) holds the W - 1
  * rows in front of the first token, final_state (NULL: not wanted) takes the last W - 1 rows: [B, W - 1, D] of io_dtype in the order of the walk, which goes from the last
- * token to the first where `reverse` is set.  Tensors begin on any element.  Limits as the scan's.  Outputs may not overlap inputs.
+ * token to the first where `reverse` is set.  Tensors begin on any element.  VIG_ENOTSUP past 2^24 tokens, 2^18 channels or 2^24 - 1 workgroups (of a sequence and 16 channels at least).
+ * Outputs may not overlap inputs.
  */
 int vig_causal_conv1d_fwd(const void* x, const float* weight, const float* bias, const void* initial_state, void* y, void* final_state, int B, int L, int D, int W,
                           const long long* x_strides, int silu, int reverse, int io_dtype, void* stream);
 /* dy dense, d_final_state (NULL: zeros) -> dx dense, d_initial_state (NULL: not wanted; also without an initial_state), dw_db: D W + D floats, the gradients of weight and bias
- * behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes. */
+ * behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes and by how the rows lie. */
 size_t vig_causal_conv1d_bwd_workspace(int B, int L, int D, int W);
 int vig_causal_conv1d_bwd(const void* x, const float* weight, const float* bias, const void* initial_state, const void* dy, const void* d_final_state, void* dx, void* d_initial_state,
                           float* dw_db, void* workspace, size_t workspace_bytes, int B, int L, int D, int W, const long long* x_strides, int silu, int reverse, int io_dtype,
@@ -911,7 +912,7 @@ int vig_causal_conv1d_step(const void* x, const float* weight, const float* bias
 int vig_add_layernorm_fwd(const void* x, const void* residual, const float* weight, const float* bias, void* sum, void* y, float* stats, long long rows, int C, float eps,
                           int io_dtype, int sum_dtype, void* stream);
 /* sum: as the forward left it (without a residual: x).  dy, and d_sum (NULL: zeros), what else came to the sum -> the sum's gradient as d_residual of sum_dtype and dx of io_dtype (each
- * may be NULL), dw_db: 2 C floats, the gradients of weight and bias behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes. */
+ * may be NULL), dw_db: 2 C floats, the gradients of weight and bias behind one another (NULL: not wanted, then no workspace either), added up in an order fixed by the sizes and by how the rows lie. */
 size_t vig_add_layernorm_bwd_workspace(long long rows, int C);
 int vig_add_layernorm_bwd(const void* sum, const float* stats, const float* weight, const void* dy, const void* d_sum, void* d_residual, void* dx, float* dw_db, void* workspace,
                           size_t workspace_bytes, long long rows, int C, int io_dtype, int sum_dtype, void* stream);

@@ -161,8 +161,10 @@ __global__ __launch_bounds__(64 * kScanWaves, FOLD ? 4 : 2) void selective_scan_
         const int i = at.j & 1, e = i + 2 * (at.j >> 2 & 1) + 4 * (at.j >> 3);
         board.v[which][token + e / NN][at.q * CN + state + e % NN] = i ? s[1] : s[0];
       };
-      // A last tile's tokens that are not there are left out by fours where a lane has eight states and more: the blocks that this makes need no spilled registers then (45 and 137 without).
-      // Up to four they are gone through with steps of 0: blocks cost 303 us for 278 there (128 x 196 x 768, 16 states, 13 tiles of which the last is a quarter).
+      // A last tile's tokens that are not there are left out by fours where a lane has eight states: the blocks that this makes need no spilled registers then (42 without).  A tile of sixteen
+      // states is four tokens, one of which is there, so that nothing is ever left out; the branches part the code all the same, and leave 51 (bf16) and 54 (fp32) spilled registers of 134.
+      // Up to four states the tokens are gone through with steps of 0: blocks cost 303 us for 278 there (128 x 196 x 768, 16 states, 13 tiles of which the last is a quarter; 2 spilled registers at
+      // four states, none below).
       constexpr bool kSkip = CN >= 8;
       float h[CN], a[T][CN], ph[T][CN], few[8], of_four[4];
       if constexpr (CN > 4) states.load(kept, p.kept, (size_t)at.b * tiles + first / T, p.D);

@@ -58,11 +58,12 @@ def selective_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     x, delta, z: [B,L,D] in fp32 or bf16, B and C of that type too: [B,L,N], or [B,L,G,N] for G groups of D/G channels side by side, N up to 64.  A [D,N] (its values <= 0), D and
     delta_bias [D]; without delta_softplus the steps are delta + delta_bias as they are (>= 0).  No D: nothing is skipped; no z: no gate.  initial_state and final_state: fp32 [B,D,N], in
     front of the first token of the walk and behind its last.  reverse: the walk goes from the last token to the first (the other direction of a bidirectional mixer, without
-    turning anything round).  A token whose step is 0 (delta of -infinity in front of the softplus) and whose x is finite leaves the state as it is: padding.  A value that is not
-    finite stays in its sequence's channel, where every later output is not finite then, and in gradients of the rows that channels share.
+    turning anything round).  A token whose step is 0 (delta of -infinity in front of the softplus) and whose x and B are finite leaves the state as it is: padding.  A value of x
+    or delta that is not finite stays in its sequence's channel, where every later output is not finite then, and in gradients of the rows that channels share; one of B or C reaches its group's.
     x, delta, z, B, C may be columns of wider rows (read in place).  Up to 2^24 tokens of 2^18 channels, G N up to 2^18, batch G ceil(D / G / 64) below 2^24; with gradients batch L G N
     (N rounded up to a power of two, 4 at least) below 2^33.  States and sums are held in fp32, in an order fixed by the sizes.
-    Differentiable in every tensor; the forward then keeps the state in front of every 16th token (8th above 16, 4th above 32 states), 4 bytes a channel and token at 16 states."""
+    Differentiable in every tensor; the forward then keeps the state in front of every 16th token (8th above 16, 4th above 32 states): 4 bytes a channel and token at 16 states, 16 at
+    32, 64 at 64."""
     calls = _ext.calls()
     if calls is not None:  # one native call for what the kernels take; None: not of that kind
         r = calls.selective_scan(x, delta, A, B, C, D, z, delta_bias, initial_state, delta_softplus, reverse, output_final_state)
@@ -412,7 +413,7 @@ def add_layernorm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 
     As rmsnorm(), with a mean and a bias, and a gradient for each.  x [..., C] in fp32 or bf16, C up to 16384; residual of its dtype or in fp32 (a residual stream in fp32 beside bf16
     branches), which is the dtype of the sum.  The sum as it is stored is what is normalised.  weight, bias [C].  Up to 2^24 rows.  Differentiable in every tensor, the weight's and
-    the bias's gradient added up in an order fixed by the sizes and by how the rows lie."""
+    the bias's gradient added up in an order fixed by the sizes and by how the rows lie; x's and the residual's are alike, each in memory of its own."""
     calls = _ext.calls()
     if calls is not None:
         r = calls.add_layernorm(x, weight, bias, residual, eps)
